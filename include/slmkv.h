@@ -230,6 +230,76 @@ slm_status slm_batch_attention_exact(slm_batch* batch, int32_t layer, const floa
  * kernel per layer. Same arguments as slm_batch_decode_layer. */
 slm_status slm_batch_decode_layer_exact(slm_batch* batch, int32_t layer, const float* d_query,
                                         const float* d_keys, const float* d_values, float* d_out);
+/* slm_batch_append_layer for models that normalise queries and keys per head
+ * (no reference counterpart), in one pass over the projections' outputs: each
+ * query and key head becomes x / sqrt(mean(x^2) + epsilon) * weight (d_query_norm
+ * and d_key_norm: head_dimension weights each, all heads alike), is rotated at
+ * its token's position when `rotate` is non-zero (as slm_batch_append_layer
+ * rotates keys), keys and values go into the cache, and the queries to
+ * d_query_out [sum(counts), q_heads, d], ready for an attention call with
+ * rotate_query 0. Rows are tokens in batch order; the strides (values from one
+ * row to the next, multiples of 4, at least a row's width) let the three be
+ * parts of one projection's output. d_query_out may be d_query when its rows are
+ * dense, and may overlap none of the inputs otherwise. Buffers are 16-byte
+ * aligned. Squares are summed in f32: a key whose square sum or normed value is
+ * not finite fails its sequence like a non-finite append, such a query is stored
+ * as NaN and fails in the attention. */
+slm_status slm_batch_append_layer_normed(slm_batch* batch, int32_t layer, const float* d_query,
+                                         const float* d_keys, const float* d_values,
+                                         int64_t query_stride, int64_t key_stride,
+                                         int64_t value_stride, const float* d_query_norm,
+                                         const float* d_key_norm, float epsilon, int32_t rotate,
+                                         float* d_query_out);
+/* slm_batch_prefill_attention for batches whose sequences share cached prefixes
+ * (slm_prefix_attach), decoded tokens and drafted ones among them: the blocks
+ * that several block tables begin with are read once for all their sequences,
+ * level by level where groups share more than the whole batch does, and the
+ * parts are joined. The result does not depend on what is shared beyond
+ * rounding; with nothing shared it is the batch's attention. f32 scores, sums
+ * and outputs for f32 and bf16 pools alike (operands enter the tensor cores in
+ * exact parts, not rounded to bf16). Same arguments; 16-byte aligned buffers that
+ * do not overlap. Meant for few new tokens a sequence: long prompts run faster
+ * through slm_batch_prefill_attention. A batch's first call plans it for all
+ * layers; plan buffers and the joined parts' scratch are allocated by the
+ * context's first call and grow when a call needs more (which waits for the
+ * device). */
+slm_status slm_batch_shared_attention(slm_batch* batch, int32_t layer, const float* d_query,
+                                      int32_t rotate_query, float* d_out);
+/* Probabilities of logit rows (no reference counterpart: greedy.rs takes the
+ * maximum): p_i = exp((x_i - max x) / T) / sum_j exp((x_j - max x) / T), and at
+ * T = 0 one at the first maximal logit (greedy.rs), zero elsewhere. d_logits:
+ * `rows` rows of vocab_size f32, logits_stride values apart; rows is the batch's
+ * number of tokens (slm_model_score) or of sequences (slm_model_prefill,
+ * slm_model_decode). d_temperatures: [rows], or NULL for 1. d_probabilities:
+ * [rows, vocab_size], dense; it may be d_logits when those are dense. A logit of
+ * -inf is a masked token. A row with a NaN or +inf logit, with nothing but -inf,
+ * or with a temperature that is negative or not finite becomes zeros and its
+ * sequence fails with SLM_ERR_NON_FINITE when the batch ends. */
+slm_status slm_batch_token_probabilities(slm_batch* batch, const float* d_logits, int32_t rows,
+                                         int32_t vocab_size, int64_t logits_stride,
+                                         const float* d_temperatures, float* d_probabilities);
+/* Verifies drafted tokens (no reference counterpart). Sequence i's count_i
+ * tokens in d_token_ids [sum(counts)] are its last accepted token and k_i =
+ * count_i - 1 drafts; row j of its rows in d_target [sum(counts), vocab_size]
+ * holds the model's probabilities after its token j. d_draft [sum(counts) - n,
+ * vocab_size] holds the probabilities each draft was drawn from, k_i rows a
+ * sequence; NULL when the drafts were chosen outright (q = 1 at the draft).
+ * d_uniforms [sum(counts)], in [0, 1): a sequence's first k_i decide its drafts,
+ * the last draws its next token. With u, p, q in 64 bits: draft j is accepted
+ * while u_j q_j(x) < p_j(x); d_accepted[i] is the number accepted before the
+ * first that is not. d_next_tokens[i] is drawn from max(p - q, 0) of the first
+ * rejected draft's row (from its p where nothing of that is left), or after the
+ * last draft from its row's p: the first token whose running sum of weights in
+ * token order exceeds u times their total. Outside [0, 1) u counts as the nearer
+ * end. Kept cache lengths: slm_seqs_truncate_all to base + 1 + accepted after
+ * the batch's end. A drafted token outside the vocabulary fails its sequence with
+ * SLM_ERR_INVALID_INPUT when the batch ends, a row it reads that is negative, not
+ * finite or all zero with SLM_ERR_NON_FINITE; both give 0 accepted and next token
+ * -1. vocab_size up to 655360. */
+slm_status slm_batch_verify_drafts(slm_batch* batch, int32_t vocab_size, const int32_t* d_token_ids,
+                                   const float* d_target, const float* d_draft,
+                                   const float* d_uniforms, int32_t* d_accepted,
+                                   int32_t* d_next_tokens);
 /* Closes the step: waits for its stream, and reports per sequence (h_status
  * may be NULL) 0 or SLM_ERR_NON_FINITE. A sequence whose appends were not
  * finite, whose attention met a score that is not finite (softmax.rs:17-22,
@@ -270,6 +340,12 @@ slm_status slm_prefix_publish(slm_ctx* ctx, int32_t seq_id, const uint32_t* h_to
                               int32_t n_tokens, int32_t* indexed_blocks);
 /* Number of blocks held by the index, and blocks free in the pool. */
 slm_status slm_pool_stats(const slm_ctx* ctx, int32_t* free_blocks, int32_t* indexed_blocks);
+/* Where the pool lies on the device, for readers that know its layout
+ * ([layer][block][kv_head][slot 0..15][head_dim], values of kv_dtype; block ids
+ * from slm_seq_blocks): the addresses of the K and V pools and the values of one
+ * layer. Valid until slm_destroy; order reads with the context's stream. */
+slm_status slm_pool_storage(const slm_ctx* ctx, int64_t* key_address, int64_t* value_address,
+                            int64_t* layer_values);
 /* Shuffles the free list with a seeded permutation, so that sequences get
  * scattered physical blocks. Pool must be unused. */
 slm_status slm_pool_shuffle(slm_ctx* ctx, uint64_t seed);
@@ -413,6 +489,12 @@ slm_status slm_model_decode(slm_model* model, slm_batch* batch, const int32_t* d
  * and d_next_token [n] (may be NULL). */
 slm_status slm_model_prefill(slm_model* model, slm_batch* batch, const int32_t* d_token_ids,
                              float* d_logits, int32_t* d_next_token);
+/* slm_model_prefill with every position projected to the vocabulary, for
+ * slm_batch_token_probabilities and slm_batch_verify_drafts: d_logits
+ * [sum(counts), vocab] (may be NULL) and d_next_token [sum(counts)] (the first
+ * maximal logit of each row; may be NULL). */
+slm_status slm_model_score(slm_model* model, slm_batch* batch, const int32_t* d_token_ids,
+                           float* d_logits, int32_t* d_next_token);
 /* ModelWeights::load (weights.rs:117-190) into a device model: a SafeTensors
  * file whose tensors are exactly the expected set for this config and the
  * context's layers and heads (names and shapes of weights.rs:344-378), every

@@ -86,6 +86,25 @@ struct StreamPlan {
   std::vector<int32_t> bucket_top, bucket_next, heads_left;  // pair packing (scratch)
 };
 
+// Plan of slm_batch_shared_attention: the tree of the batch's block tables
+// (an edge per run of blocks, with the sequences that hold it) and its cut
+// into CTAs.
+struct SharedPlan {
+  struct Edge {
+    int32_t parent, first_block, last_block;  // blocks [first, last)
+    int32_t seq0, seq1;                       // members order[seq0 .. seq1)
+  };
+  std::vector<int32_t> order;  // batch rows, members of an edge next to each other
+  std::vector<Edge> tree;
+  std::vector<int32_t> by_size;  // edges, longest runs first
+  std::vector<int32_t> token0;   // first token of order[i]
+  std::vector<SharedItem> items;
+  std::vector<SharedToken> tokens;
+  std::vector<SharedEdge> edges;
+  std::vector<int32_t> merge;
+  int64_t parts = 0;
+};
+
 // Device addresses of one uploaded step descriptor.
 struct StepDev {
   SeqEntry* seqs = nullptr;
@@ -116,6 +135,13 @@ struct slm_batch {
   std::vector<uint8_t> layer_done;
   StepDev dev;
   int32_t up_slot = 0;  // descriptor slot (its `consumed` event is recorded at the end)
+  // slm_batch_shared_attention: the plan, uploaded by the batch's first call.
+  bool shared_ready = false;
+  const SharedItem* d_items = nullptr;
+  const SharedToken* d_tokens = nullptr;
+  const SharedEdge* d_edges = nullptr;
+  const int32_t* d_merge = nullptr;
+  int32_t n_items = 0, n_merge = 0;
   // Submitted (slm_batch_submit): its status readback slot; per sequence
   // whether every layer advanced, and a rollback forced by an earlier batch
   // (poison_base >= 0: roll back to at most that length with poison_code).
@@ -187,6 +213,18 @@ struct slm_ctx {
     cudaEvent_t read[kUploadSlots] = {};     // the slot's outputs are on the host
     cudaStream_t h2d = nullptr;
   } io;
+  // slm_batch_shared_attention: plan staging, one buffer per descriptor slot
+  // (the batch's up_slot), and the parts of rows joined from several runs.
+  // Both are allocated at the first call and grown on demand.
+  struct SharedIo {
+    uint8_t* h[kUploadSlots] = {};
+    uint8_t* d[kUploadSlots] = {};
+    cudaEvent_t copied[kUploadSlots] = {};
+    size_t cap = 0;  // bytes a slot
+    float* part_acc = nullptr;
+    float2* part_ml = nullptr;
+    size_t part_cap = 0;  // row slots
+  } shared;
   size_t upd_cap = 0, copy_cap = 0;
 
   // host state
@@ -202,6 +240,7 @@ struct slm_ctx {
   std::vector<CopyJob> pending_copies;
   slm_batch* open_batch = nullptr;
   StreamPlan plan;  // decode plan of the open batch (reused storage)
+  SharedPlan shared_plan;  // reused storage
 
   PoolGeom geom() const {
     PoolGeom g{};
@@ -776,6 +815,13 @@ void destroy_device(slm_ctx* c) {
       if (ev) cudaEventDestroy(ev);
   }
   if (c->io.h2d) cudaStreamDestroy(c->io.h2d);
+  for (int k = 0; k < kUploadSlots; ++k) {
+    if (c->shared.h[k]) cudaFreeHost(c->shared.h[k]);
+    if (c->shared.d[k]) cudaFree(c->shared.d[k]);
+    if (c->shared.copied[k]) cudaEventDestroy(c->shared.copied[k]);
+  }
+  if (c->shared.part_acc) cudaFree(c->shared.part_acc);
+  if (c->shared.part_ml) cudaFree(c->shared.part_ml);
   if (c->copy_stream) cudaStreamDestroy(c->copy_stream);
   if (c->readback_stream) cudaStreamDestroy(c->readback_stream);
 }
@@ -1682,6 +1728,416 @@ slm_status slm_batch_prefill_attention(slm_batch* b, int32_t layer, const float*
   return SLM_OK;
 }
 
+// ---- a speculative step over shared prefixes ------------------------------------
+
+slm_status slm_batch_append_layer_normed(slm_batch* b, int32_t layer, const float* d_query,
+                                         const float* d_keys, const float* d_values,
+                                         int64_t query_stride, int64_t key_stride,
+                                         int64_t value_stride, const float* d_query_norm,
+                                         const float* d_key_norm, float epsilon, int32_t rotate,
+                                         float* d_query_out) {
+  if (!b) return SLM_ERR_INVALID_INPUT;
+  slm_ctx* ctx = b->ctx;
+  slm_status rc = batch_layer_check(b, layer);
+  if (rc) return rc;
+  const char* what = "normed append";
+  if (b->layer_done[layer])
+    return input_error(ctx, SLM_ERR_INVALID_INPUT, "batch", "layer %d was already appended", layer);
+  if (!d_query || !d_keys || !d_values || !d_query_norm || !d_key_norm || !d_query_out)
+    return input_error(ctx, SLM_ERR_INVALID_INPUT, what, "null tensor");
+  for (const void* p : {static_cast<const void*>(d_query), static_cast<const void*>(d_keys),
+                        static_cast<const void*>(d_values), static_cast<const void*>(d_query_norm),
+                        static_cast<const void*>(d_key_norm), static_cast<const void*>(d_query_out)})
+    if (!aligned16(p)) return input_error(ctx, SLM_ERR_INVALID_INPUT, what, "buffers must be 16-byte aligned");
+  const int64_t qw = static_cast<int64_t>(ctx->cfg.num_query_heads) * kHeadDim;
+  const int64_t kw = static_cast<int64_t>(ctx->cfg.num_key_value_heads) * kHeadDim;
+  if (query_stride < qw || key_stride < kw || value_stride < kw || query_stride % 4 || key_stride % 4 ||
+      value_stride % 4)
+    return input_error(ctx, SLM_ERR_INVALID_INPUT, what,
+                       "row strides must be multiples of 4 values and at least a row's width");
+  if (!(epsilon > 0.f) || !std::isfinite(epsilon))
+    return input_error(ctx, SLM_ERR_INVALID_INPUT, what, "epsilon must be finite and greater than zero");
+  const int64_t rows = b->total_tokens;
+  const size_t out_bytes = static_cast<size_t>(rows * qw) * sizeof(float);
+  auto span = [&](int64_t stride, int64_t width) { return static_cast<size_t>((rows - 1) * stride + width) * sizeof(float); };
+  const bool in_place = d_query_out == d_query && query_stride == qw;
+  if ((!in_place && ranges_overlap(d_query_out, out_bytes, d_query, span(query_stride, qw))) ||
+      ranges_overlap(d_query_out, out_bytes, d_keys, span(key_stride, kw)) ||
+      ranges_overlap(d_query_out, out_bytes, d_values, span(value_stride, kw)))
+    return input_error(ctx, SLM_ERR_INVALID_INPUT, what, "the output may not overlap the inputs");
+  rc = flush_excess(ctx, b->stream, 0, 0);  // the append reads the device block table
+  if (rc) return rc;
+  NormedAppendLaunch a{};
+  a.g = ctx->geom();
+  a.layer = layer;
+  a.seqs = b->dev.seqs;
+  a.n_seq = static_cast<int32_t>(b->seq_ids.size());
+  a.total_tokens = b->total_tokens;
+  a.q = d_query;
+  a.k = d_keys;
+  a.v = d_values;
+  a.q_stride = query_stride;
+  a.k_stride = key_stride;
+  a.v_stride = value_stride;
+  a.q_norm = d_query_norm;
+  a.k_norm = d_key_norm;
+  a.eps = epsilon;
+  a.rotate = rotate != 0;
+  a.q_out = d_query_out;
+  a.status = b->dev.status;
+  ctx->prev_decode_layer = -1;
+  CU(ctx, launch_normed_append(a, b->stream));
+  ++ctx->launches;
+  b->layer_done[layer] = 1;
+  for (size_t i = 0; i < b->seq_ids.size(); ++i)
+    ctx->seqs[b->seq_ids[i]].layer_len[layer] = b->base[i] + b->counts[i];
+  return SLM_OK;
+}
+
+namespace {
+// A run of blocks that several sequences share becomes an edge of its own from
+// this many blocks on: a shorter one costs more in joining than it saves.
+constexpr int32_t kSharedMinBlocks = 4;
+
+// The tree below the members order[lo, hi), which share their blocks before
+// `start` (edge `parent` ends there) and, beyond it, those before `probe`.
+void shared_tree(const slm_ctx* c, const slm_batch* b, SharedPlan& plan, int32_t parent, int32_t lo,
+                 int32_t hi, int32_t start, int32_t probe) {
+  // whole blocks before the new tokens; what the step writes is a sequence's own
+  auto limit = [&](int32_t i) { return b->base[i] / kBlockTokens; };
+  auto blocks = [&](int32_t i) { return c->seqs[b->seq_ids[i]].blocks.data(); };
+  auto key = [&](int32_t i) { return probe < limit(i) ? blocks(i)[probe] : -1; };
+  std::stable_sort(plan.order.begin() + lo, plan.order.begin() + hi,
+                   [&](int32_t x, int32_t y) { return key(x) < key(y); });
+  for (int32_t at = lo; at < hi;) {
+    const int32_t first = plan.order[at], block = key(first);
+    int32_t end = at + 1;
+    if (block >= 0)
+      while (end < hi && key(plan.order[end]) == block) ++end;
+    if (end - at == 1) {  // the sequence's own run, to its last new token
+      const int32_t stop = blocks_for(b->base[first] + b->counts[first]);
+      plan.tree.push_back({parent, start, stop, at, end});
+    } else {
+      int32_t same = limit(first);
+      for (int32_t i = at + 1; i < end; ++i) {
+        const int32_t o = plan.order[i], n = std::min(same, limit(o));
+        const int32_t *x = blocks(first), *y = blocks(o);
+        int32_t j = probe + 1;
+        while (j < n && x[j] == y[j]) ++j;
+        same = j;
+      }
+      if (same - start >= kSharedMinBlocks) {
+        plan.tree.push_back({parent, start, same, at, end});
+        shared_tree(c, b, plan, static_cast<int32_t>(plan.tree.size()) - 1, at, end, same, same);
+      } else {
+        shared_tree(c, b, plan, parent, at, end, start, same);
+      }
+    }
+    at = end;
+  }
+}
+
+void build_shared_plan(const slm_ctx* c, const slm_batch* b, SharedPlan& plan) {
+  const int32_t n = static_cast<int32_t>(b->seq_ids.size());
+  const int32_t Hkv = c->cfg.num_key_value_heads, G = c->group, tile = 16 / G;
+  plan.order.resize(n);
+  for (int32_t i = 0; i < n; ++i) plan.order[i] = i;
+  plan.tree.clear();
+  shared_tree(c, b, plan, -1, 0, n, 0, 0);
+
+  const int32_t n_edges = static_cast<int32_t>(plan.tree.size());
+  plan.token0.resize(n + 1);
+  std::vector<int32_t> row0(n);  // rows of the batch in batch order
+  for (int32_t i = 0, row = 0; i < n; ++i) {
+    row0[i] = row;
+    row += b->counts[i];
+  }
+  plan.token0[0] = 0;
+  for (int32_t i = 0; i < n; ++i) plan.token0[i + 1] = plan.token0[i] + b->counts[plan.order[i]];
+  plan.tokens.resize(b->total_tokens);
+  for (int32_t i = 0; i < n; ++i) {
+    const int32_t s = plan.order[i];
+    for (int32_t j = 0; j < b->counts[s]; ++j)
+      plan.tokens[plan.token0[i] + j] = SharedToken{row0[s] + j, b->base[s] + j, s, -1};
+  }
+  // Runs are cut so that the items fill the SMs (three CTAs each) about once,
+  // none shorter than what keeps a CTA's warps busy.
+  auto tiles_of = [&](const SharedPlan::Edge& e) {
+    return (plan.token0[e.seq1] - plan.token0[e.seq0] + tile - 1) / tile;
+  };
+  int64_t work = 0;
+  for (const auto& e : plan.tree)
+    work += static_cast<int64_t>(tiles_of(e)) * Hkv * (e.last_block - e.first_block);
+  const int64_t slots = 3ll * c->num_sms;
+  const int32_t least = shared_rows_min_blocks(c->cfg.kv_dtype == SLM_KV_BF16);
+  const int32_t room = static_cast<int32_t>(std::max<int64_t>(least, (work + slots - 1) / slots));
+  plan.edges.resize(n_edges);
+  plan.by_size.resize(n_edges);
+  plan.parts = 0;
+  plan.merge.clear();
+  for (int32_t i = 0; i < n_edges; ++i) {
+    const auto& e = plan.tree[i];
+    const int32_t nb = e.last_block - e.first_block;
+    SharedEdge& d = plan.edges[i];
+    d.parent = e.parent;
+    d.token0 = plan.token0[e.seq0];
+    d.n_splits = std::max(1, (nb + room - 1) / room);
+    d.n_rows = (plan.token0[e.seq1] - d.token0) * G;
+    plan.by_size[i] = i;
+    const bool own = e.seq1 - e.seq0 == 1;
+    const bool whole = own && e.parent < 0 && d.n_splits == 1;
+    d.part0 = -1;
+    if (!whole) {
+      d.part0 = static_cast<int32_t>(plan.parts);
+      plan.parts += static_cast<int64_t>(Hkv) * d.n_splits * d.n_rows;
+    }
+    if (own)
+      for (int32_t k = d.token0; k < plan.token0[e.seq1]; ++k) {
+        plan.tokens[k].edge = i;
+        if (!whole) plan.merge.push_back(k);
+      }
+  }
+  auto run_of = [&](int32_t i) {
+    const auto& e = plan.tree[i];
+    return (e.last_block - e.first_block + plan.edges[i].n_splits - 1) / plan.edges[i].n_splits;
+  };
+  std::sort(plan.by_size.begin(), plan.by_size.end(), [&](int32_t x, int32_t y) {
+    const int32_t a = run_of(x), c2 = run_of(y);
+    return a != c2 ? a > c2 : x < y;
+  });
+  plan.items.clear();
+  for (int32_t i : plan.by_size) {
+    const auto& e = plan.tree[i];
+    const SharedEdge& d = plan.edges[i];
+    const int32_t run = run_of(i), end = plan.token0[e.seq1];
+    const int32_t slot = b->seq_ids[plan.order[e.seq0]];
+    for (int32_t s = 0; s < d.n_splits; ++s)
+      for (int32_t h = 0; h < Hkv; ++h)
+        for (int32_t t = d.token0; t < end; t += tile) {
+          SharedItem it{};
+          it.slot = slot;
+          it.head = h;
+          it.token0 = t;
+          it.n_tokens = std::min(tile, end - t);
+          // an own run is read up to the tile's last token; shared ones whole
+          int32_t last = e.last_block;
+          it.mask_from = INT32_MAX;
+          if (plan.tokens[t].edge == i) {
+            last = std::min(last, plan.tokens[t + it.n_tokens - 1].pos / kBlockTokens + 1);
+            it.mask_from = plan.tokens[t].pos + 1;
+          }
+          it.first_block = e.first_block + s * run;
+          it.n_blocks = std::max(0, std::min(last, it.first_block + run) - it.first_block);
+          it.part = d.part0 < 0 ? -1
+                                : d.part0 + (h * d.n_splits + s) * d.n_rows + (t - d.token0) * G;
+          plan.items.push_back(it);
+        }
+  }
+}
+
+// Builds and uploads the open batch's plan (once a batch: its layers share it).
+slm_status shared_prepare(slm_batch* b) {
+  slm_ctx* c = b->ctx;
+  SharedPlan& plan = c->shared_plan;
+  build_shared_plan(c, b, plan);
+  if (plan.parts > INT32_MAX || plan.items.size() > static_cast<size_t>(INT32_MAX))
+    return input_error(c, SLM_ERR_INVALID_INPUT, "shared prefix attention", "the step has too many rows");
+  const size_t o_tokens = align16(plan.items.size() * sizeof(SharedItem));
+  const size_t o_edges = align16(o_tokens + plan.tokens.size() * sizeof(SharedToken));
+  const size_t o_merge = align16(o_edges + plan.edges.size() * sizeof(SharedEdge));
+  const size_t bytes = align16(o_merge + plan.merge.size() * sizeof(int32_t));
+  slm_ctx::SharedIo& io = c->shared;
+  const int k = b->up_slot;
+  if (bytes > io.cap) {
+    CU(c, cudaDeviceSynchronize());  // a slot may be in use
+    for (int i = 0; i < kUploadSlots; ++i) {
+      if (io.h[i]) cudaFreeHost(io.h[i]);
+      if (io.d[i]) cudaFree(io.d[i]);
+      io.h[i] = io.d[i] = nullptr;
+    }
+    c->device_bytes -= static_cast<int64_t>(io.cap) * kUploadSlots;
+    io.cap = 0;
+    const size_t cap = align16(bytes + bytes / 2 + 4096);
+    for (int i = 0; i < kUploadSlots; ++i) {
+      CU(c, cudaMallocHost(reinterpret_cast<void**>(&io.h[i]), cap));
+      CU(c, cudaMalloc(reinterpret_cast<void**>(&io.d[i]), cap));
+      if (!io.copied[i]) CU(c, cudaEventCreateWithFlags(&io.copied[i], cudaEventDisableTiming));
+    }
+    io.cap = cap;
+    c->device_bytes += static_cast<int64_t>(cap) * kUploadSlots;
+  }
+  if (static_cast<size_t>(plan.parts) > io.part_cap) {
+    CU(c, cudaDeviceSynchronize());
+    if (io.part_acc) cudaFree(io.part_acc);
+    if (io.part_ml) cudaFree(io.part_ml);
+    io.part_acc = nullptr;
+    io.part_ml = nullptr;
+    constexpr size_t kPart = kHeadDim * sizeof(float) + sizeof(float2);
+    c->device_bytes -= static_cast<int64_t>(io.part_cap * kPart);
+    io.part_cap = 0;
+    const size_t cap = static_cast<size_t>(plan.parts) + static_cast<size_t>(plan.parts) / 4;
+    CU(c, cudaMalloc(reinterpret_cast<void**>(&io.part_acc), cap * kHeadDim * sizeof(float)));
+    CU(c, cudaMalloc(reinterpret_cast<void**>(&io.part_ml), cap * sizeof(float2)));
+    io.part_cap = cap;
+    c->device_bytes += static_cast<int64_t>(cap * kPart);
+  }
+  CU(c, cudaEventSynchronize(io.copied[k]));  // the slot's last upload has left the pinned buffer
+  uint8_t* h = io.h[k];
+  memcpy(h, plan.items.data(), plan.items.size() * sizeof(SharedItem));
+  memcpy(h + o_tokens, plan.tokens.data(), plan.tokens.size() * sizeof(SharedToken));
+  memcpy(h + o_edges, plan.edges.data(), plan.edges.size() * sizeof(SharedEdge));
+  memcpy(h + o_merge, plan.merge.data(), plan.merge.size() * sizeof(int32_t));
+  // the kernels that last read the slot's device buffer are done
+  CU(c, cudaStreamWaitEvent(b->stream, c->up_batch.consumed[k], 0));
+  CU(c, cudaMemcpyAsync(io.d[k], h, bytes, cudaMemcpyHostToDevice, b->stream));
+  CU(c, cudaEventRecord(io.copied[k], b->stream));
+  b->d_items = reinterpret_cast<const SharedItem*>(io.d[k]);
+  b->d_tokens = reinterpret_cast<const SharedToken*>(io.d[k] + o_tokens);
+  b->d_edges = reinterpret_cast<const SharedEdge*>(io.d[k] + o_edges);
+  b->d_merge = reinterpret_cast<const int32_t*>(io.d[k] + o_merge);
+  b->n_items = static_cast<int32_t>(plan.items.size());
+  b->n_merge = static_cast<int32_t>(plan.merge.size());
+  b->shared_ready = true;
+  return SLM_OK;
+}
+}  // namespace
+
+slm_status slm_batch_shared_attention(slm_batch* b, int32_t layer, const float* d_query,
+                                      int32_t rotate_query, float* d_out) {
+  if (!b) return SLM_ERR_INVALID_INPUT;
+  slm_ctx* ctx = b->ctx;
+  slm_status rc = batch_layer_check(b, layer);
+  if (rc) return rc;
+  const char* what = "shared prefix attention";
+  if (!b->layer_done[layer])
+    return input_error(ctx, SLM_ERR_INVALID_INPUT, what, "layer %d must be appended before its attention", layer);
+  if (!d_query || !d_out) return input_error(ctx, SLM_ERR_INVALID_INPUT, what, "null tensor");
+  if (!aligned16(d_query) || !aligned16(d_out))
+    return input_error(ctx, SLM_ERR_INVALID_INPUT, what, "query and output buffers must be 16-byte aligned");
+  const size_t bytes = static_cast<size_t>(b->total_tokens) * ctx->cfg.num_query_heads * kHeadDim * sizeof(float);
+  if (ranges_overlap(d_query, bytes, d_out, bytes))
+    return input_error(ctx, SLM_ERR_INVALID_INPUT, what, "the output may not overlap the query");
+  rc = flush_excess(ctx, b->stream, 0, 0);  // the kernels read the device block table
+  if (rc) return rc;
+  if (!b->shared_ready && (rc = shared_prepare(b))) return rc;
+  SharedAttentionLaunch p{};
+  p.g = ctx->geom();
+  p.layer = layer;
+  p.q = d_query;
+  p.out = d_out;
+  p.rotate = rotate_query != 0;
+  p.status = b->dev.status;
+  p.items = b->d_items;
+  p.n_items = b->n_items;
+  p.tokens = b->d_tokens;
+  p.edges = b->d_edges;
+  p.merge_tokens = b->d_merge;
+  p.n_merge = b->n_merge;
+  p.part_acc = ctx->shared.part_acc;
+  p.part_ml = ctx->shared.part_ml;
+  ctx->prev_decode_layer = -1;
+  CU(ctx, launch_shared_attention(p, b->stream));
+  ctx->launches += p.n_merge ? 2 : 1;
+  return SLM_OK;
+}
+
+namespace {
+slm_status batch_open_check(slm_batch* b) {
+  if (b->ctx->open_batch != b)
+    return input_error(b->ctx, SLM_ERR_INVALID_INPUT, "batch", "the batch is not open");
+  return need_device(b->ctx);
+}
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+}  // namespace
+
+slm_status slm_batch_token_probabilities(slm_batch* b, const float* d_logits, int32_t rows,
+                                         int32_t vocab_size, int64_t logits_stride,
+                                         const float* d_temperatures, float* d_probabilities) {
+  if (!b) return SLM_ERR_INVALID_INPUT;
+  slm_ctx* ctx = b->ctx;
+  slm_status rc = batch_open_check(b);
+  if (rc) return rc;
+  const char* what = "token probabilities";
+  const int32_t n = static_cast<int32_t>(b->seq_ids.size());
+  if (!d_logits || !d_probabilities) return input_error(ctx, SLM_ERR_INVALID_INPUT, what, "null tensor");
+  if (!aligned4(d_logits) || !aligned4(d_temperatures) || !aligned4(d_probabilities))
+    return input_error(ctx, SLM_ERR_INVALID_INPUT, what, "buffers must be 4-byte aligned");
+  if (rows != n && rows != b->total_tokens)
+    return input_error(ctx, SLM_ERR_INVALID_INPUT, what,
+                       "%d rows are neither one a sequence (%d) nor one a token (%d)", rows, n, b->total_tokens);
+  if (vocab_size <= 0 || logits_stride < vocab_size)
+    return input_error(ctx, SLM_ERR_INVALID_INPUT, what,
+                       "the vocabulary must be positive and no wider than the logits' row stride");
+  const size_t in = static_cast<size_t>((rows - 1) * logits_stride + vocab_size) * sizeof(float);
+  const size_t out = static_cast<size_t>(rows) * vocab_size * sizeof(float);
+  const bool in_place = d_logits == d_probabilities && (rows == 1 || logits_stride == vocab_size);
+  if (!in_place && ranges_overlap(d_logits, in, d_probabilities, out))
+    return input_error(ctx, SLM_ERR_INVALID_INPUT, what, "the output may not overlap the logits");
+  if (d_temperatures &&
+      ranges_overlap(d_temperatures, static_cast<size_t>(rows) * sizeof(float), d_probabilities, out))
+    return input_error(ctx, SLM_ERR_INVALID_INPUT, what, "the output may not overlap the temperatures");
+  ProbabilitiesLaunch p{};
+  p.logits = d_logits;
+  p.logits_stride = logits_stride;
+  p.rows = rows;
+  p.vocab = vocab_size;
+  p.temperatures = d_temperatures;
+  p.out = d_probabilities;
+  p.seqs = b->dev.seqs;
+  p.n_seq = n;
+  p.status = b->dev.status;
+  ctx->prev_decode_layer = -1;
+  CU(ctx, launch_probabilities(p, b->stream));
+  ++ctx->launches;
+  return SLM_OK;
+}
+
+slm_status slm_batch_verify_drafts(slm_batch* b, int32_t vocab_size, const int32_t* d_token_ids,
+                                   const float* d_target, const float* d_draft, const float* d_uniforms,
+                                   int32_t* d_accepted, int32_t* d_next_tokens) {
+  if (!b) return SLM_ERR_INVALID_INPUT;
+  slm_ctx* ctx = b->ctx;
+  slm_status rc = batch_open_check(b);
+  if (rc) return rc;
+  const char* what = "draft verification";
+  if (!d_token_ids || !d_target || !d_uniforms || !d_accepted || !d_next_tokens)
+    return input_error(ctx, SLM_ERR_INVALID_INPUT, what, "null tensor");
+  for (const void* p : {static_cast<const void*>(d_token_ids), static_cast<const void*>(d_target),
+                        static_cast<const void*>(d_draft), static_cast<const void*>(d_uniforms),
+                        static_cast<const void*>(d_accepted), static_cast<const void*>(d_next_tokens)})
+    if (!aligned4(p)) return input_error(ctx, SLM_ERR_INVALID_INPUT, what, "buffers must be 4-byte aligned");
+  if (vocab_size <= 0 || vocab_size > verify_max_vocab())
+    return input_error(ctx, SLM_ERR_INVALID_INPUT, what, "vocabulary size %d is outside 1..=%lld", vocab_size,
+                       static_cast<long long>(verify_max_vocab()));
+  VerifyLaunch p{};
+  p.seqs = b->dev.seqs;
+  p.n_seq = static_cast<int32_t>(b->seq_ids.size());
+  p.vocab = vocab_size;
+  p.token_ids = d_token_ids;
+  p.target = d_target;
+  p.draft = d_draft;
+  p.uniforms = d_uniforms;
+  p.accepted = d_accepted;
+  p.next_tokens = d_next_tokens;
+  p.status = b->dev.status;
+  ctx->prev_decode_layer = -1;
+  CU(ctx, launch_verify(p, b->stream));
+  ++ctx->launches;
+  return SLM_OK;
+}
+
+slm_status slm_pool_storage(const slm_ctx* ctx, int64_t* key_address, int64_t* value_address,
+                            int64_t* layer_values) {
+  if (!ctx || !key_address || !value_address || !layer_values) return SLM_ERR_INVALID_INPUT;
+  slm_ctx* c = const_cast<slm_ctx*>(ctx);  // for the error message
+  slm_status rc = need_device(c);
+  if (rc) return rc;
+  *key_address = static_cast<int64_t>(reinterpret_cast<uintptr_t>(ctx->k_pool));
+  *value_address = static_cast<int64_t>(reinterpret_cast<uintptr_t>(ctx->v_pool));
+  *layer_values = ctx->geom().layer_elems;
+  return SLM_OK;
+}
+
 slm_status slm_batch_decode_layer_exact(slm_batch* b, int32_t layer, const float* d_query,
                                         const float* d_keys, const float* d_values, float* d_out) {
   if (!b) return SLM_ERR_INVALID_INPUT;
@@ -1857,7 +2313,9 @@ void resolve_oldest(slm_ctx* ctx) {
     int32_t code = SLM_OK;
     if (dev != SLM_OK) code = dev;
     else if (b->poison_base[i] >= 0) code = b->poison_code[i];
-    else if (st & (kStatusNonFinite | kStatusNonFiniteScore)) code = SLM_ERR_NON_FINITE;
+    else if (st & (kStatusNonFinite | kStatusNonFiniteScore | kStatusLogits | kStatusProbability))
+      code = SLM_ERR_NON_FINITE;
+    else if (st & kStatusToken) code = SLM_ERR_INVALID_INPUT;
     else if (!b->complete[i]) code = SLM_ERR_INVALID_INPUT;
     b->codes[i] = code;
     if (code != SLM_OK && b->first == SLM_OK) {
@@ -1877,10 +2335,17 @@ void resolve_oldest(slm_ctx* ctx) {
   if (b->first == SLM_ERR_NON_FINITE && !(first_bits & kStatusNonFinite) &&
       (first_bits & kStatusNonFiniteScore))  // softmax.rs:17-22 through attention.rs:731
     b->msg = "invalid input for softmax: all input values must be finite";
+  else if (b->first == SLM_ERR_NON_FINITE && !(first_bits & kStatusNonFinite) && (first_bits & kStatusLogits))
+    b->msg = "invalid input for token probabilities: a row's logits give no distribution";
+  else if (b->first == SLM_ERR_NON_FINITE && !(first_bits & kStatusNonFinite) &&
+           (first_bits & kStatusProbability))
+    b->msg = "invalid input for draft verification: a row's probabilities give no distribution";
   else if (b->first == SLM_ERR_NON_FINITE)
     b->msg = "invalid input for KV cache: all appended key/value values must be finite";
   else if (dev != SLM_OK)
     b->msg = dev_msg;
+  else if (b->first == SLM_ERR_INVALID_INPUT && (first_bits & kStatusToken))
+    b->msg = "invalid input for draft verification: token id outside the vocabulary";
   else if (b->first == SLM_ERR_INVALID_INPUT)
     b->msg = "invalid input for model cached decode: all cache layers must advance by exactly "
              "one step";

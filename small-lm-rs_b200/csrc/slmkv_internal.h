@@ -73,7 +73,17 @@ struct CopyJob {
 // Device status words (per batch sequence, and one per context).
 // kStatusNonFinite: appended K/V not finite (kv_cache.rs:192-197);
 // kStatusNonFiniteScore: an attention score not finite (softmax.rs:17-22).
-enum : int32_t { kStatusNonFinite = 1, kStatusNonFiniteScore = 2 };
+// kStatusLogits: a logit row that gives no distribution (NaN, +inf, nothing
+// finite, a bad temperature); kStatusToken: a drafted token outside the
+// vocabulary; kStatusProbability: probabilities that are negative, not finite
+// or all zero.
+enum : int32_t {
+  kStatusNonFinite = 1,
+  kStatusNonFiniteScore = 2,
+  kStatusLogits = 4,
+  kStatusToken = 8,
+  kStatusProbability = 16
+};
 // Device error word bits: a bounded wait expired; a block table held an id
 // outside the pool; a kernel found its shared-memory layout misaligned.
 enum : int32_t { kErrTimeout = 1, kErrBadBlock = 2, kErrLayout = 4, kErrBadToken = 8, kErrLogits = 16 };
@@ -189,6 +199,96 @@ cudaError_t launch_prefill_tc(const PrefillLaunch& p, cudaStream_t s);
 
 cudaError_t launch_apply_updates(const PoolGeom& g, const TableUpdate* updates, int32_t n_updates,
                                  const CopyJob* copies, int32_t n_copies, cudaStream_t s);
+
+// ---- append with per-head norms (slmkv_normed_append.cu) ----
+struct NormedAppendLaunch {
+  PoolGeom g;
+  int32_t layer;
+  const SeqEntry* seqs;
+  int32_t n_seq;
+  int32_t total_tokens;
+  const float* q;  // token rows, heads contiguous; elements from a row to the next:
+  const float* k;
+  const float* v;
+  int64_t q_stride, k_stride, v_stride;
+  const float* q_norm;  // [d]
+  const float* k_norm;
+  float eps;
+  int32_t rotate;
+  float* q_out;  // [total_tokens, Hq, d]
+  int32_t* status;
+};
+cudaError_t launch_normed_append(const NormedAppendLaunch& p, cudaStream_t s);
+
+// ---- attention over shared prefixes (slmkv_shared_attention.cu) ----
+// The batch's tokens, sequences with a common prefix next to each other.
+struct SharedToken {
+  int32_t row;   // the token's row in the batch
+  int32_t pos;   // its position: it sees positions 0..pos
+  int32_t seq;   // its sequence's batch row
+  int32_t edge;  // its sequence's own edge
+};
+// An edge of the tree of block tables: a run of blocks that the tokens from
+// token0 on see, and no others. Its parts: [kv_head][split][row of the edge].
+struct SharedEdge {
+  int32_t parent;  // -1: none
+  int32_t token0;
+  int32_t n_splits;
+  int32_t n_rows;  // tokens x query heads per KV head
+  int32_t part0;   // first part (row slots)
+};
+// One CTA: up to 16 rows (tokens x query heads of one KV head) over a run of
+// an edge's blocks.
+struct SharedItem {
+  int32_t slot, first_block, n_blocks, head;
+  int32_t token0, n_tokens;
+  int32_t part;       // first part slot, -1: the rows' whole output
+  int32_t mask_from;  // positions from here on are hidden from some row
+};
+struct SharedAttentionLaunch {
+  PoolGeom g;
+  int32_t layer;
+  const float* q;  // [total_tokens, Hq, d]
+  float* out;
+  int32_t rotate;
+  int32_t* status;  // [n_seq]
+  const SharedItem* items;
+  int32_t n_items;
+  const SharedToken* tokens;
+  const SharedEdge* edges;
+  const int32_t* merge_tokens;  // tokens whose output is joined from parts
+  int32_t n_merge;
+  float* part_acc;  // [slots][d]
+  float2* part_ml;  // [slots]: maximum (exp2 domain), sum
+};
+int shared_rows_min_blocks(bool bf16);  // blocks that keep every warp of a CTA busy
+cudaError_t launch_shared_attention(const SharedAttentionLaunch& p, cudaStream_t s);
+
+// ---- probabilities and draft verification (slmkv_sampling.cu) ----
+struct ProbabilitiesLaunch {
+  const float* logits;
+  int64_t logits_stride;
+  int32_t rows, vocab;
+  const float* temperatures;  // [rows] or null: 1
+  float* out;                 // [rows, vocab]
+  const SeqEntry* seqs;
+  int32_t n_seq;
+  int32_t* status;
+};
+cudaError_t launch_probabilities(const ProbabilitiesLaunch& p, cudaStream_t s);
+struct VerifyLaunch {
+  const SeqEntry* seqs;
+  int32_t n_seq, vocab;
+  const int32_t* token_ids;  // [total_tokens]
+  const float* target;       // [total_tokens, vocab]
+  const float* draft;        // [total_tokens - n_seq, vocab] or null
+  const float* uniforms;     // [total_tokens]
+  int32_t* accepted;         // [n_seq]
+  int32_t* next_tokens;      // [n_seq]
+  int32_t* status;
+};
+int64_t verify_max_vocab();
+cudaError_t launch_verify(const VerifyLaunch& p, cudaStream_t s);
 
 // ---- few-row projections on the tensor cores (slmkv_rowgemm.cu) ----
 enum : int { kRowQKV = 0, kRowO = 1, kRowGU = 2, kRowDown = 3, kRowHead = 4 };

@@ -1323,8 +1323,8 @@ cudaError_t launch_proj(const ProjArgs& a, cudaStream_t s) {
 // projections are the fused kernels above (5 launches a layer with the cache
 // step); beyond, tensor-core GEMMs with separate norm / rounding / SiTU.
 slm_status run_step(slm_model* m, slm_batch* b, const BatchRows& br, const int32_t* ids, int32_t rows,
-                    bool prefill, float* logits, int32_t* next) {
-  const int32_t out_rows = prefill ? br.n_seq : rows;
+                    bool prefill, float* logits, int32_t* next, bool every_row = false) {
+  const int32_t out_rows = prefill && !every_row ? br.n_seq : rows;
   slm_status rc = ensure_scratch(m, rows, out_rows, br.stream);
   if (rc) return rc;
   cudaStream_t s = br.stream;
@@ -1509,7 +1509,7 @@ slm_status run_step(slm_model* m, slm_batch* b, const BatchRows& br, const int32
       return blas_fail(m->ctx, "slm_model down projection", bs);
   }
   if (logits || next) {
-    const SeqEntry* last_rows = prefill ? br.d_seqs : nullptr;
+    const SeqEntry* last_rows = prefill && !every_row ? br.d_seqs : nullptr;
     // the row-GEMM path's head: tensor cores over the split operands
     const bool head3 = !fused && m->head3 != nullptr && out_rows <= kRowGemmRows;
     if (fused)
@@ -1846,6 +1846,18 @@ slm_status slm_model_prefill(slm_model* m, slm_batch* b, const int32_t* d_token_
   const BatchRows br = batch_rows(b);
   if (br.n_seq == 0 || br.total_tokens == 0) return SLM_OK;
   return run_step(m, b, br, d_token_ids, br.total_tokens, true, d_logits, d_next_token);
+}
+
+slm_status slm_model_score(slm_model* m, slm_batch* b, const int32_t* d_token_ids, float* d_logits,
+                           int32_t* d_next_token) {
+  if (!m || !b || !d_token_ids) return SLM_ERR_INVALID_INPUT;
+  if (batch_ctx(b) != m->ctx)
+    return ctx_fail(m->ctx, SLM_ERR_INVALID_INPUT, "invalid input for model step: batch of another context");
+  slm_status rc = ctx_need_device(m->ctx);
+  if (rc) return rc;
+  const BatchRows br = batch_rows(b);
+  if (br.n_seq == 0 || br.total_tokens == 0) return SLM_OK;
+  return run_step(m, b, br, d_token_ids, br.total_tokens, true, d_logits, d_next_token, true);
 }
 
 }  // extern "C"

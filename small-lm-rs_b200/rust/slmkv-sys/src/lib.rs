@@ -119,6 +119,10 @@ extern "C" {
     pub fn slm_batch_prefill_attention(batch: *mut SlmBatch, layer: i32, d_query: *const f32, rotate_query: i32, d_out: *mut f32) -> i32;
     pub fn slm_batch_attention_exact(batch: *mut SlmBatch, layer: i32, d_query: *const f32, rotate_query: i32, d_out: *mut f32) -> i32;
     pub fn slm_batch_decode_layer_exact(batch: *mut SlmBatch, layer: i32, d_query: *const f32, d_keys: *const f32, d_values: *const f32, d_out: *mut f32) -> i32;
+    pub fn slm_batch_append_layer_normed(batch: *mut SlmBatch, layer: i32, d_query: *const f32, d_keys: *const f32, d_values: *const f32, query_stride: i64, key_stride: i64, value_stride: i64, d_query_norm: *const f32, d_key_norm: *const f32, epsilon: f32, rotate: i32, d_query_out: *mut f32) -> i32;
+    pub fn slm_batch_shared_attention(batch: *mut SlmBatch, layer: i32, d_query: *const f32, rotate_query: i32, d_out: *mut f32) -> i32;
+    pub fn slm_batch_token_probabilities(batch: *mut SlmBatch, d_logits: *const f32, rows: i32, vocab_size: i32, logits_stride: i64, d_temperatures: *const f32, d_probabilities: *mut f32) -> i32;
+    pub fn slm_batch_verify_drafts(batch: *mut SlmBatch, vocab_size: i32, d_token_ids: *const i32, d_target: *const f32, d_draft: *const f32, d_uniforms: *const f32, d_accepted: *mut i32, d_next_tokens: *mut i32) -> i32;
     pub fn slm_batch_end(batch: *mut SlmBatch, h_status: *mut i32) -> i32;
     pub fn slm_batch_rollback(batch: *mut SlmBatch) -> i32;
     pub fn slm_batch_submit(batch: *mut SlmBatch) -> i32;
@@ -126,6 +130,7 @@ extern "C" {
     pub fn slm_prefix_attach(ctx: *mut SlmCtx, seq_id: i32, h_tokens: *const u32, n_tokens: i32, reused_tokens: *mut i32) -> i32;
     pub fn slm_prefix_publish(ctx: *mut SlmCtx, seq_id: i32, h_tokens: *const u32, n_tokens: i32, indexed_blocks: *mut i32) -> i32;
     pub fn slm_pool_stats(ctx: *const SlmCtx, free_blocks: *mut i32, indexed_blocks: *mut i32) -> i32;
+    pub fn slm_pool_storage(ctx: *const SlmCtx, key_address: *mut i64, value_address: *mut i64, layer_values: *mut i64) -> i32;
     pub fn slm_pool_shuffle(ctx: *mut SlmCtx, seed: u64) -> i32;
     pub fn slm_ctx_config(ctx: *const SlmCtx, out: *mut SlmConfig) -> i32;
     pub fn slm_sched_create(ctx: *mut SlmCtx, config: *const SlmSchedConfig, out: *mut *mut SlmSched) -> i32;
@@ -141,6 +146,7 @@ extern "C" {
     pub fn slm_model_set_exact_rows(model: *mut SlmModel, max_rows: i32) -> i32;
     pub fn slm_model_decode(model: *mut SlmModel, batch: *mut SlmBatch, d_token_ids: *const i32, d_logits: *mut f32, d_next_token: *mut i32) -> i32;
     pub fn slm_model_prefill(model: *mut SlmModel, batch: *mut SlmBatch, d_token_ids: *const i32, d_logits: *mut f32, d_next_token: *mut i32) -> i32;
+    pub fn slm_model_score(model: *mut SlmModel, batch: *mut SlmBatch, d_token_ids: *const i32, d_logits: *mut f32, d_next_token: *mut i32) -> i32;
     pub fn slm_model_load_safetensors(ctx: *mut SlmCtx, config: *const SlmModelConfig, path: *const c_char, expected_parameter_count: i64, out: *mut *mut SlmModel) -> i32;
     pub fn slm_safetensors_check(config: *const SlmModelConfig, num_layers: i32, num_key_value_heads: i32, head_dimension: i32, path: *const c_char, expected_parameter_count: i64, parameter_count: *mut i64) -> i32;
 }

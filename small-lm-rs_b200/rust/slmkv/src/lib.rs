@@ -487,6 +487,57 @@ impl<'c> Batch<'c> {
         })
     }
 
+    /// `append_layer` with per-head norms of queries and keys and the rotation
+    /// in one pass; the queries go to `q_out` `[tokens, q_heads, 64]`. Strides
+    /// are values from one token's row to the next.
+    #[allow(clippy::too_many_arguments)]
+    pub fn append_layer_normed(&mut self, layer: i32, q: DevicePtr<f32>, k: DevicePtr<f32>,
+                               v: DevicePtr<f32>, strides: (i64, i64, i64), q_norm: DevicePtr<f32>,
+                               k_norm: DevicePtr<f32>, epsilon: f32, rotate: bool,
+                               q_out: DevicePtr<f32>) -> Result<()> {
+        let b = self.open_raw()?;
+        check(self.ctx.raw, unsafe {
+            sys::slm_batch_append_layer_normed(b, layer, q.c(), k.c(), v.c(), strides.0, strides.1,
+                                               strides.2, q_norm.c(), k_norm.c(), epsilon,
+                                               rotate as i32, q_out.m())
+        })
+    }
+
+    /// `prefill_attention` for caches that share prefixes, whose blocks are
+    /// read once for all of them.
+    pub fn shared_attention(&mut self, layer: i32, q: DevicePtr<f32>, rotate_query: bool,
+                            out: DevicePtr<f32>) -> Result<()> {
+        let b = self.open_raw()?;
+        check(self.ctx.raw, unsafe {
+            sys::slm_batch_shared_attention(b, layer, q.c(), rotate_query as i32, out.m())
+        })
+    }
+
+    /// Softmax of `rows` logit rows (one a token or one a cache) by their
+    /// temperatures (null: 1; 0: the first maximum).
+    pub fn token_probabilities(&mut self, logits: DevicePtr<f32>, rows: i32, vocab_size: i32,
+                               stride: i64, temperatures: DevicePtr<f32>,
+                               probabilities: DevicePtr<f32>) -> Result<()> {
+        let b = self.open_raw()?;
+        check(self.ctx.raw, unsafe {
+            sys::slm_batch_token_probabilities(b, logits.c(), rows, vocab_size, stride,
+                                               temperatures.c(), probabilities.m())
+        })
+    }
+
+    /// Verifies the drafts among the batch's tokens: accepted counts and the
+    /// next token of each cache (`draft` null: drafts chosen outright).
+    #[allow(clippy::too_many_arguments)]
+    pub fn verify_drafts(&mut self, vocab_size: i32, token_ids: DevicePtr<i32>,
+                         target: DevicePtr<f32>, draft: DevicePtr<f32>, uniforms: DevicePtr<f32>,
+                         accepted: DevicePtr<i32>, next_tokens: DevicePtr<i32>) -> Result<()> {
+        let b = self.open_raw()?;
+        check(self.ctx.raw, unsafe {
+            sys::slm_batch_verify_drafts(b, vocab_size, token_ids.c(), target.c(), draft.c(),
+                                         uniforms.c(), accepted.m(), next_tokens.m())
+        })
+    }
+
     /// Closes the step: per cache `Ok(())` or the error that rolled it back
     /// to its length at the step's start (model.rs:390-396).
     pub fn end(mut self) -> Result<Vec<Result<()>>> {
@@ -608,6 +659,16 @@ impl<'c> Model<'c> {
         let b = batch.open_raw()?;
         check(self.ctx.raw, unsafe {
             sys::slm_model_prefill(self.raw, b, token_ids.c(), logits.m(), next_tokens.m())
+        })
+    }
+
+    /// `prefill` with every position projected: logits `[tokens, vocab]` and
+    /// greedy next tokens `[tokens]` (either may be null).
+    pub fn score(&self, batch: &mut Batch<'c>, token_ids: DevicePtr<i32>,
+                 logits: DevicePtr<f32>, next_tokens: DevicePtr<i32>) -> Result<()> {
+        let b = batch.open_raw()?;
+        check(self.ctx.raw, unsafe {
+            sys::slm_model_score(self.raw, b, token_ids.c(), logits.m(), next_tokens.m())
         })
     }
 }

@@ -150,6 +150,11 @@ SIGNATURES = {
     "slm_batch_prefill_attention": (C.c_int, [_vp, _i32, _vp, _i32, _vp]),
     "slm_batch_attention_exact": (C.c_int, [_vp, _i32, _vp, _i32, _vp]),
     "slm_batch_decode_layer_exact": (C.c_int, [_vp, _i32, _vp, _vp, _vp, _vp]),
+    "slm_batch_append_layer_normed": (
+        C.c_int, [_vp, _i32, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp, C.c_float, _i32, _vp]),
+    "slm_batch_shared_attention": (C.c_int, [_vp, _i32, _vp, _i32, _vp]),
+    "slm_batch_token_probabilities": (C.c_int, [_vp, _vp, _i32, _i32, _i64, _vp, _vp]),
+    "slm_batch_verify_drafts": (C.c_int, [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp]),
     "slm_batch_end": (C.c_int, [_vp, _pi32]),
     "slm_batch_rollback": (C.c_int, [_vp]),
     "slm_batch_submit": (C.c_int, [_vp]),
@@ -157,6 +162,7 @@ SIGNATURES = {
     "slm_prefix_attach": (C.c_int, [_vp, _i32, _pu32, _i32, _pi32]),
     "slm_prefix_publish": (C.c_int, [_vp, _i32, _pu32, _i32, _pi32]),
     "slm_pool_stats": (C.c_int, [_vp, _pi32, _pi32]),
+    "slm_pool_storage": (C.c_int, [_vp, C.POINTER(_i64), C.POINTER(_i64), C.POINTER(_i64)]),
     "slm_pool_shuffle": (C.c_int, [_vp, _u64]),
     "slm_ctx_config": (C.c_int, [_vp, C.POINTER(SlmConfig)]),
     "slm_sched_create": (C.c_int, [_vp, C.POINTER(SchedConfig), C.POINTER(_vp)]),
@@ -174,6 +180,7 @@ SIGNATURES = {
     "slm_model_set_exact_rows": (C.c_int, [_vp, _i32]),
     "slm_model_decode": (C.c_int, [_vp, _vp, _vp, _vp, _vp]),
     "slm_model_prefill": (C.c_int, [_vp, _vp, _vp, _vp, _vp]),
+    "slm_model_score": (C.c_int, [_vp, _vp, _vp, _vp, _vp]),
     "slm_model_load_safetensors": (C.c_int, [_vp, C.POINTER(ModelConfig), C.c_char_p, _i64,
                                              C.POINTER(_vp)]),
     "slm_safetensors_check": (C.c_int, [C.POINTER(ModelConfig), _i32, _i32, _i32, C.c_char_p,
@@ -329,6 +336,26 @@ class KvPool:
         f, i = C.c_int32(), C.c_int32()
         self.check(lib().slm_pool_stats(self.handle, C.byref(f), C.byref(i)))
         return f.value, i.value
+
+    def storage(self):
+        """The pool's keys and values (``slm_pool_storage``) as torch views
+        [num_layers, num_blocks, kv_heads, 16, head_dim] of its element type,
+        indexed by the block ids of ``KvCache.blocks``. The views do not keep
+        the pool alive; order their use with the pool's stream."""
+        import torch
+
+        k, v, n = C.c_int64(), C.c_int64(), C.c_int64()
+        self.check(lib().slm_pool_storage(self.handle, C.byref(k), C.byref(v), C.byref(n)))
+        bf16 = self.config.kv_dtype == KV_BF16
+        shape = (self.num_layers, self.config.num_blocks, self.kv_heads, BLOCK_TOKENS, self.head_dim)
+
+        class _Memory:
+            def __init__(self, address):
+                self.__cuda_array_interface__ = {"shape": shape, "typestr": "<i2" if bf16 else "<f4",
+                                                 "data": (address, False), "version": 3}
+
+        views = [torch.as_tensor(_Memory(a.value), device=f"cuda:{self.device}") for a in (k, v)]
+        return tuple(x.view(torch.bfloat16) if bf16 else x for x in views)
 
     def shuffle(self, seed: int) -> None:
         self.check(lib().slm_pool_shuffle(self.handle, C.c_uint64(seed)))
@@ -632,6 +659,89 @@ class Batch:
         self.pool.check(lib().slm_batch_attention_exact(self._h, int(layer), _ptr(query),
                                                         int(bool(rotate_query)), _ptr(out)))
 
+    def _tensor(self, what: str, t, shape, dtype: str = "float32", rows=False) -> int:
+        """Device address of a CUDA tensor of the pool's device with this
+        shape; ``rows``: dense rows at any distance instead of contiguous."""
+        import torch
+
+        if not isinstance(t, torch.Tensor):
+            raise TypeError("expected a torch tensor")
+        if t.shape == shape and t.dtype is getattr(torch, dtype) and t.device.type == "cuda" \
+                and t.device.index == self.pool.device:
+            if t.is_contiguous():
+                return t.data_ptr()
+            if rows and t[0].is_contiguous() and t.stride(0) >= t[0].numel():
+                return t.data_ptr()
+        raise InvalidInput(ERR_INVALID_INPUT,
+                           f"invalid input for slmkv: {what} must be a "
+                           f"{'row-strided' if rows else 'contiguous'} {dtype} CUDA tensor "
+                           f"{list(shape)} on the pool's device")
+
+    def _token_rows(self) -> int:
+        if self.token_counts is None:
+            self.token_counts = list(self._counts[: len(self.caches)])
+        return sum(self.token_counts)
+
+    def append_layer_normed(self, layer: int, query, keys, values, query_norm, key_norm, query_out,
+                            *, epsilon: float = 1e-5, rotate: bool = True) -> None:
+        """slm_batch_append_layer_normed: per-head norms of queries and keys,
+        rotation at the tokens' positions, keys and values into the cache,
+        queries to ``query_out`` [tokens, q_heads, d]. query [tokens, q_heads,
+        d], keys / values [tokens, kv_heads, d]: rows may be strided (slices of
+        one projection's output); query_norm, key_norm [d]."""
+        p, t = self.pool, self._token_rows()
+        ins = [self._tensor("query", query, (t, p.q_heads, p.head_dim), rows=True),
+               self._tensor("keys", keys, (t, p.kv_heads, p.head_dim), rows=True),
+               self._tensor("values", values, (t, p.kv_heads, p.head_dim), rows=True)]
+        # one row has no distance to a next one
+        strides = [x.stride(0) if t > 1 else x[0].numel() for x in (query, keys, values)]
+        p.check(lib().slm_batch_append_layer_normed(
+            self._h, int(layer), *ins, *strides, self._tensor("query_norm", query_norm, (p.head_dim,)),
+            self._tensor("key_norm", key_norm, (p.head_dim,)), float(epsilon), int(bool(rotate)),
+            self._tensor("query_out", query_out, (t, p.q_heads, p.head_dim))))
+
+    def shared_prefix_attention(self, layer: int, query, out, rotate_query: bool = True) -> None:
+        """slm_batch_shared_attention: prefill_attention for sequences that
+        share cached prefixes, whose blocks are read once for all of them;
+        query / out [tokens, q_heads, d]."""
+        p, t = self.pool, self._token_rows()
+        p.check(lib().slm_batch_shared_attention(
+            self._h, int(layer), self._tensor("query", query, (t, p.q_heads, p.head_dim)),
+            int(bool(rotate_query)), self._tensor("out", out, (t, p.q_heads, p.head_dim))))
+
+    def token_probabilities(self, logits, probabilities, temperatures=None) -> None:
+        """slm_batch_token_probabilities: softmax of logits / temperature per
+        row ([tokens or sequences, vocab], rows may be strided; temperature 0:
+        the first maximum), into ``probabilities`` (same shape, dense; may be
+        ``logits``). temperatures: [rows] float32, or None for 1."""
+        import torch
+
+        if not isinstance(logits, torch.Tensor) or logits.dim() != 2:
+            raise InvalidInput(ERR_INVALID_INPUT, "invalid input for slmkv: logits must be [rows, vocab]")
+        rows, vocab = logits.shape
+        src = self._tensor("logits", logits, (rows, vocab), rows=True)
+        t = None if temperatures is None else self._tensor("temperatures", temperatures, (rows,))
+        self.pool.check(lib().slm_batch_token_probabilities(
+            self._h, src, rows, vocab, logits.stride(0) if rows > 1 else vocab, t,
+            self._tensor("probabilities", probabilities, (rows, vocab))))
+
+    def verify_drafts(self, token_ids, target, draft, uniforms, accepted, next_tokens) -> None:
+        """slm_batch_verify_drafts: token_ids [tokens] int32 (each sequence's
+        last accepted token, then its drafts), target [tokens, vocab], draft
+        [tokens - sequences, vocab] or None, uniforms [tokens]; accepted and
+        next_tokens [sequences] int32 are written."""
+        import torch
+
+        if not isinstance(target, torch.Tensor) or target.dim() != 2:
+            raise InvalidInput(ERR_INVALID_INPUT, "invalid input for slmkv: target must be [tokens, vocab]")
+        t, n, vocab = self._token_rows(), len(self.caches), target.shape[1]
+        q = None if draft is None else self._tensor("draft", draft, (t - n, vocab))
+        self.pool.check(lib().slm_batch_verify_drafts(
+            self._h, vocab, self._tensor("token_ids", token_ids, (t,), "int32"),
+            self._tensor("target", target, (t, vocab)), q, self._tensor("uniforms", uniforms, (t,)),
+            self._tensor("accepted", accepted, (n,), "int32"),
+            self._tensor("next_tokens", next_tokens, (n,), "int32")))
+
     def end(self, raise_on_error: bool = True) -> list[int]:
         if self._h is None:
             return self.statuses or []
@@ -849,6 +959,12 @@ class Model:
         last position ([n, vocab], [n])."""
         self.pool.check(lib().slm_model_prefill(self._h, batch._h, _ptr_i32(token_ids),
                                                 _ptr(logits), _ptr_i32(next_tokens)))
+
+    def score(self, batch: "Batch", token_ids, logits=None, next_tokens=None) -> None:
+        """prefill with every position projected: logits [tokens, vocab],
+        next_tokens [tokens] (for Batch.token_probabilities / verify_drafts)."""
+        self.pool.check(lib().slm_model_score(self._h, batch._h, _ptr_i32(token_ids),
+                                              _ptr(logits), _ptr_i32(next_tokens)))
 
     def close(self) -> None:
         if getattr(self, "_h", None) is not None:
