@@ -274,6 +274,7 @@ struct ProbabilitiesLaunch {
   const SeqEntry* seqs;
   int32_t n_seq;
   int32_t* status;
+  int32_t cluster;  // CTAs a row (chosen by the launcher)
 };
 cudaError_t launch_probabilities(const ProbabilitiesLaunch& p, cudaStream_t s);
 struct VerifyLaunch {
@@ -286,6 +287,7 @@ struct VerifyLaunch {
   int32_t* accepted;         // [n_seq]
   int32_t* next_tokens;      // [n_seq]
   int32_t* status;
+  int32_t cluster;  // CTAs a sequence (chosen by the launcher)
 };
 int64_t verify_max_vocab();
 cudaError_t launch_verify(const VerifyLaunch& p, cudaStream_t s);

@@ -1,5 +1,5 @@
 // Token probabilities of logit rows, and the verification of drafted tokens
-// against them.
+// against them. Both spread a row over a thread-block cluster and read it once.
 #include <cfloat>
 
 #include "slmkv_device.h"
@@ -8,61 +8,190 @@ namespace slmkv {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kMaxCluster = 8;  // the portable cluster size
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// Writes a 16-byte record to CTA `rank`'s shared memory, at the same place as p
+// in this one's.
+__device__ __forceinline__ void cluster_write(void* p, uint32_t rank, uint4 v) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+               : "=r"(a)
+               : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))), "r"(rank));
+  asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+               : "memory");
+}
+
+template <typename T, int kThreads, typename Op>
+__device__ __forceinline__ T block_reduce(T v, T* scratch, Op op) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(kFullMask, v, o));
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = scratch[threadIdx.x & (kThreads / 32 - 1)];
+#pragma unroll
+  for (int o = kThreads / 64; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(kFullMask, v, o));
+  return v;
+}
 
 // ---------------------------------------------------------------------------
 // p_i = exp((x_i - max x) / T) / sum, or the one-hot of the first maximum at
 // T = 0; a masked token (-inf) gets 0.
+//
+// Bound by memory (8 bytes a value). A cluster of C CTAs holds a row in shared
+// memory between its one read and its one write: each CTA takes the maximum m_r
+// and the sum s_r of its slice, the CTAs exchange them once over distributed
+// shared memory, and a slice's powers are scaled by
+// 2^(m_r - m) / sum_r s_r 2^(m_r - m). Rows wider than the shared memory of a
+// cluster are read again from global memory instead.
+//
+// Every thread copies, and reads back, its own 16-byte lines, so the copies need
+// no barrier; slices of up to 56 KiB leave four CTAs an SM, one's copies under
+// another's arithmetic. (Slices in registers, 8 lines a thread, took 91 us for
+// 320 rows of 100003 at two CTAs an SM, 126 us at one.) Rows may start anywhere
+// in a line (odd vocabularies): threads take whole lines, and the values of the
+// first and last line outside the row are left alone.
 // ---------------------------------------------------------------------------
-constexpr int kProbThreads = 512;
+constexpr int kProbThreads = 256;
 
-template <typename T, typename Op>
-__device__ __forceinline__ T block_reduce(T v, T* scratch, Op op) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(kFullMask, v, o));
-  __syncthreads();  // scratch may hold an earlier reduction
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = scratch[threadIdx.x & (kProbThreads / 32 - 1)];
-#pragma unroll
-  for (int o = kProbThreads / 64; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(kFullMask, v, o));
-  return v;
-}
+struct ProbSlice {  // exchanged between the CTAs of a row
+  float max, sum;
+  int first, bad;  // first index of the maximum; the row gives no distribution
+};
+static_assert(sizeof(ProbSlice) == 16, "written as one uint4");
 
-__global__ void __launch_bounds__(kProbThreads) probabilities_kernel(const ProbabilitiesLaunch p) {
-  __shared__ float red[kProbThreads / 32];
-  __shared__ int redi[kProbThreads / 32];
-  const int row = blockIdx.x, V = p.vocab;
+// KEEP: the slice stays in shared memory; otherwise it is read again.
+template <bool KEEP>
+__global__ void __launch_bounds__(kProbThreads, 4) probabilities_kernel(const ProbabilitiesLaunch p) {
+  extern __shared__ float4 kept[];
+  __shared__ float red_max[kProbThreads / 32], red_sum[kProbThreads / 32];
+  __shared__ int red_first[kProbThreads / 32], red_bad[kProbThreads / 32];
+  __shared__ __align__(16) ProbSlice slices[kMaxCluster];
+  const int ctas = p.cluster, rank = static_cast<int>(cluster_rank()), row = blockIdx.x / ctas, V = p.vocab;
+  if (ctas > 1) cluster_arrive();  // the row's CTAs have all started once the wait below returns
   const float* x = p.logits + row * p.logits_stride;
   float* y = p.out + static_cast<int64_t>(row) * V;
+  const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(x) >> 2) & 3);
+  const bool lines = static_cast<int>((reinterpret_cast<uintptr_t>(y) >> 2) & 3) == shift;  // stores too
+  const int n_lines = (V + shift + 3) >> 2, per = (n_lines + ctas - 1) / ctas;
+  const int begin = rank * per, end = min(n_lines, begin + per);
+
+  auto inside = [&](int e) { return e >= 0 && e + 4 <= V; };
+  auto edge = [&](int e) {  // a line of which some values lie outside the row: -inf there
+    return make_float4(e >= 0 ? x[e] : -INFINITY, e + 1 >= 0 && e + 1 < V ? x[e + 1] : -INFINITY,
+                       e + 2 >= 0 && e + 2 < V ? x[e + 2] : -INFINITY,
+                       e + 3 >= 0 && e + 3 < V ? x[e + 3] : -INFINITY);
+  };
+  if constexpr (KEEP) {
+    for (int i = begin + threadIdx.x; i < end; i += kProbThreads) {
+      const int e = 4 * i - shift;
+      if (inside(e))
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                         static_cast<uint32_t>(__cvta_generic_to_shared(kept + (i - begin)))),
+                     "l"(x + e)
+                     : "memory");
+      else
+        kept[i - begin] = edge(e);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  }
+  auto load = [&](int i) -> float4 {
+    if constexpr (KEEP) return kept[i - begin];
+    const int e = 4 * i - shift;
+    return inside(e) ? *reinterpret_cast<const float4*>(x + e) : edge(e);
+  };
+  auto store = [&](int i, float4 v) {
+    const int e = 4 * i - shift;
+    if (lines && inside(e)) {
+      *reinterpret_cast<float4*>(y + e) = v;
+      return;
+    }
+    if (e >= 0) y[e] = v.x;
+    if (e + 1 >= 0 && e + 1 < V) y[e + 1] = v.y;
+    if (e + 2 >= 0 && e + 2 < V) y[e + 2] = v.z;
+    if (e + 3 >= 0 && e + 3 < V) y[e + 3] = v.w;
+  };
   const float t = p.temperatures ? p.temperatures[row] : 1.f;
-  float m = -INFINITY;
   int bad = !(t >= 0.f && t <= FLT_MAX);
-  for (int i = threadIdx.x; i < V; i += kProbThreads) {
-    m = fmaxf(m, x[i]);
-    bad |= !(x[i] <= FLT_MAX);  // NaN or +inf
+  float m = -INFINITY;
+#pragma unroll 4
+  for (int i = begin + threadIdx.x; i < end; i += kProbThreads) {
+    const float4 a = load(i);
+    m = fmaxf(fmaxf(m, fmaxf(a.x, a.y)), fmaxf(a.z, a.w));
+    // not a number, or +inf
+    bad |= !(a.x <= FLT_MAX) | !(a.y <= FLT_MAX) | !(a.z <= FLT_MAX) | !(a.w <= FLT_MAX);
   }
-  m = block_reduce(m, red, [](float a, float b) { return fmaxf(a, b); });
-  bad = block_reduce(bad, redi, [](int a, int b) { return a | b; });
-  if (bad || m == -INFINITY) {
-    for (int i = threadIdx.x; i < V; i += kProbThreads) y[i] = 0.f;
-    if (threadIdx.x == 0)
-      atomicOr(&p.status[p.rows == p.n_seq ? row : find_sequence(p.seqs, p.n_seq, row)], kStatusLogits);
-    return;
-  }
-  if (t == 0.f) {
-    int first = INT32_MAX;
-    for (int i = threadIdx.x; i < V; i += kProbThreads)
-      if (x[i] == m) first = min(first, i);
-    first = block_reduce(first, redi, [](int a, int b) { return min(a, b); });
-    for (int i = threadIdx.x; i < V; i += kProbThreads) y[i] = i == first ? 1.f : 0.f;
-    return;
-  }
-  const float c = fminf(kLog2e / t, FLT_MAX);
+  m = block_reduce<float, kProbThreads>(m, red_max, [](float a, float b) { return fmaxf(a, b); });
+  const float base = m == -INFINITY ? 0.f : m;
+  // the least T whose reciprocal is in range keeps 0 * c = 0 at the maximum
+  const float c = t > 0.f ? fminf(kLog2e / t, FLT_MAX) : 0.f;
+  auto power = [&](const float4& a) {
+    return make_float4(exp2_fast((a.x - base) * c), exp2_fast((a.y - base) * c), exp2_fast((a.z - base) * c),
+                       exp2_fast((a.w - base) * c));
+  };
   float sum = 0.f;
-  for (int i = threadIdx.x; i < V; i += kProbThreads) sum += exp2_fast((x[i] - m) * c);
-  sum = block_reduce(sum, red, [](float a, float b) { return a + b; });
-  const float inv = 1.f / sum;
-  for (int i = threadIdx.x; i < V; i += kProbThreads) y[i] = exp2_fast((x[i] - m) * c) * inv;
+  int first = INT32_MAX;
+  if (t > 0.f) {
+#pragma unroll 4
+    for (int i = begin + threadIdx.x; i < end; i += kProbThreads) {
+      const float4 a = power(load(i));
+      sum += (a.x + a.y) + (a.z + a.w);
+    }
+  } else {
+    for (int i = begin + threadIdx.x; i < end; i += kProbThreads) {
+      const float4 a = load(i);
+      const int at = a.x == m ? 0 : a.y == m ? 1 : a.z == m ? 2 : a.w == m ? 3 : -1;
+      if (at >= 0) first = min(first, 4 * i - shift + at);
+    }
+    first = block_reduce<int, kProbThreads>(first, red_first, [](int a, int b) { return min(a, b); });
+  }
+  sum = block_reduce<float, kProbThreads>(sum, red_sum, [](float a, float b) { return a + b; });
+  bad = block_reduce<int, kProbThreads>(bad, red_bad, [](int a, int b) { return a | b; });
+
+  float top = m, total = sum;
+  if (ctas > 1) {
+    cluster_wait();
+    // every CTA sends its record to all of the row's, so that after one barrier
+    // each reads its own copy
+    if (static_cast<int>(threadIdx.x) < ctas)
+      cluster_write(&slices[rank], threadIdx.x,
+                    make_uint4(__float_as_uint(m), __float_as_uint(sum), static_cast<uint32_t>(first),
+                               static_cast<uint32_t>(bad)));
+    cluster_arrive();
+    cluster_wait();
+    for (int r = 0; r < ctas; ++r) top = fmaxf(top, slices[r].max);
+    total = 0.f;
+    first = INT32_MAX;
+    for (int r = 0; r < ctas; ++r) {
+      const ProbSlice o = slices[r];
+      bad |= o.bad;
+      if (o.max == top) first = min(first, o.first);
+      if (o.max != -INFINITY) total += o.sum * exp2_fast((o.max - top) * c);  // (a slice of masked tokens has none)
+    }
+  }
+  if (bad || top == -INFINITY) {
+    for (int i = begin + threadIdx.x; i < end; i += kProbThreads) store(i, make_float4(0.f, 0.f, 0.f, 0.f));
+    if (rank == 0 && threadIdx.x == 0)
+      atomicOr(&p.status[p.rows == p.n_seq ? row : find_sequence(p.seqs, p.n_seq, row)], kStatusLogits);
+  } else if (t == 0.f) {
+    for (int i = begin + threadIdx.x; i < end; i += kProbThreads) {
+      const int e = 4 * i - shift;
+      store(i, make_float4(e == first, e + 1 == first, e + 2 == first, e + 3 == first));
+    }
+  } else {
+    const float f = m == -INFINITY ? 0.f : exp2_fast((m - top) * c) / total;
+#pragma unroll 4
+    for (int i = begin + threadIdx.x; i < end; i += kProbThreads) {
+      const float4 a = power(load(i));
+      store(i, make_float4(a.x * f, a.y * f, a.z * f, a.w * f));
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -71,15 +200,30 @@ __global__ void __launch_bounds__(kProbThreads) probabilities_kernel(const Proba
 // last row's p, as the first index whose running sum passes u times the total.
 // Differences, sums and the border are in 64 bits: the draw is a whole number
 // that must not move with the order of a sum.
+//
+// Bound by memory where there are many sequences (one row of p each, one of q
+// where a draft is rejected), by latency otherwise. A cluster of C CTAs shares
+// a row: every warp sums tiles of 128 consecutive values, the CTAs exchange
+// their totals, and the one that holds the border finds its tile among the
+// sums and reads that tile again.
 // ---------------------------------------------------------------------------
 constexpr int kVerifyThreads = 256;
-constexpr int kTile = 128;  // consecutive values a warp takes at a time
+constexpr int kTile = 128;  // consecutive values a warp sums
+constexpr int kVerifyTiles = 640;  // of a CTA, at most
 
-__global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyLaunch p) {
-  extern __shared__ double tile_sum[];
-  __shared__ int s_first, s_flags, s_tile;
-  __shared__ double s_before, s_total;
-  const int i = blockIdx.x, V = p.vocab, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+struct VerifySlice {
+  double total;
+  int flags, pad;
+};
+static_assert(sizeof(VerifySlice) == 16, "read as one uint4");
+
+__global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyLaunch p) {
+  __shared__ double tile_sum[kVerifyTiles];
+  __shared__ __align__(16) VerifySlice slices[2][kMaxCluster];
+  __shared__ int s_first, s_flags;
+  const int ctas = p.cluster, rank = static_cast<int>(cluster_rank()), i = blockIdx.x / ctas, V = p.vocab;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (ctas > 1) cluster_arrive();  // the row's CTAs have all started once the wait below returns
   const SeqEntry se = p.seqs[i];
   const int k = se.count - 1;              // drafts
   const int r0 = se.row_offset;            // target rows of the sequence
@@ -97,114 +241,212 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyLaun
     }
     const float pt = p.target[static_cast<int64_t>(r0 + j) * V + x];
     const float qt = p.draft ? p.draft[(q0 + j) * V + x] : 1.f;
-    if (!(pt >= 0.f && pt <= FLT_MAX && qt >= 0.f && qt <= FLT_MAX)) atomicOr(&s_flags, kStatusProbability);
     if (!(static_cast<double>(p.uniforms[r0 + j]) * qt < static_cast<double>(pt))) atomicMin(&s_first, j);
   }
+  const double u = fmax(static_cast<double>(p.uniforms[r0 + k]), 0.0);
   __syncthreads();
   const int a = s_first;
   const int skip = !p.draft && a < k ? p.token_ids[r0 + a + 1] : -1;  // a draft without probabilities: q = 1 there
   const float* pr = p.target + static_cast<int64_t>(r0 + a) * V;
   const float* qr = p.draft && a < k ? p.draft + (q0 + a) * V : nullptr;
-  const int tiles = (V + kTile - 1) / kTile;
+  const int tiles = (V + kTile - 1) / kTile, per = (tiles + ctas - 1) / ctas;
+  const int first_tile = rank * per, n_tiles = max(0, min(tiles, first_tile + per) - first_tile);
   bool rest = a < k;  // the residual; the row itself when nothing of it is left
-  auto weight = [&](int x, int& bad) -> double {
-    if (x >= V) return 0.0;
-    const float pv = pr[x];
-    bad |= !(pv >= 0.f && pv <= FLT_MAX);
+  auto usable = [](float w) { return w >= 0.f && w <= FLT_MAX; };
+  auto weight = [&](float pv, float qv, int x) -> double {
     if (!rest) return pv;
     if (!qr) return x == skip ? 0.0 : pv;
-    const float qv = qr[x];
-    bad |= !(qv >= 0.f && qv <= FLT_MAX);
     return fmax(static_cast<double>(pv) - static_cast<double>(qv), 0.0);
   };
-  for (;;) {
+  double total = 0.0, run_sum = 0.0, run_upto = 0.0;  // runs: of warp 0's lanes
+  int flags = 0, round = 0;
+  const int run = (n_tiles + 31) >> 5;  // tiles of a lane
+  for (; round < 2; ++round) {
     int bad = 0;
-    for (int t = warp; t < tiles; t += kVerifyThreads / 32) {
-      double s = 0.0;
+    constexpr int kUnroll = 4;  // tiles in flight a warp
+    for (int t = warp; t < n_tiles; t += kUnroll * (kVerifyThreads / 32)) {
+      float pv[kUnroll][4], qv[kUnroll][4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s += weight(t * kTile + 32 * e + lane, bad);
+      for (int n = 0; n < kUnroll; ++n)
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kFullMask, s, o);
-      if (lane == 0) tile_sum[t] = s;
+        for (int e = 0; e < 4; ++e) {
+          const int tt = t + n * (kVerifyThreads / 32), x = (first_tile + tt) * kTile + 32 * e + lane;
+          const bool in = tt < n_tiles && x < V;
+          pv[n][e] = in ? pr[x] : 0.f;
+          qv[n][e] = in && qr && rest ? qr[x] : 0.f;
+        }
+#pragma unroll
+      for (int n = 0; n < kUnroll; ++n) {
+        const int tt = t + n * (kVerifyThreads / 32);
+        double s = 0.0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          bad |= !usable(pv[n][e]) | !usable(qv[n][e]);
+          s += weight(pv[n][e], qv[n][e], (first_tile + tt) * kTile + 32 * e + lane);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kFullMask, s, o);
+        if (lane == 0 && tt < n_tiles) tile_sum[tt] = s;
+      }
     }
     if (bad) atomicOr(&s_flags, kStatusProbability);
+    if (ctas > 1 && round == 0) cluster_wait();
     __syncthreads();
-    if (tid == 0) {
-      double total = 0.0;
-      for (int t = 0; t < tiles; ++t) total += tile_sum[t];
-      const double u = p.uniforms[r0 + k];
-      const double point = u * total;
-      double before = 0.0;
-      int pick = -1, last = -1;
-      double last_before = 0.0;
-      for (int t = 0; t < tiles && pick < 0; ++t) {
-        if (tile_sum[t] > 0.0) {
-          last = t;
-          last_before = before;
-        }
-        if (before + tile_sum[t] > point) pick = t;
-        else before += tile_sum[t];
+    if (warp == 0) {  // the CTA's total: lane l sums its run of tiles, then across lanes in order
+      run_sum = 0.0;
+      for (int t = lane * run; t < min(n_tiles, (lane + 1) * run); ++t) run_sum += tile_sum[t];
+      run_upto = run_sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double up = __shfl_up_sync(kFullMask, run_upto, o);
+        if (lane >= o) run_upto += up;
       }
-      if (pick < 0) {  // u >= 1 or not a number: the last token with a weight
-        pick = last;
-        before = last_before;
-      }
-      s_tile = pick;
-      s_before = before;
-      s_total = total;
+      const double sum = __shfl_sync(kFullMask, run_upto, 31);
+      if (lane < ctas)  // to every CTA of the row
+        cluster_write(&slices[round][rank], lane,
+                      make_uint4(static_cast<uint32_t>(__double2loint(sum)), static_cast<uint32_t>(__double2hiint(sum)),
+                                 static_cast<uint32_t>(s_flags), 0u));
     }
-    __syncthreads();
-    if (s_flags || s_total > 0.0 || !rest) break;
+    if (ctas > 1) {
+      cluster_arrive();
+      cluster_wait();
+    } else {
+      __syncthreads();
+    }
+    total = 0.0;
+    flags = 0;
+    for (int r = 0; r < ctas; ++r) {
+      total += slices[round][r].total;
+      flags |= slices[round][r].flags;
+    }
+    if (flags || total > 0.0 || !rest) break;  // the same in every CTA of the row
     rest = false;
-    __syncthreads();
   }
   if (warp != 0) return;
-  if (s_flags || !(s_total > 0.0)) {
-    if (lane == 0) {
+  if (flags || !(total > 0.0)) {
+    if (rank == 0 && lane == 0) {
       p.accepted[i] = 0;
       p.next_tokens[i] = -1;
-      atomicOr(&p.status[i], s_flags ? s_flags : kStatusProbability);
+      atomicOr(&p.status[i], flags ? flags : kStatusProbability);
     }
     return;
   }
-  const double point = static_cast<double>(p.uniforms[r0 + k]) * s_total;
-  double before = s_before;
-  int pick = -1, last = -1, bad = 0;
+  // The border's CTA: the first whose running total passes it, or where none
+  // does (u is 1 or more) the last with a weight. The same rule then finds the
+  // lane's run of tiles, the tile and the value.
+  const double point = u * total;
+  double before = 0.0, upto = 0.0;
+  int owner = 0;
+  for (int r = 0; r < ctas; ++r) {
+    const double w = slices[round][r].total;
+    if (w > 0.0) {
+      owner = r;
+      before = upto;
+      if (upto + w > point) break;
+    }
+    upto += w;
+  }
+  if (rank != owner) return;
+  unsigned over = __ballot_sync(kFullMask, run_sum > 0.0 && before + run_upto > point);
+  unsigned live = __ballot_sync(kFullMask, run_sum > 0.0);
+  const int src = over ? __ffs(over) - 1 : 31 - __clz(live);
+  upto = before + __shfl_sync(kFullMask, run_upto - run_sum, src);
+  int tile = src * run;
+  for (int t = src * run; t < min(n_tiles, (src + 1) * run); ++t) {
+    const double w = tile_sum[t];
+    if (w > 0.0) {
+      tile = t;
+      before = upto;
+      if (upto + w > point) break;
+    }
+    upto += w;
+  }
+  // the tile's values again, four consecutive ones a lane
+  const int x0 = (first_tile + tile) * kTile + 4 * lane;
+  double w[4], sum = 0.0;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const int x = s_tile * kTile + 32 * e + lane;
-    const double w = weight(x, bad);
-    double run = w;
+    const int x = x0 + e;
+    w[e] = x < V ? weight(pr[x], qr && rest ? qr[x] : 0.f, x) : 0.0;
+    sum += w[e];
+  }
+  double to = sum;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double up = __shfl_up_sync(kFullMask, run, o);
-      if (lane >= o) run += up;
+  for (int o = 1; o < 32; o <<= 1) {
+    const double up = __shfl_up_sync(kFullMask, to, o);
+    if (lane >= o) to += up;
+  }
+  over = __ballot_sync(kFullMask, sum > 0.0 && before + to > point);
+  live = __ballot_sync(kFullMask, sum > 0.0);
+  if (lane != (over ? __ffs(over) - 1 : 31 - __clz(live))) return;
+  double at = before + (to - sum);
+  int pick = x0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (w[e] > 0.0) {
+      pick = x0 + e;
+      if (at + w[e] > point) break;
     }
-    const unsigned over = __ballot_sync(kFullMask, w > 0.0 && before + run > point);
-    const unsigned live = __ballot_sync(kFullMask, w > 0.0);
-    if (pick < 0 && over) pick = s_tile * kTile + 32 * e + __ffs(over) - 1;
-    if (live) last = s_tile * kTile + 32 * e + 31 - __clz(live);
-    before += __shfl_sync(kFullMask, run, 31);
+    at += w[e];
   }
-  if (lane == 0) {
-    p.accepted[i] = a;
-    p.next_tokens[i] = pick >= 0 ? pick : last;
-  }
+  p.accepted[i] = a;
+  p.next_tokens[i] = pick;
+}
+
+template <typename Kernel, typename Launch>
+cudaError_t launch_clusters(Kernel kernel, const Launch& p, int rows, int threads, size_t smem, cudaStream_t s) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(rows) * p.cluster);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {static_cast<unsigned>(p.cluster), 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = p.cluster > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
 }  // namespace
 
-cudaError_t launch_probabilities(const ProbabilitiesLaunch& p, cudaStream_t s) {
-  probabilities_kernel<<<p.rows, kProbThreads, 0, s>>>(p);
-  return cudaGetLastError();
+cudaError_t launch_probabilities(const ProbabilitiesLaunch& p0, cudaStream_t s) {
+  ProbabilitiesLaunch p = p0;
+  // The fewest CTAs a row whose slices are small enough for four CTAs an SM (up
+  // to 3 values of a first line lie outside the row); more while the SMs are not
+  // filled and a thread keeps two lines.
+  const int64_t lines = (static_cast<int64_t>(p.vocab) + 6) / 4;
+  auto per = [&](int c) { return (lines + c - 1) / c; };
+  p.cluster = 1;
+  while (p.cluster < kMaxCluster && per(p.cluster) * 16 > 56 * 1024) p.cluster *= 2;
+  while (p.cluster < kMaxCluster && p.rows * p.cluster * 2 <= 2 * 148 && per(p.cluster) >= 4 * kProbThreads)
+    p.cluster *= 2;
+  const size_t bytes = static_cast<size_t>(per(p.cluster)) * 16;
+  constexpr size_t kMost = 224 * 1024;
+  if (bytes > kMost) return launch_clusters(probabilities_kernel<false>, p, p.rows, kProbThreads, 0, s);
+  static unsigned long long configured = 0;  // one bit per device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !(configured & (1ull << dev)))) {
+    e = cudaFuncSetAttribute(probabilities_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+    if (e == cudaSuccess && dev < 64) configured |= 1ull << dev;
+  }
+  if (e != cudaSuccess) return e;
+  return launch_clusters(probabilities_kernel<true>, p, p.rows, kProbThreads, bytes, s);
 }
 
-int64_t verify_max_vocab() { return static_cast<int64_t>(kTile) * (40 * 1024 / sizeof(double)); }
+int64_t verify_max_vocab() { return static_cast<int64_t>(kMaxCluster) * kVerifyTiles * kTile; }
 
-cudaError_t launch_verify(const VerifyLaunch& p, cudaStream_t s) {
-  const size_t smem = sizeof(double) * ((p.vocab + kTile - 1) / kTile);
-  verify_kernel<<<p.n_seq, kVerifyThreads, smem, s>>>(p);
-  return cudaGetLastError();
+cudaError_t launch_verify(const VerifyLaunch& p0, cudaStream_t s) {
+  VerifyLaunch p = p0;
+  // CTAs a row: until the SMs hold four each or a warp has a tile left, and at
+  // least what the tile sums of a CTA have room for.
+  const int tiles = (p.vocab + kTile - 1) / kTile;
+  p.cluster = 1;
+  while (p.cluster < kMaxCluster && ((p.n_seq * p.cluster * 2 <= 4 * 148 && tiles / p.cluster > 8) ||
+                                     (tiles + p.cluster - 1) / p.cluster > kVerifyTiles))
+    p.cluster *= 2;
+  return launch_clusters(verify_kernel, p, p.n_seq, kVerifyThreads, 0, s);
 }
 
 }  // namespace slmkv
