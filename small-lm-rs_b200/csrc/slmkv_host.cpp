@@ -96,13 +96,16 @@ struct SharedPlan {
   };
   std::vector<int32_t> order;  // batch rows, members of an edge next to each other
   std::vector<Edge> tree;
-  std::vector<int32_t> by_size;  // edges, longest runs first
-  std::vector<int32_t> token0;   // first token of order[i]
-  std::vector<SharedItem> items;
+  std::vector<int32_t> token0;  // first token of order[i]
+  std::vector<uint8_t> on_tc;   // per edge
+  std::vector<SharedItem> items, tc_items;
+  std::vector<int32_t> list_start;  // first item of a warp's or team's list, and the end
   std::vector<SharedToken> tokens;
   std::vector<SharedEdge> edges;
+  std::vector<SharedUnit> units;
   std::vector<int32_t> merge;
   int64_t parts = 0;
+  int32_t most_parts = 0, team = 0;
 };
 
 // Device addresses of one uploaded step descriptor.
@@ -137,11 +140,7 @@ struct slm_batch {
   int32_t up_slot = 0;  // descriptor slot (its `consumed` event is recorded at the end)
   // slm_batch_shared_attention: the plan, uploaded by the batch's first call.
   bool shared_ready = false;
-  const SharedItem* d_items = nullptr;
-  const SharedToken* d_tokens = nullptr;
-  const SharedEdge* d_edges = nullptr;
-  const int32_t* d_merge = nullptr;
-  int32_t n_items = 0, n_merge = 0;
+  SharedAttentionLaunch shared{};
   // Submitted (slm_batch_submit): its status readback slot; per sequence
   // whether every layer advanced, and a rollback forced by an earlier batch
   // (poison_base >= 0: roll back to at most that length with poison_code).
@@ -1798,6 +1797,9 @@ namespace {
 // A run of blocks that several sequences share becomes an edge of its own from
 // this many blocks on: a shorter one costs more in joining than it saves.
 constexpr int32_t kSharedMinBlocks = 4;
+// Rows (tokens x query heads of a KV head) from which a shared run goes to the
+// tensor cores' 128-row tiles.
+constexpr int32_t kSharedTcMinRows = 48;
 
 // The tree below the members order[lo, hi), which share their blocks before
 // `start` (edge `parent` ends there) and, beyond it, those before `probe`.
@@ -1839,7 +1841,7 @@ void shared_tree(const slm_ctx* c, const slm_batch* b, SharedPlan& plan, int32_t
 
 void build_shared_plan(const slm_ctx* c, const slm_batch* b, SharedPlan& plan) {
   const int32_t n = static_cast<int32_t>(b->seq_ids.size());
-  const int32_t Hkv = c->cfg.num_key_value_heads, G = c->group, tile = 16 / G;
+  const int32_t Hkv = c->cfg.num_key_value_heads, G = c->group;
   plan.order.resize(n);
   for (int32_t i = 0; i < n; ++i) plan.order[i] = i;
   plan.tree.clear();
@@ -1860,78 +1862,143 @@ void build_shared_plan(const slm_ctx* c, const slm_batch* b, SharedPlan& plan) {
     for (int32_t j = 0; j < b->counts[s]; ++j)
       plan.tokens[plan.token0[i] + j] = SharedToken{row0[s] + j, b->base[s] + j, s, -1};
   }
-  // Runs are cut so that the items fill the SMs (three CTAs each) about once,
-  // none shorter than what keeps a CTA's warps busy.
-  auto tiles_of = [&](const SharedPlan::Edge& e) {
-    return (plan.token0[e.seq1] - plan.token0[e.seq0] + tile - 1) / tile;
-  };
-  int64_t work = 0;
-  for (const auto& e : plan.tree)
-    work += static_cast<int64_t>(tiles_of(e)) * Hkv * (e.last_block - e.first_block);
-  const int64_t slots = 3ll * c->num_sms;
-  const int32_t least = shared_rows_min_blocks(c->cfg.kv_dtype == SLM_KV_BF16);
-  const int32_t room = static_cast<int32_t>(std::max<int64_t>(least, (work + slots - 1) / slots));
-  plan.edges.resize(n_edges);
-  plan.by_size.resize(n_edges);
-  plan.parts = 0;
-  plan.merge.clear();
+  // Tensor-core runs are cut into items that fill the SMs (two CTAs each) about
+  // once, of two tiles at least, or of one while those do not fill the SMs.
+  plan.on_tc.assign(n_edges, 0);
   for (int32_t i = 0; i < n_edges; ++i) {
     const auto& e = plan.tree[i];
-    const int32_t nb = e.last_block - e.first_block;
+    const int32_t rows = (plan.token0[e.seq1] - plan.token0[e.seq0]) * G;
+    plan.on_tc[i] = e.seq1 - e.seq0 > 1 && rows >= kSharedTcMinRows &&
+                    e.last_block - e.first_block >= 2 * kSharedTcBlocks;
+  }
+  const int32_t tile = kSharedRows / G, tc_tile = kSharedTcRows / G;
+  auto tiles_of = [&](int32_t i) {
+    const auto& e = plan.tree[i];
+    const int32_t per = plan.on_tc[i] ? tc_tile : tile;
+    return (plan.token0[e.seq1] - plan.token0[e.seq0] + per - 1) / per;
+  };
+  int64_t work = 0, tc_work = 0, n_units = 0;
+  for (int32_t i = 0; i < n_edges; ++i) {
+    const int64_t nb = plan.tree[i].last_block - plan.tree[i].first_block, units = tiles_of(i) * Hkv;
+    if (plan.on_tc[i]) {
+      tc_work += units * ((nb + kSharedTcBlocks - 1) / kSharedTcBlocks);
+    } else {
+      work += units * nb;
+      n_units += units;
+    }
+  }
+  const int64_t tc_slots = 2ll * c->num_sms;
+  int32_t tc_room =
+      static_cast<int32_t>(std::max<int64_t>(tc_work <= c->num_sms ? 1 : 2, (tc_work + tc_slots - 1) / tc_slots)) *
+      kSharedTcBlocks;
+  for (;;) {  // longer runs until the items are one wave (or none is cut)
+    int64_t items = 0;
+    bool cut = false;
+    for (int32_t i = 0; i < n_edges; ++i) {
+      if (!plan.on_tc[i]) continue;
+      const int32_t n = (plan.tree[i].last_block - plan.tree[i].first_block + tc_room - 1) / tc_room;
+      items += static_cast<int64_t>(tiles_of(i)) * Hkv * n;
+      cut = cut || n > 1;
+    }
+    if (!cut || items <= tc_slots) break;
+    tc_room += kSharedTcBlocks;
+  }
+  // The other runs form one stream of (edge, head, row tile) units that the
+  // warps of one wave share evenly, or its CTAs as teams of four warps where a
+  // warp would get fewer than kTeamBelow blocks. A list's budget counts blocks,
+  // and for each piece of a unit what starting and delivering it costs.
+  constexpr int32_t kTeamBelow = 6, kPieceCost = 3;
+  const int64_t ctas = static_cast<int64_t>(kSharedCtasPerSm) * c->num_sms;
+  plan.team = work < kTeamBelow * 4 * ctas;
+  const int64_t lists = plan.team ? ctas : 4 * ctas;
+  const int32_t step = plan.team ? 8 : 2;  // blocks of a step, at most
+  const int32_t budget = static_cast<int32_t>(
+      std::max<int64_t>(step + kPieceCost, (work + kPieceCost * (n_units + lists) + lists - 1) / lists));
+
+  plan.edges.resize(n_edges);
+  plan.units.clear();
+  plan.items.clear();
+  plan.tc_items.clear();
+  plan.list_start.assign(1, 0);
+  plan.merge.clear();
+  plan.parts = 0;
+  plan.most_parts = 0;
+  int32_t room = budget;  // left to the list being filled
+  for (int32_t i = 0; i < n_edges; ++i) {
+    const auto& e = plan.tree[i];
+    const int32_t end = plan.token0[e.seq1], n_tiles = tiles_of(i);
+    const bool own = e.seq1 - e.seq0 == 1;
     SharedEdge& d = plan.edges[i];
     d.parent = e.parent;
     d.token0 = plan.token0[e.seq0];
-    d.n_splits = std::max(1, (nb + room - 1) / room);
-    d.n_rows = (plan.token0[e.seq1] - d.token0) * G;
-    plan.by_size[i] = i;
-    const bool own = e.seq1 - e.seq0 == 1;
-    const bool whole = own && e.parent < 0 && d.n_splits == 1;
-    d.part0 = -1;
-    if (!whole) {
-      d.part0 = static_cast<int32_t>(plan.parts);
-      plan.parts += static_cast<int64_t>(Hkv) * d.n_splits * d.n_rows;
-    }
+    d.unit0 = static_cast<int32_t>(plan.units.size());
+    d.n_tiles = n_tiles;
+    d.tile_tokens = plan.on_tc[i] ? tc_tile : tile;
+    SharedItem it{};
+    it.slot = b->seq_ids[plan.order[e.seq0]];
+    bool joined = e.parent >= 0;  // some row's output has parts
+    for (int32_t h = 0; h < Hkv; ++h)
+      for (int32_t t = d.token0; t < end; t += d.tile_tokens) {
+        it.head = h;
+        it.token0 = t;
+        it.n_tokens = std::min(d.tile_tokens, end - t);
+        // an own run is read up to the tile's last token; shared ones whole
+        int32_t last = e.last_block;
+        it.mask_from = INT32_MAX;
+        if (own) {
+          last = std::min(last, plan.tokens[t + it.n_tokens - 1].pos / kBlockTokens + 1);
+          it.mask_from = plan.tokens[t].pos + 1;
+        }
+        SharedUnit u{static_cast<int32_t>(plan.parts), 0, it.n_tokens * G, 0};
+        if (plan.on_tc[i]) {
+          const int32_t nb = last - e.first_block, n = (nb + tc_room - 1) / tc_room;
+          const int32_t run = ((nb + n - 1) / n + kSharedTcBlocks - 1) / kSharedTcBlocks * kSharedTcBlocks;
+          for (int32_t at = e.first_block; at < last; at += run, ++u.n_parts) {
+            it.first_block = at;
+            it.n_blocks = std::min(run, last - at);
+            it.part = static_cast<int32_t>(plan.parts) + u.n_parts * u.n_rows;
+            plan.tc_items.push_back(it);
+          }
+        } else {
+          const size_t first_item = plan.items.size();
+          for (int32_t at = e.first_block; at < last;) {
+            const int32_t left = last - at;
+            if (room < kPieceCost + step / 2 && room < budget) {  // no use starting a piece: the next list
+              plan.list_start.push_back(static_cast<int32_t>(plan.items.size()));
+              room = budget;
+            }
+            // whole steps; a last few blocks do not go to another list
+            int32_t take = std::max(2, (room - kPieceCost) / 2 * 2);
+            if (take + step / 2 >= left) take = left;
+            it.first_block = at;
+            it.n_blocks = take;
+            it.part = static_cast<int32_t>(plan.parts) + u.n_parts * u.n_rows;
+            plan.items.push_back(it);
+            ++u.n_parts;
+            at += take;
+            room -= take + kPieceCost;
+          }
+          if (e.parent < 0 && own && u.n_parts == 1) {  // all that its rows see
+            plan.items[first_item].part = -1;
+            u.n_parts = 0;
+          }
+        }
+        if (u.n_parts) joined = true;
+        plan.parts += static_cast<int64_t>(u.n_parts) * u.n_rows;
+        plan.units.push_back(u);
+      }
     if (own)
-      for (int32_t k = d.token0; k < plan.token0[e.seq1]; ++k) {
+      for (int32_t k = d.token0; k < end; ++k) {
         plan.tokens[k].edge = i;
-        if (!whole) plan.merge.push_back(k);
+        if (joined) plan.merge.push_back(k);
       }
   }
-  auto run_of = [&](int32_t i) {
-    const auto& e = plan.tree[i];
-    return (e.last_block - e.first_block + plan.edges[i].n_splits - 1) / plan.edges[i].n_splits;
-  };
-  std::sort(plan.by_size.begin(), plan.by_size.end(), [&](int32_t x, int32_t y) {
-    const int32_t a = run_of(x), c2 = run_of(y);
-    return a != c2 ? a > c2 : x < y;
-  });
-  plan.items.clear();
-  for (int32_t i : plan.by_size) {
-    const auto& e = plan.tree[i];
-    const SharedEdge& d = plan.edges[i];
-    const int32_t run = run_of(i), end = plan.token0[e.seq1];
-    const int32_t slot = b->seq_ids[plan.order[e.seq0]];
-    for (int32_t s = 0; s < d.n_splits; ++s)
-      for (int32_t h = 0; h < Hkv; ++h)
-        for (int32_t t = d.token0; t < end; t += tile) {
-          SharedItem it{};
-          it.slot = slot;
-          it.head = h;
-          it.token0 = t;
-          it.n_tokens = std::min(tile, end - t);
-          // an own run is read up to the tile's last token; shared ones whole
-          int32_t last = e.last_block;
-          it.mask_from = INT32_MAX;
-          if (plan.tokens[t].edge == i) {
-            last = std::min(last, plan.tokens[t + it.n_tokens - 1].pos / kBlockTokens + 1);
-            it.mask_from = plan.tokens[t].pos + 1;
-          }
-          it.first_block = e.first_block + s * run;
-          it.n_blocks = std::max(0, std::min(last, it.first_block + run) - it.first_block);
-          it.part = d.part0 < 0 ? -1
-                                : d.part0 + (h * d.n_splits + s) * d.n_rows + (t - d.token0) * G;
-          plan.items.push_back(it);
-        }
+  plan.list_start.push_back(static_cast<int32_t>(plan.items.size()));
+  for (int32_t i = 0; i < n_edges; ++i) {  // the most parts of a row, over its edges up to the root
+    if (plan.tree[i].seq1 - plan.tree[i].seq0 > 1) continue;
+    int32_t n_parts = 0;
+    for (int32_t e = i; e >= 0; e = plan.tree[e].parent) n_parts += plan.units[plan.edges[e].unit0].n_parts;
+    plan.most_parts = std::max(plan.most_parts, n_parts);
   }
 }
 
@@ -1940,12 +2007,17 @@ slm_status shared_prepare(slm_batch* b) {
   slm_ctx* c = b->ctx;
   SharedPlan& plan = c->shared_plan;
   build_shared_plan(c, b, plan);
-  if (plan.parts > INT32_MAX || plan.items.size() > static_cast<size_t>(INT32_MAX))
+  if (plan.parts > INT32_MAX || plan.items.size() + plan.units.size() > static_cast<size_t>(INT32_MAX))
     return input_error(c, SLM_ERR_INVALID_INPUT, "shared prefix attention", "the step has too many rows");
-  const size_t o_tokens = align16(plan.items.size() * sizeof(SharedItem));
-  const size_t o_edges = align16(o_tokens + plan.tokens.size() * sizeof(SharedToken));
-  const size_t o_merge = align16(o_edges + plan.edges.size() * sizeof(SharedEdge));
-  const size_t bytes = align16(o_merge + plan.merge.size() * sizeof(int32_t));
+  size_t bytes = 0;
+  auto place = [&](const auto& v) {
+    const size_t at = bytes;
+    bytes = align16(at + v.size() * sizeof(v[0]));
+    return at;
+  };
+  const size_t o_items = place(plan.items), o_tc = place(plan.tc_items), o_lists = place(plan.list_start),
+               o_tokens = place(plan.tokens), o_edges = place(plan.edges), o_units = place(plan.units),
+               o_merge = place(plan.merge);
   slm_ctx::SharedIo& io = c->shared;
   const int k = b->up_slot;
   if (bytes > io.cap) {
@@ -1983,20 +2055,36 @@ slm_status shared_prepare(slm_batch* b) {
   }
   CU(c, cudaEventSynchronize(io.copied[k]));  // the slot's last upload has left the pinned buffer
   uint8_t* h = io.h[k];
-  memcpy(h, plan.items.data(), plan.items.size() * sizeof(SharedItem));
-  memcpy(h + o_tokens, plan.tokens.data(), plan.tokens.size() * sizeof(SharedToken));
-  memcpy(h + o_edges, plan.edges.data(), plan.edges.size() * sizeof(SharedEdge));
-  memcpy(h + o_merge, plan.merge.data(), plan.merge.size() * sizeof(int32_t));
+  auto put = [&](size_t at, const auto& v) { memcpy(h + at, v.data(), v.size() * sizeof(v[0])); };
+  put(o_items, plan.items);
+  put(o_tc, plan.tc_items);
+  put(o_lists, plan.list_start);
+  put(o_tokens, plan.tokens);
+  put(o_edges, plan.edges);
+  put(o_units, plan.units);
+  put(o_merge, plan.merge);
   // the kernels that last read the slot's device buffer are done
   CU(c, cudaStreamWaitEvent(b->stream, c->up_batch.consumed[k], 0));
   CU(c, cudaMemcpyAsync(io.d[k], h, bytes, cudaMemcpyHostToDevice, b->stream));
   CU(c, cudaEventRecord(io.copied[k], b->stream));
-  b->d_items = reinterpret_cast<const SharedItem*>(io.d[k]);
-  b->d_tokens = reinterpret_cast<const SharedToken*>(io.d[k] + o_tokens);
-  b->d_edges = reinterpret_cast<const SharedEdge*>(io.d[k] + o_edges);
-  b->d_merge = reinterpret_cast<const int32_t*>(io.d[k] + o_merge);
-  b->n_items = static_cast<int32_t>(plan.items.size());
-  b->n_merge = static_cast<int32_t>(plan.merge.size());
+  SharedAttentionLaunch& p = b->shared;
+  const uint8_t* d = io.d[k];
+  p.items = reinterpret_cast<const SharedItem*>(d + o_items);
+  p.tc_items = reinterpret_cast<const SharedItem*>(d + o_tc);
+  p.list_start = reinterpret_cast<const int32_t*>(d + o_lists);
+  p.tokens = reinterpret_cast<const SharedToken*>(d + o_tokens);
+  p.edges = reinterpret_cast<const SharedEdge*>(d + o_edges);
+  p.units = reinterpret_cast<const SharedUnit*>(d + o_units);
+  p.merge_tokens = reinterpret_cast<const int32_t*>(d + o_merge);
+  p.n_lists = static_cast<int32_t>(plan.list_start.size()) - 1;
+  p.team = plan.team;
+  p.n_tc_items = static_cast<int32_t>(plan.tc_items.size());
+  p.n_merge = static_cast<int32_t>(plan.merge.size());
+  p.most_parts = plan.most_parts;
+  p.g = c->geom();
+  p.status = b->dev.status;
+  p.tmap_k = c->tmap_k;
+  p.tmap_v = c->tmap_v;
   b->shared_ready = true;
   return SLM_OK;
 }
@@ -2020,24 +2108,16 @@ slm_status slm_batch_shared_attention(slm_batch* b, int32_t layer, const float* 
   rc = flush_excess(ctx, b->stream, 0, 0);  // the kernels read the device block table
   if (rc) return rc;
   if (!b->shared_ready && (rc = shared_prepare(b))) return rc;
-  SharedAttentionLaunch p{};
-  p.g = ctx->geom();
+  SharedAttentionLaunch& p = b->shared;
   p.layer = layer;
   p.q = d_query;
   p.out = d_out;
   p.rotate = rotate_query != 0;
-  p.status = b->dev.status;
-  p.items = b->d_items;
-  p.n_items = b->n_items;
-  p.tokens = b->d_tokens;
-  p.edges = b->d_edges;
-  p.merge_tokens = b->d_merge;
-  p.n_merge = b->n_merge;
   p.part_acc = ctx->shared.part_acc;
   p.part_ml = ctx->shared.part_ml;
   ctx->prev_decode_layer = -1;
   CU(ctx, launch_shared_attention(p, b->stream));
-  ctx->launches += p.n_merge ? 2 : 1;
+  ctx->launches += 1 + (p.n_tc_items ? 1 : 0) + (p.n_merge ? 1 : 0);
   return SLM_OK;
 }
 

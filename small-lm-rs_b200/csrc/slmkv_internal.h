@@ -229,16 +229,20 @@ struct SharedToken {
   int32_t edge;  // its sequence's own edge
 };
 // An edge of the tree of block tables: a run of blocks that the tokens from
-// token0 on see, and no others. Its parts: [kv_head][split][row of the edge].
+// token0 on see, and no others. Its units: [kv_head][row tile].
 struct SharedEdge {
   int32_t parent;  // -1: none
   int32_t token0;
-  int32_t n_splits;
-  int32_t n_rows;  // tokens x query heads per KV head
-  int32_t part0;   // first part (row slots)
+  int32_t unit0, n_tiles, tile_tokens;
 };
-// One CTA: up to 16 rows (tokens x query heads of one KV head) over a run of
-// an edge's blocks.
+// The parts that an edge gave the rows of one tile and KV head: part s of row r
+// (tokens x query heads of the KV head) in slot part0 + s n_rows + r. None where
+// the rows' output is whole.
+struct SharedUnit {
+  int32_t part0, n_parts, n_rows, pad;
+};
+// Up to 8 rows (tokens x query heads of one KV head; a tensor-core item: up to
+// 128) over a run of an edge's blocks.
 struct SharedItem {
   int32_t slot, first_block, n_blocks, head;
   int32_t token0, n_tokens;
@@ -252,16 +256,27 @@ struct SharedAttentionLaunch {
   float* out;
   int32_t rotate;
   int32_t* status;  // [n_seq]
-  const SharedItem* items;
-  int32_t n_items;
+  const SharedItem* items;    // a list's next to each other
+  const int32_t* list_start;  // [n_lists + 1]
+  int32_t n_lists;
+  int32_t team;  // 1: a list is a CTA's, else a warp's
+  int32_t most_parts;  // of a row that is joined
+  const SharedItem* tc_items;  // runs that many rows see
+  int32_t n_tc_items;
+  CUtensorMap tmap_k, tmap_v;  // bf16 pools: the decode kernel's pool maps
   const SharedToken* tokens;
   const SharedEdge* edges;
+  const SharedUnit* units;
   const int32_t* merge_tokens;  // tokens whose output is joined from parts
   int32_t n_merge;
   float* part_acc;  // [slots][d]
   float2* part_ml;  // [slots]: maximum (exp2 domain), sum
 };
-int shared_rows_min_blocks(bool bf16);  // blocks that keep every warp of a CTA busy
+// Runs on the tensor cores (slmkv_shared_tc.cu): tiles of 128 rows x 4 blocks.
+constexpr int kSharedTcRows = 128, kSharedTcBlocks = 4;
+// CTAs an SM of the kernel for the other runs, four warps each.
+constexpr int kSharedCtasPerSm = 3, kSharedRows = 8;
+cudaError_t launch_shared_tc(const SharedAttentionLaunch& p, cudaStream_t s);
 cudaError_t launch_shared_attention(const SharedAttentionLaunch& p, cudaStream_t s);
 
 // ---- probabilities and draft verification (slmkv_sampling.cu) ----

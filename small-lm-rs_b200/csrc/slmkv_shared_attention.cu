@@ -8,6 +8,7 @@
 //   out = sum_e 2^(m_e - m) a_e / sum_e 2^(m_e - m) l_e
 // (attention.rs:677-759 and 195-399 with the softmax taken in parts).
 #include <cfloat>
+#include <type_traits>
 
 #include "slmkv_device.h"
 
@@ -18,10 +19,6 @@ constexpr int D = kHeadDim;
 constexpr float kScaleLog2e = 0.125f * 1.4426950408889634f;
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kStageBytes = 8192;  // K and V of one warp step: 32 bf16 tokens or 16 f32 ones
-constexpr int kStages = 2;
-constexpr int kQBytes = 4 * 3 * 512;  // Q fragments: 4 k-steps x 3 parts x 32 lanes x 16 B
-constexpr int kSmem = kQBytes + kWarps * kStages * kStageBytes;
 
 __device__ __forceinline__ uint32_t saddr(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -35,429 +32,578 @@ __device__ __forceinline__ void copy_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 // c += a b, 16 x 8 x 16, bf16 operands (a: rows, b: columns), f32 sums.
-__device__ __forceinline__ void mma(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                    uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// An f32 pair as three bf16 pairs, x = hi + mid + lo exactly: hi is cut off (so
-// it cannot overflow), mid rounds to nearest what is left, and 8 bits hold the
-// rest. |mid| < 2^-7 |x| and |lo| <= 2^-16 |x|, of either sign.
-struct Parts {
-  uint32_t hi, mid, lo;
-};
-__device__ __forceinline__ Parts split(float x, float y) {
-  const uint32_t xb = __float_as_uint(x), yb = __float_as_uint(y);
-  Parts r;
-  r.hi = __byte_perm(xb, yb, 0x7632);
-  const float x1 = x - __uint_as_float(xb & 0xffff0000u), y1 = y - __uint_as_float(yb & 0xffff0000u);
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r.mid) : "f"(y1), "f"(x1));
-  const float x2 = x1 - __uint_as_float(r.mid << 16), y2 = y1 - __uint_as_float(r.mid & 0xffff0000u);
-  r.lo = __byte_perm(__float_as_uint(x2), __float_as_uint(y2), 0x7632);
+// Transposes an 8 x 8 matrix of bf16 spread over the warp (a pair of a row a lane).
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
-// One CTA: 16 rows (16/G tokens x the G query heads of a key head) over a run
-// of blocks; its warps take turns at the run's steps. All operands are bf16
-// parts that hold the f32 (or bf16) values exactly, so scores and outputs are
-// f32 sums of exact products (f32 pages: the products of a mid or lo part with a
-// lo part, below 2^-23 of a term, are dropped). Fragments are loaded so that each thread copies, and reads back,
-// only its own 16-byte pieces: in the products' inner dimensions any order
-// serves, so thread (g, c) of a warp (g = lane / 4, c = lane % 4) takes
-//   K: token 8u + g, four consecutive values a k-step (one 16 B piece is one
-//      k-step of f32, two of bf16)
-//   V: tokens 2c, 2c+1, 2c+8, 2c+9 of 16, values 8g..8g+7; output tile j holds
-//      values 8n + j, so a thread ends with values 16c..16c+15 of rows g, g+8
-// which keeps global reads full sectors and needs no barrier in the loop.
+template <int BF16>
+struct RowsCfg {
+  static constexpr int kBlocks = BF16 ? 2 : 1;            // of a step
+  static constexpr int kBlockBytes = BF16 ? 4096 : 8192;   // K and V of 16 tokens
+  static constexpr int kStages = 2;
+  static constexpr int kStageBytes = kBlocks * kBlockBytes;
+  static constexpr int kWarpBytes = kStages * kStageBytes;
+  static constexpr int kPartBytes = 8 * (D * 4 + 8);  // a warp's rows: values, then (maximum, sum)
+  static constexpr int kSmem = kWarps * kWarpBytes;
+  static constexpr int kTeamSmem = kSmem + kWarps * kPartBytes;
+};
+
+__device__ __forceinline__ SharedItem load_item(const SharedItem* p) {
+  SharedItem it;
+  const int4 a = reinterpret_cast<const int4*>(p)[0], b = reinterpret_cast<const int4*>(p)[1];
+  it.slot = a.x;
+  it.first_block = a.y;
+  it.n_blocks = a.z;
+  it.head = a.w;
+  it.token0 = b.x;
+  it.n_tokens = b.y;
+  it.part = b.z;
+  it.mask_from = b.w;
+  return it;
+}
+
+// Up to 8 rows (tokens x the G query heads of a key head) over runs of
+// blocks: every warp has a list of such items, of about the same length for all
+// warps, and streams their blocks through its own stages without a break. Where
+// a warp would get few blocks, a CTA's four warps are a team: they share a list,
+// take turns at an item's steps and join their rows through shared memory.
+//
+// Tokens and head values fill the sixteen rows of the products, the queries
+// their eight columns:
+//   S^T (16 tokens x 8 rows) = K Q^T,  O^T (16 values x 8 rows, four times) = V^T P^T
+// so a decode step's few rows waste nothing. All operands are bf16 parts that
+// hold the f32 (or bf16) values exactly, so scores and outputs are f32 sums of
+// exact products (f32 pages: the products of a mid or lo part with a lo part,
+// below 2^-23 of a term, are dropped).
+//
+// Each thread copies, and reads back, only its own 16-byte pieces of a block: in
+// the products' inner dimensions any order serves, so thread (g, c) of a warp
+// (g = lane / 4, c = lane % 4) takes
+//   K: tokens g and g + 8, four consecutive values a k-step (a 16-byte piece is
+//      one k-step of f32, two of bf16)
+//   V: tokens 2c, 2c+1, 2c+8, 2c+9, values 8g..8g+7; value tile j holds the
+//      values 8n + 2j and 8n + 2j + 1, so a thread ends with values 8g..8g+7 of
+//      rows 2c and 2c + 1
+// which keeps global reads full sectors and needs no barrier but a team's.
+//
+// Bound by memory at the start, when every warp asks for its first stages, and
+// by the latency of a step's chain of products, maximum and powers after that.
 template <int BF16, int G>
-__global__ void __launch_bounds__(kThreads) shared_rows_kernel(const SharedAttentionLaunch p) {
-  constexpr int kTok = BF16 ? 32 : 16;      // tokens a warp takes a step
-  constexpr int kBlk = kTok / kBlockTokens;  // blocks a step
-  constexpr int kTiles = kTok / 8;           // 8-token score tiles a step
+__global__ void __launch_bounds__(kThreads, 3) shared_rows_kernel(const SharedAttentionLaunch p) {
+  using Cfg = RowsCfg<BF16>;
+  constexpr int NB = Cfg::kBlocks, kStages = Cfg::kStages;
   extern __shared__ __align__(16) uint8_t sm[];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
-  const SharedItem it = p.items[blockIdx.x];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  let_next_start();
+  const bool team = p.team != 0;
+  const int list = team ? static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x) * kWarps + warp;
+  if (list >= p.n_lists) return;
+  const int item0 = p.list_start[list], item1 = p.list_start[list + 1];
+  const int offset = team ? warp * NB : 0, stride = team ? kWarps * NB : NB;  // the warp's steps of an item
   const int Hkv = p.g.kv_heads, Hq = p.g.q_heads;
-  const int n_steps = (it.n_blocks + kBlk - 1) / kBlk;
-  const int mine = n_steps > warp ? (n_steps - warp + kWarps - 1) / kWarps : 0;  // steps warp, warp + 4, ...
-  const int32_t* table = p.g.block_table + static_cast<size_t>(it.slot) * p.g.max_blocks_per_seq + it.first_block;
-  const size_t esz = BF16 ? 2 : 4;
-  const size_t chunk = static_cast<size_t>(kBlockTokens) * D * esz;
-  const uint8_t* kbase = static_cast<const uint8_t*>(p.g.k) + static_cast<size_t>(p.layer) * p.g.layer_elems * esz;
-  const uint8_t* vbase = static_cast<const uint8_t*>(p.g.v) + static_cast<size_t>(p.layer) * p.g.layer_elems * esz;
-  uint8_t* stage0 = sm + kQBytes + warp * kStages * kStageBytes;
+  constexpr size_t esz = BF16 ? 2 : 4;
+  constexpr size_t chunk = static_cast<size_t>(kBlockTokens) * D * esz;
+  const size_t layer = static_cast<size_t>(p.layer) * p.g.layer_elems * esz;
+  const uint8_t* kbase = static_cast<const uint8_t*>(p.g.k) + layer + g * (D * esz) + 16 * c;
+  const uint8_t* vbase = static_cast<const uint8_t*>(p.g.v) + layer + 2 * c * (D * esz) + g * (8 * esz);
+  uint8_t* stage0 = sm + warp * Cfg::kWarpBytes;
   const uint32_t stage_addr = saddr(stage0) + lane * 16;
 
-  auto issue = [&](int n) {  // the warp's n-th step into stage n % kStages
-    const uint32_t dst = stage_addr + (n % kStages) * kStageBytes;
+  // The copies run ahead of the products, across the ends of items: their own
+  // place in the list, the next item's record and first block ids at hand.
+  auto table_of = [&](const SharedItem& it) {
+    return p.g.block_table + static_cast<size_t>(it.slot) * p.g.max_blocks_per_seq + it.first_block;
+  };
+  auto first_ids = [&](const SharedItem& it) { return lane < it.n_blocks ? table_of(it)[lane] : 0; };
+  SharedItem cur = load_item(p.items + item0);
+  SharedItem ahead = cur, ahead_next = load_item(p.items + min(item0 + 1, item1 - 1));
+  int ahead_at = item0, block = offset;  // the copies' item and its next block
+  int32_t ids = first_ids(ahead), ids_next = first_ids(ahead_next), window = 0;
+  auto issue = [&](int stage) {  // the next step's blocks, or nothing at the end
+    while (block >= ahead.n_blocks) {  // (an item may have no step for a warp of a team)
+      if (ahead_at + 1 >= item1) return;
+      ++ahead_at;
+      ahead = ahead_next;
+      ids = ids_next;
+      block = offset;
+      window = 0;
+      ahead_next = load_item(p.items + min(ahead_at + 1, item1 - 1));
+      ids_next = first_ids(ahead_next);
+    }
 #pragma unroll
-    for (int b = 0; b < kBlk; ++b) {
-      // a step's blocks past the run repeat the last one (masked below)
-      const int j = min((n * kWarps + warp) * kBlk + b, it.n_blocks - 1);
-      const size_t at = (static_cast<size_t>(pool_block(p.g, table[j])) * Hkv + it.head) * chunk;
-      constexpr int kP = BF16 ? 2 : 4;  // 16 B pieces of K a token row and thread
+    for (int b = 0; b < NB; ++b) {
+      // a step's block past the run repeats the last one (masked below)
+      const int j = min(block + b, ahead.n_blocks - 1);
+      // the ids at hand are those of a window of 32 blocks
+      if ((j >> 5) != window) {
+        window = j >> 5;
+        const int at = 32 * window + lane;
+        ids = at < ahead.n_blocks ? table_of(ahead)[at] : 0;
+      }
+      const int32_t id = pool_block(p.g, __shfl_sync(kFullMask, ids, j & 31));
+      const size_t at = (static_cast<size_t>(id) * Hkv + ahead.head) * chunk;
+      const uint32_t dst = stage_addr + stage * Cfg::kStageBytes + b * Cfg::kBlockBytes;
+      constexpr int kP = BF16 ? 2 : 4;  // 16-byte pieces of K a token and thread
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int i = 0; i < kP; ++i)
-          copy16(dst + ((b * 2 + u) * kP + i) * 512, kbase + at + (8 * u + g) * (D * esz) + 64 * i + 16 * c);
-      constexpr int kW = BF16 ? 1 : 2;  // pieces of V a token
+          copy16(dst + (u * kP + i) * 512, kbase + at + u * (8 * D * esz) + 64 * i);
+      constexpr int kW = BF16 ? 1 : 2;  // of V
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int i = 0; i < kW; ++i)
-          copy16(dst + kStageBytes / 2 + ((b * 4 + t) * kW + i) * 512,
-                 vbase + at + (2 * c + (t & 1) + 8 * (t >> 1)) * (D * esz) + g * (8 * esz) + 16 * i);
+          copy16(dst + Cfg::kBlockBytes / 2 + (t * kW + i) * 512,
+                 vbase + at + ((t & 1) + 8 * (t >> 1)) * (D * esz) + 16 * i);
     }
+    block += stride;
   };
 #pragma unroll
   for (int n = 0; n < kStages; ++n) {
-    if (n < mine) issue(n);
+    issue(n);
     copy_commit();
   }
 
-  // Q: warp s prepares k-step s of the 16 rows (rotated, scaled into the exp2
-  // domain, in three parts), in the order the fragments are read.
-  {
-    float4 qv[2];
-    const int d = BF16 ? 32 * (warp >> 1) + 8 * c + 4 * (warp & 1) : 16 * warp + 4 * c;
+  // the token of an item's row g
+  auto row_token = [&](const SharedItem& it) { return p.tokens[it.token0 + min(g / G, it.n_tokens - 1)]; };
+  SharedToken tk, tk_next = row_token(cur);
+  SharedItem next = cur;
+  int stage = 0;
+
+  for (int at = item0; at < item1; ++at) {
+    cur = next;
+    tk = tk_next;
+    // Q: rotated, scaled into the exp2 domain, in parts, kept in registers in
+    // the order of K's pieces
+    const int rows = cur.n_tokens * G;
+    uint2 q[4][3];
+    int qpos[2];
+    {
+      float4 x[4];
+      const float* src = p.q + (static_cast<size_t>(tk.row) * Hq + cur.head * G + g % G) * D;
+      const float2* rope = p.g.rope + static_cast<size_t>(tk.pos) * (D / 2);
+      auto value = [&](int s) { return BF16 ? 32 * (s >> 1) + 8 * c + 4 * (s & 1) : 16 * s + 4 * c; };
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = g + 8 * h, t = r / G;
-      qv[h] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (t < it.n_tokens) {
-        const SharedToken tk = p.tokens[it.token0 + t];
-        qv[h] = *reinterpret_cast<const float4*>(
-            p.q + (static_cast<size_t>(tk.row) * Hq + it.head * G + r % G) * D + d);
-        if (p.rotate)
-          qv[h] = rotate_quad(qv[h], *reinterpret_cast<const float4*>(p.g.rope + static_cast<size_t>(tk.pos) * (D / 2) + d / 2));
-        qv[h].x *= kScaleLog2e;
-        qv[h].y *= kScaleLog2e;
-        qv[h].z *= kScaleLog2e;
-        qv[h].w *= kScaleLog2e;
+      for (int s = 0; s < 4; ++s) x[s] = *reinterpret_cast<const float4*>(src + value(s));
+      if (at + 1 < item1) {  // what the next item needs is on its way meanwhile
+        next = load_item(p.items + at + 1);
+        tk_next = row_token(next);
+      }
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        float4 y = x[s];
+        if (p.rotate) y = rotate_quad(y, *reinterpret_cast<const float4*>(rope + value(s) / 2));
+        const bool live = g < rows;
+        const Parts a = split_pair(live ? y.x * kScaleLog2e : 0.f, live ? y.y * kScaleLog2e : 0.f);
+        const Parts b = split_pair(live ? y.z * kScaleLog2e : 0.f, live ? y.w * kScaleLog2e : 0.f);
+        q[s][0] = make_uint2(a.hi, b.hi);
+        q[s][1] = make_uint2(a.mid, b.mid);
+        q[s][2] = make_uint2(a.lo, b.lo);
+      }
+      // the positions of rows 2c and 2c + 1 lie with the threads of those rows
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int pos = __shfl_sync(kFullMask, tk.pos, 4 * (2 * c + e));
+        qpos[e] = 2 * c + e < rows ? pos : INT32_MAX;
       }
     }
-    const Parts a0 = split(qv[0].x, qv[0].y), a1 = split(qv[1].x, qv[1].y);
-    const Parts a2 = split(qv[0].z, qv[0].w), a3 = split(qv[1].z, qv[1].w);
-    uint4* dst = reinterpret_cast<uint4*>(sm) + warp * 96 + lane;
-    dst[0] = make_uint4(a0.hi, a1.hi, a2.hi, a3.hi);
-    dst[32] = make_uint4(a0.mid, a1.mid, a2.mid, a3.mid);
-    dst[64] = make_uint4(a0.lo, a1.lo, a2.lo, a3.lo);
-  }
-  int qpos[2];
+    float o[4][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, fin[2] = {0.f, 0.f};
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int t = (g + 8 * h) / G;
-    qpos[h] = t < it.n_tokens ? p.tokens[it.token0 + t].pos : INT32_MAX;
-  }
-  __syncthreads();
-  const uint4* qf = reinterpret_cast<const uint4*>(sm) + lane;
+    for (int j = 0; j < 4; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
 
-  float o[8][4];
+    for (int n = offset; n < cur.n_blocks; n += stride) {
+      copy_wait<kStages - 1>();
+      const uint8_t* st0 = stage0 + stage * Cfg::kStageBytes + lane * 16;
+      // scores: the products with a mid or lo part apart from those of two hi
+      // parts, since a tensor core's sum is cut off at each step
+      float s[NB][4], small[NB][4];
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
+      for (int k = 0; k < NB; ++k) {
+        s[k][0] = s[k][1] = s[k][2] = s[k][3] = 0.f;
+        small[k][0] = small[k][1] = small[k][2] = small[k][3] = 0.f;
+      }
+      if constexpr (BF16) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, fin[2] = {0.f, 0.f};
-  const int run_end = (it.first_block + it.n_blocks) * kBlockTokens;
-
-  for (int n = 0; n < mine; ++n) {
-    copy_wait<kStages - 1>();
-    const uint8_t* st = stage0 + (n % kStages) * kStageBytes + lane * 16;
-    float s[kTiles][4];
+        for (int i = 0; i < 2; ++i) {
+          uint4 k0[NB], k1[NB];
 #pragma unroll
-    for (int u = 0; u < kTiles; ++u) s[u][0] = s[u][1] = s[u][2] = s[u][3] = 0.f;
-    if constexpr (BF16) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        uint4 kf[kTiles];
-#pragma unroll
-        for (int u = 0; u < kTiles; ++u) kf[u] = *reinterpret_cast<const uint4*>(st + (u * 2 + i) * 512);
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int part = 2; part >= 0; --part) {  // small terms first
-            const uint4 a = qf[(2 * i + h) * 96 + part * 32];
-#pragma unroll
-            for (int u = 0; u < kTiles; ++u) mma(s[u], a, h ? kf[u].z : kf[u].x, h ? kf[u].w : kf[u].y);
+          for (int k = 0; k < NB; ++k) {
+            k0[k] = *reinterpret_cast<const uint4*>(st0 + k * Cfg::kBlockBytes + i * 512);
+            k1[k] = *reinterpret_cast<const uint4*>(st0 + k * Cfg::kBlockBytes + (2 + i) * 512);
           }
-      }
-    } else {
-      // the small products apart: a tensor core sum is cut off at each step,
-      // so the large ones take as few as they can
-      float small[kTiles][4];
 #pragma unroll
-      for (int u = 0; u < kTiles; ++u) small[u][0] = small[u][1] = small[u][2] = small[u][3] = 0.f;
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint4 ah = qf[i * 96], am = qf[i * 96 + 32], al = qf[i * 96 + 64];
+            for (int part = 2; part >= 0; --part)
 #pragma unroll
-        for (int u = 0; u < kTiles; ++u) {
-          const float4 k4 = *reinterpret_cast<const float4*>(st + (u * 4 + i) * 512);
-          const Parts b0 = split(k4.x, k4.y), b1 = split(k4.z, k4.w);
-          mma(small[u], al, b0.hi, b1.hi);
-          mma(small[u], ah, b0.lo, b1.lo);
-          mma(small[u], am, b0.mid, b1.mid);
-          mma(small[u], am, b0.hi, b1.hi);
-          mma(small[u], ah, b0.mid, b1.mid);
-          mma(s[u], ah, b0.hi, b1.hi);
+              for (int k = 0; k < NB; ++k) {
+                const uint2 x = q[2 * i + h][part];
+                mma(part ? small[k] : s[k], word(k0[k], 2 * h), word(k1[k], 2 * h), word(k0[k], 2 * h + 1),
+                    word(k1[k], 2 * h + 1), x.x, x.y);
+              }
         }
+      } else {
+        float other[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float4 k0 = *reinterpret_cast<const float4*>(st0 + i * 512);
+          const float4 k1 = *reinterpret_cast<const float4*>(st0 + (4 + i) * 512);
+          const Parts a0 = split_pair(k0.x, k0.y), a1 = split_pair(k1.x, k1.y);
+          const Parts a2 = split_pair(k0.z, k0.w), a3 = split_pair(k1.z, k1.w);
+          const uint2(&x)[3] = q[i];
+          mma(small[0], a0.lo, a1.lo, a2.lo, a3.lo, x[0].x, x[0].y);
+          mma(other, a0.hi, a1.hi, a2.hi, a3.hi, x[2].x, x[2].y);
+          mma(s[0], a0.hi, a1.hi, a2.hi, a3.hi, x[0].x, x[0].y);
+          mma(small[0], a0.mid, a1.mid, a2.mid, a3.mid, x[1].x, x[1].y);
+          mma(other, a0.hi, a1.hi, a2.hi, a3.hi, x[1].x, x[1].y);
+          mma(small[0], a0.mid, a1.mid, a2.mid, a3.mid, x[0].x, x[0].y);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) small[0][e] += other[e];
       }
+      // causal: a row sees the positions up to its own; a step's last block may
+      // lie past the run
+      const int kp = (cur.first_block + n) * kBlockTokens;
+      const bool masked = kp + NB * kBlockTokens > cur.mask_from || n + NB > cur.n_blocks;
+      const int end = (cur.first_block + cur.n_blocks) * kBlockTokens;
+      float corr[2], mx[2] = {m[0], m[1]};
 #pragma unroll
-      for (int u = 0; u < kTiles; ++u)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[u][e] += small[u][e];
-    }
-    // causal: a row sees the positions up to its own; a run ends at run_end
-    const int kp0 = (it.first_block + (n * kWarps + warp) * kBlk) * kBlockTokens;
-    if (kp0 + kTok > it.mask_from || kp0 + kTok > run_end) {
-#pragma unroll
-      for (int u = 0; u < kTiles; ++u)
+      for (int k = 0; k < NB; ++k)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int kp = kp0 + 8 * u + 2 * c + (e & 1);
-          const bool seen = kp < run_end && kp <= qpos[e >> 1];
-          fin[e >> 1] = fmaf(seen ? s[u][e] : 0.f, 0.f, fin[e >> 1]);
-          if (!seen) s[u][e] = -INFINITY;
-        }
-    } else {
-#pragma unroll
-      for (int u = 0; u < kTiles; ++u)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) fin[e >> 1] = fmaf(s[u][e], 0.f, fin[e >> 1]);
-    }
-    float corr[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float mx = m[h];
-#pragma unroll
-      for (int u = 0; u < kTiles; ++u) mx = fmaxf(mx, fmaxf(s[u][2 * h], s[u][2 * h + 1]));
-      mx = fmaxf(mx, __shfl_xor_sync(kFullMask, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(kFullMask, mx, 2));
-      const float base = mx == -INFINITY ? 0.f : mx;  // nothing seen yet: every weight is 2^-inf = 0
-      corr[h] = exp2_fast(m[h] - base);
-      m[h] = mx;
-      float sum = 0.f;
-#pragma unroll
-      for (int u = 0; u < kTiles; ++u)
-#pragma unroll
-        for (int e = 2 * h; e < 2 * h + 2; ++e) {
-          s[u][e] = exp2_fast(s[u][e] - base);
-          sum += s[u][e];
-        }
-      l[h] = fmaf(l[h], corr[h], sum);
-    }
-    uint4 pf[kBlk][3];
-#pragma unroll
-    for (int b = 0; b < kBlk; ++b) {
-      const Parts a0 = split(s[2 * b][0], s[2 * b][1]), a1 = split(s[2 * b][2], s[2 * b][3]);
-      const Parts a2 = split(s[2 * b + 1][0], s[2 * b + 1][1]), a3 = split(s[2 * b + 1][2], s[2 * b + 1][3]);
-      pf[b][0] = make_uint4(a0.hi, a1.hi, a2.hi, a3.hi);
-      pf[b][1] = make_uint4(a0.mid, a1.mid, a2.mid, a3.mid);
-      pf[b][2] = make_uint4(a0.lo, a1.lo, a2.lo, a3.lo);
-    }
-    // P V of this step in fresh sums, added to the running output in f32: the
-    // tensor cores cut off their running sums, which over a long run would
-    // show as a bias
-    const uint8_t* sv = st + kStageBytes / 2;
-    if constexpr (BF16) {
-      uint4 vf[kBlk][4];
-#pragma unroll
-      for (int b = 0; b < kBlk; ++b)
-#pragma unroll
-        for (int t = 0; t < 4; ++t) vf[b][t] = *reinterpret_cast<const uint4*>(sv + (b * 4 + t) * 512);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        uint32_t b0[kBlk], b1[kBlk];
-#pragma unroll
-        for (int b = 0; b < kBlk; ++b) {
-          const uint32_t sel = (j & 1) ? 0x7632 : 0x5410;
-          auto word = [&](const uint4& v) { return (j >> 1) == 0 ? v.x : (j >> 1) == 1 ? v.y : (j >> 1) == 2 ? v.z : v.w; };
-          b0[b] = __byte_perm(word(vf[b][0]), word(vf[b][1]), sel);
-          b1[b] = __byte_perm(word(vf[b][2]), word(vf[b][3]), sel);
+          float& x = s[k][e];
+          x += small[k][e];
+          const int pos = kp + 16 * k + g + 8 * (e >> 1);
+          const bool seen = !masked || (pos <= qpos[e & 1] && pos < end);
+          fin[e & 1] = fmaf(seen ? x : 0.f, 0.f, fin[e & 1]);
+          if (!seen) x = -INFINITY;
         }
 #pragma unroll
-        for (int part = 2; part >= 0; --part)
+      for (int k = 0; k < NB; ++k)
 #pragma unroll
-          for (int b = 0; b < kBlk; ++b) mma(acc, pf[b][part], b0[b], b1[b]);
+        for (int e = 0; e < 2; ++e) mx[e] = fmax3(mx[e], s[k][e], s[k][e + 2]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[j][e] = fmaf(o[j][e], corr[e >> 1], acc[e]);
+      for (int x = 4; x < 32; x <<= 1)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) mx[e] = fmaxf(mx[e], __shfl_xor_sync(kFullMask, mx[e], x));
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float base = mx[e] == -INFINITY ? 0.f : mx[e];  // nothing seen yet: every weight is 2^-inf = 0
+        corr[e] = exp2_fast(m[e] - base);
+        m[e] = mx[e];
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < NB; ++k)
+#pragma unroll
+          for (int h = e; h < 4; h += 2) {
+            s[k][h] = exp2_fast(s[k][h] - base);
+            sum += s[k][h];
+          }
+        l[e] = fmaf(l[e], corr[e], sum);
       }
-    } else {
+      uint32_t pt[NB][3][2];  // P^T in parts: rows g, tokens 2c, 2c + 1 (+ 8)
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        float4 vf[4];
+      for (int k = 0; k < NB; ++k)
 #pragma unroll
-        for (int t = 0; t < 4; ++t) vf[t] = *reinterpret_cast<const float4*>(sv + (t * 2 + half) * 512);
+        for (int h = 0; h < 2; ++h) {
+          const Parts x = split_pair(s[k][2 * h], s[k][2 * h + 1]);
+          pt[k][0][h] = transpose8(x.hi);
+          pt[k][1][h] = transpose8(x.mid);
+          pt[k][2][h] = transpose8(x.lo);
+        }
+      // V^T P^T of this step in fresh sums, added to the running output in f32:
+      // cut off at each step, a long run's sum would show a bias
+      const uint8_t* sv = st0 + Cfg::kBlockBytes / 2;
+      float acc[4][4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          auto word = [&](const float4& v) { return q == 0 ? v.x : q == 1 ? v.y : q == 2 ? v.z : v.w; };
-          const Parts b0 = split(word(vf[0]), word(vf[1])), b1 = split(word(vf[2]), word(vf[3]));
-          float acc[4] = {0.f, 0.f, 0.f, 0.f};
-          mma(acc, pf[0][2], b0.hi, b1.hi);
-          mma(acc, pf[0][0], b0.lo, b1.lo);
-          mma(acc, pf[0][1], b0.mid, b1.mid);
-          mma(acc, pf[0][1], b0.hi, b1.hi);
-          mma(acc, pf[0][0], b0.mid, b1.mid);
-          mma(acc, pf[0][0], b0.hi, b1.hi);
-          const int j = half * 4 + q;
+      for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+      if constexpr (BF16) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[j][e] = fmaf(o[j][e], corr[e >> 1], acc[e]);
+        for (int k = 0; k < NB; ++k) {
+          uint4 v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint4*>(sv + k * Cfg::kBlockBytes + i * 512);
+#pragma unroll
+          for (int part = 2; part >= 0; --part)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              mma(acc[j], __byte_perm(word(v[0], j), word(v[1], j), 0x5410),
+                  __byte_perm(word(v[0], j), word(v[1], j), 0x7632), __byte_perm(word(v[2], j), word(v[3], j), 0x5410),
+                  __byte_perm(word(v[2], j), word(v[3], j), 0x7632), pt[k][part][0], pt[k][part][1]);
+        }
+      } else {
+        const uint32_t(&x)[3][2] = pt[0];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float2 v[4];  // values 8g + 2j, 8g + 2j + 1 of the four tokens
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            v[i] = *reinterpret_cast<const float2*>(sv + (2 * i + (j >> 1)) * 512 + 8 * (j & 1));
+          const Parts a0 = split_pair(v[0].x, v[1].x), a1 = split_pair(v[0].y, v[1].y);
+          const Parts a2 = split_pair(v[2].x, v[3].x), a3 = split_pair(v[2].y, v[3].y);
+          mma(acc[j], a0.lo, a1.lo, a2.lo, a3.lo, x[0][0], x[0][1]);
+          mma(acc[j], a0.hi, a1.hi, a2.hi, a3.hi, x[2][0], x[2][1]);
+          mma(acc[j], a0.mid, a1.mid, a2.mid, a3.mid, x[1][0], x[1][1]);
+          mma(acc[j], a0.mid, a1.mid, a2.mid, a3.mid, x[0][0], x[0][1]);
+          mma(acc[j], a0.hi, a1.hi, a2.hi, a3.hi, x[1][0], x[1][1]);
+          mma(acc[j], a0.hi, a1.hi, a2.hi, a3.hi, x[0][0], x[0][1]);
         }
       }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[j][e] = fmaf(o[j][e], corr[e & 1], acc[j][e]);
+      issue(stage);
+      copy_commit();
+      stage = stage + 1 == kStages ? 0 : stage + 1;
     }
-    if (n + kStages < mine) issue(n + kStages);
-    copy_commit();
+    // Deliver the rows: to the output where the run holds all that they see,
+    // else as parts. softmax.rs:17-22: a score that is not finite fails the
+    // row's sequence.
+    const bool whole = cur.part < 0;
+    auto deliver = [&](int r, int row, int d0, float4 x, float4 y, float mx, float sum) {
+      const float f = whole ? 1.f / sum : 1.f;
+      float* dst = whole ? p.out + (static_cast<size_t>(row) * Hq + cur.head * G + r % G) * D
+                         : p.part_acc + (static_cast<size_t>(cur.part) + r) * D;
+      if (!whole && d0 == 0) p.part_ml[static_cast<size_t>(cur.part) + r] = make_float2(mx, sum);
+      float4* d4 = reinterpret_cast<float4*>(dst + d0);
+      d4[0] = make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
+      d4[1] = make_float4(y.x * f, y.y * f, y.z * f, y.w * f);
+    };
+    uint8_t* parts = sm + Cfg::kSmem;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) l[e] += __shfl_xor_sync(kFullMask, l[e], x);
+      const int src = 4 * (2 * c + e), out_row = __shfl_sync(kFullMask, tk.row, src);
+      const int seq = __shfl_sync(kFullMask, tk.seq, src), r = 2 * c + e;
+      if (r < rows) {
+        if ((!(fin[e] == 0.f) || (whole && !team && !(isfinite(l[e]) && l[e] > 0.f))) && p.status)
+          atomicOr(&p.status[seq], kStatusNonFiniteScore);
+        const float4 x = make_float4(o[0][e], o[0][e + 2], o[1][e], o[1][e + 2]);
+        const float4 y = make_float4(o[2][e], o[2][e + 2], o[3][e], o[3][e + 2]);
+        if (!team) {
+          deliver(r, out_row, 8 * g, x, y, m[e], l[e]);
+        } else {
+          uint8_t* mine = parts + warp * Cfg::kPartBytes;
+          float4* d4 = reinterpret_cast<float4*>(mine + r * (D * 4) + 32 * g);
+          d4[0] = x;
+          d4[1] = y;
+          if (g == 0) reinterpret_cast<float2*>(mine + 8 * D * 4)[r] = make_float2(m[e], l[e]);
+        }
+      }
+      __syncwarp();
+    }
+    if (team) {  // (every warp of the CTA has the same list)
+      __syncthreads();
+      const int r = static_cast<int>(threadIdx.x) >> 3, d0 = (static_cast<int>(threadIdx.x) & 7) * 8;
+      if (r < rows) {
+        float2 ml[kWarps];
+        float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) {
+          ml[k] = reinterpret_cast<const float2*>(parts + k * Cfg::kPartBytes + 8 * D * 4)[r];
+          mx = fmaxf(mx, ml[k].x);
+        }
+        const float base = mx == -INFINITY ? 0.f : mx;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) {
+          const float f = exp2_fast(ml[k].x - base);
+          const float4* v = reinterpret_cast<const float4*>(parts + k * Cfg::kPartBytes + r * (D * 4) + 4 * d0);
+          const float4 a = v[0], b = v[1];
+          sum = fmaf(ml[k].y, f, sum);
+          x = make_float4(fmaf(a.x, f, x.x), fmaf(a.y, f, x.y), fmaf(a.z, f, x.z), fmaf(a.w, f, x.w));
+          y = make_float4(fmaf(b.x, f, y.x), fmaf(b.y, f, y.y), fmaf(b.z, f, y.z), fmaf(b.w, f, y.w));
+        }
+        const SharedToken own = p.tokens[cur.token0 + r / G];
+        if (whole && !(isfinite(sum) && sum > 0.f) && p.status) atomicOr(&p.status[own.seq], kStatusNonFiniteScore);
+        deliver(r, own.row, d0, x, y, mx, sum);
+      }
+      __syncthreads();
+    }
   }
   copy_wait<0>();
-  // softmax.rs:17-22: a score that is not finite fails the row's sequence
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    l[h] += __shfl_xor_sync(kFullMask, l[h], 1);
-    l[h] += __shfl_xor_sync(kFullMask, l[h], 2);
-    const int t = (g + 8 * h) / G;
-    if (t < it.n_tokens && !(fin[h] == 0.f) && p.status)
-      atomicOr(&p.status[p.tokens[it.token0 + t].seq], kStatusNonFiniteScore);
-  }
-  // The warps' parts of a row, merged through shared memory (each warp's own
-  // stages: its copies are complete, its lanes have read them).
-  __syncwarp();
-  float* part = reinterpret_cast<float*>(stage0);  // [16][64], then (m, l) [16]
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float* row = part + (g + 8 * h) * D + 16 * c;
-#pragma unroll
-    for (int e = 0; e < 2; ++e)  // column 2c + e holds values 16c + 8e + j
-#pragma unroll
-      for (int j = 0; j < 8; j += 4)
-        *reinterpret_cast<float4*>(row + 8 * e + j) =
-            make_float4(o[j][2 * h + e], o[j + 1][2 * h + e], o[j + 2][2 * h + e], o[j + 3][2 * h + e]);
-    if (c == 0) reinterpret_cast<float2*>(part + 16 * D)[g + 8 * h] = make_float2(m[h], l[h]);
-  }
-  __syncthreads();
-  const int r = tid >> 3, d0 = (tid & 7) * 8, t = r / G;
-  if (t >= it.n_tokens) return;
-  float mm = -INFINITY;
-  float2 ml[kWarps];
-  const int used = min(kWarps, n_steps);
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    ml[w] = reinterpret_cast<const float2*>(sm + kQBytes + w * kStages * kStageBytes + 16 * D * 4)[r];
-    if (w < used) mm = fmaxf(mm, ml[w].x);
-  }
-  const float base = mm == -INFINITY ? 0.f : mm;
-  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, ll = 0.f;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w >= used) break;
-    const float wt = exp2_fast(ml[w].x - base);
-    ll = fmaf(ml[w].y, wt, ll);
-    const float* src = reinterpret_cast<const float*>(sm + kQBytes + w * kStages * kStageBytes) + r * D + d0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] = fmaf(src[i], wt, acc[i]);
-  }
-  const SharedToken tk = p.tokens[it.token0 + t];
-  float* dst;
-  float scale = 1.f;
-  if (it.part < 0) {  // the run holds all that these rows see
-    if (!(isfinite(ll) && ll > 0.f) && p.status) atomicOr(&p.status[tk.seq], kStatusNonFiniteScore);
-    scale = 1.f / ll;
-    dst = p.out + (static_cast<size_t>(tk.row) * Hq + it.head * G + r % G) * D;
-  } else {
-    const size_t slot = static_cast<size_t>(it.part) + r;
-    dst = p.part_acc + slot * D;
-    if ((tid & 7) == 0) p.part_ml[slot] = make_float2(mm, ll);
-  }
-  *reinterpret_cast<float4*>(dst + d0) = make_float4(acc[0] * scale, acc[1] * scale, acc[2] * scale, acc[3] * scale);
-  *reinterpret_cast<float4*>(dst + d0 + 4) = make_float4(acc[4] * scale, acc[5] * scale, acc[6] * scale, acc[7] * scale);
+  // The tensor-core kernel, under which this one may have run (it reads nothing
+  // of it), is part of what the joining kernel waits for.
+  wait_for_previous();
 }
 
-// Joins a row's parts: one CTA per (token, query head), a warp per quarter of
-// the parts, lane l holding values 2l, 2l + 1.
-__global__ void __launch_bounds__(kThreads) shared_merge_kernel(const SharedAttentionLaunch p) {
-  __shared__ float2 s_ml[kWarps];
-  __shared__ float2 s_acc[kWarps][32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// Joins rows' parts: a CTA takes one token and 8 / W query heads, W warps a row
+// (the more parts a row has, the more), lane l holding values 2l, 2l + 1. The
+// parts of a row are those of the edges from its own up to the root. The plan is
+// read while the kernels before finish; what is left then is one round of reads
+// for a row of up to kBatch parts an edge.
+constexpr int kMergeThreads = 256;
+constexpr int kMergeDepth = 4;  // edges whose units are read ahead
+template <int W>
+__global__ void __launch_bounds__(kMergeThreads) shared_merge_kernel(const SharedAttentionLaunch p) {
+  __shared__ float2 s_ml[8];
+  __shared__ float2 s_acc[8][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, share = warp % W;
   const int Hq = p.g.q_heads, G = Hq / p.g.kv_heads;
-  const int k = p.merge_tokens[blockIdx.x], hq = blockIdx.y, head = hq / G, gq = hq % G;
+  const int k = p.merge_tokens[blockIdx.x], hq = blockIdx.y * (8 / W) + warp / W;
+  const bool live = hq < Hq;
+  const int head = min(hq, Hq - 1) / G, gq = min(hq, Hq - 1) % G;
   const SharedToken tk = p.tokens[k];
+  // parts of the row on one edge: the first slot, their number and their distance
+  struct Run {
+    size_t slot0;
+    int n_parts, n_rows;
+  };
+  auto run_of = [&](int e, int& parent) {
+    const SharedEdge ed = p.edges[e];
+    parent = ed.parent;
+    const int tile = (k - ed.token0) / ed.tile_tokens;
+    const SharedUnit u = p.units[ed.unit0 + head * ed.n_tiles + tile];
+    return Run{static_cast<size_t>(u.part0) + (k - ed.token0 - tile * ed.tile_tokens) * G + gq, u.n_parts, u.n_rows};
+  };
+  Run runs[kMergeDepth];
+  int e = tk.edge, depth = 0;
+#pragma unroll
+  for (int d = 0; d < kMergeDepth; ++d) {
+    if (e < 0) break;
+    int parent;
+    runs[d] = run_of(e, parent);
+    e = parent;
+    depth = d + 1;
+  }
+  wait_for_previous();
   float m = -INFINITY, l = 0.f;
   float2 a = make_float2(0.f, 0.f);
-  for (int e = tk.edge; e >= 0; e = p.edges[e].parent) {  // the edges from the row's own up to the root
-    const SharedEdge ed = p.edges[e];
-    const int row = (k - ed.token0) * G + gq;
-    for (int s = warp; s < ed.n_splits; s += kWarps) {
-      const size_t slot =
-          static_cast<size_t>(ed.part0) + (static_cast<size_t>(head) * ed.n_splits + s) * ed.n_rows + row;
-      const float2 ml = p.part_ml[slot];
-      const float2 v = reinterpret_cast<const float2*>(p.part_acc + slot * D)[lane];
-      const float mx = fmaxf(m, ml.x), base = mx == -INFINITY ? 0.f : mx;
-      const float w0 = exp2_fast(m - base), w1 = exp2_fast(ml.x - base);
-      l = l * w0 + ml.y * w1;
-      a.x = a.x * w0 + v.x * w1;
-      a.y = a.y * w0 + v.y * w1;
+  bool any = false;
+  auto add = [&](const Run& u) {
+    any = any || u.n_parts > 0;
+    constexpr int kBatch = 8;  // parts in flight
+    for (int s = share; s < u.n_parts; s += W * kBatch) {
+      float2 ml[kBatch], v[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const bool in = s + i * W < u.n_parts;
+        const size_t slot = u.slot0 + static_cast<size_t>(in ? s + i * W : s) * u.n_rows;
+        ml[i] = in ? p.part_ml[slot] : make_float2(-INFINITY, 0.f);
+        v[i] = in ? reinterpret_cast<const float2*>(p.part_acc + slot * D)[lane] : make_float2(0.f, 0.f);
+      }
+      float mx = m;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) mx = fmaxf(mx, ml[i].x);
+      const float base = mx == -INFINITY ? 0.f : mx, w0 = exp2_fast(m - base);
       m = mx;
+      l *= w0;
+      a.x *= w0;
+      a.y *= w0;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const float w = exp2_fast(ml[i].x - base);
+        l = fmaf(ml[i].y, w, l);
+        a.x = fmaf(v[i].x, w, a.x);
+        a.y = fmaf(v[i].y, w, a.y);
+      }
+    }
+  };
+#pragma unroll
+  for (int d = 0; d < kMergeDepth; ++d)
+    if (d < depth) add(runs[d]);
+  while (e >= 0) {  // deeper trees
+    int parent;
+    const Run u = run_of(e, parent);
+    e = parent;
+    add(u);
+  }
+  if constexpr (W > 1) {
+    if (lane == 0) s_ml[warp] = make_float2(m, l);
+    s_acc[warp][lane] = a;
+    __syncthreads();
+    if (share) return;
+    float mm = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < W; ++w) mm = fmaxf(mm, s_ml[warp + w].x);
+    const float base = mm == -INFINITY ? 0.f : mm;
+    l = 0.f;
+    a = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float wt = exp2_fast(s_ml[warp + w].x - base);
+      l = fmaf(s_ml[warp + w].y, wt, l);
+      a.x = fmaf(s_acc[warp + w][lane].x, wt, a.x);
+      a.y = fmaf(s_acc[warp + w][lane].y, wt, a.y);
     }
   }
-  if (lane == 0) s_ml[warp] = make_float2(m, l);
-  s_acc[warp][lane] = a;
-  __syncthreads();
-  if (warp) return;
-  float mm = -INFINITY;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, s_ml[w].x);
-  const float base = mm == -INFINITY ? 0.f : mm;
-  l = 0.f;
-  a = make_float2(0.f, 0.f);
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    const float wt = exp2_fast(s_ml[w].x - base);
-    l = fmaf(s_ml[w].y, wt, l);
-    a.x = fmaf(s_acc[w][lane].x, wt, a.x);
-    a.y = fmaf(s_acc[w][lane].y, wt, a.y);
-  }
+  if (!live || !any) return;  // (none: another head's run was cut, this one's output is whole)
   if (lane == 0 && !(isfinite(l) && l > 0.f) && p.status) atomicOr(&p.status[tk.seq], kStatusNonFiniteScore);
   const float inv = 1.f / l;
   reinterpret_cast<float2*>(p.out + (static_cast<size_t>(tk.row) * Hq + hq) * D)[lane] =
       make_float2(a.x * inv, a.y * inv);
 }
 
+// Launches with or without the start under the kernel before.
+template <typename Kernel>
+cudaError_t launch(Kernel kernel, dim3 grid, int threads, int smem, bool early, const SharedAttentionLaunch& p,
+                   cudaStream_t s) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = early ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
 }  // namespace
 
-int shared_rows_min_blocks(bool bf16) { return kWarps * (bf16 ? 2 : 1); }
-
 cudaError_t launch_shared_attention(const SharedAttentionLaunch& p, cudaStream_t s) {
+  cudaError_t e = launch_shared_tc(p, s);
+  if (e != cudaSuccess) return e;
   int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+  e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   static unsigned long long configured[8] = {};  // per variant, one bit per device
-  auto run = [&](auto kernel, int v) {
+  auto run = [&](auto kernel, int v, int smem, int team_smem) {
+    if (p.team) smem = team_smem;
     if (dev >= 64 || !(configured[v] & (1ull << dev))) {
-      const cudaError_t a = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+      const cudaError_t a = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, team_smem);
       if (a != cudaSuccess) return a;
       if (dev < 64) configured[v] |= 1ull << dev;
     }
-    kernel<<<p.n_items, kThreads, kSmem, s>>>(p);
-    return cudaGetLastError();
+    const int lists = p.team ? 1 : kWarps;  // a CTA's
+    // under the tensor-core kernel where there is one: what both read was
+    // complete when that one started
+    return launch(kernel, dim3((p.n_lists + lists - 1) / lists), kThreads, smem, p.n_tc_items > 0, p, s);
   };
-  const int G = p.g.q_heads / p.g.kv_heads;
-  const int v = (p.g.bf16 ? 4 : 0);
-  switch (G + (p.g.bf16 ? 16 : 0)) {
-    case 1: e = run(shared_rows_kernel<0, 1>, v); break;
-    case 2: e = run(shared_rows_kernel<0, 2>, v + 1); break;
-    case 4: e = run(shared_rows_kernel<0, 4>, v + 2); break;
-    case 8: e = run(shared_rows_kernel<0, 8>, v + 3); break;
-    case 17: e = run(shared_rows_kernel<1, 1>, v); break;
-    case 18: e = run(shared_rows_kernel<1, 2>, v + 1); break;
-    case 20: e = run(shared_rows_kernel<1, 4>, v + 2); break;
-    case 24: e = run(shared_rows_kernel<1, 8>, v + 3); break;
-    default: return cudaErrorInvalidValue;
-  }
+  auto of_group = [&](auto bf16, int v) {
+    constexpr int B = decltype(bf16)::value;
+    using Cfg = RowsCfg<B>;
+    switch (p.g.q_heads / p.g.kv_heads) {
+      case 1: return run(shared_rows_kernel<B, 1>, v, Cfg::kSmem, Cfg::kTeamSmem);
+      case 2: return run(shared_rows_kernel<B, 2>, v + 1, Cfg::kSmem, Cfg::kTeamSmem);
+      case 4: return run(shared_rows_kernel<B, 4>, v + 2, Cfg::kSmem, Cfg::kTeamSmem);
+      case 8: return run(shared_rows_kernel<B, 8>, v + 3, Cfg::kSmem, Cfg::kTeamSmem);
+      default: return cudaErrorInvalidValue;
+    }
+  };
+  e = p.g.bf16 ? of_group(std::integral_constant<int, 1>{}, 4) : of_group(std::integral_constant<int, 0>{}, 0);
   if (e != cudaSuccess || p.n_merge == 0) return e;
-  shared_merge_kernel<<<dim3(p.n_merge, p.g.q_heads), kThreads, 0, s>>>(p);
-  return cudaGetLastError();
+  // a warp a row while rows fill the SMs or have few parts
+  const int64_t rows = static_cast<int64_t>(p.n_merge) * p.g.q_heads;
+  if (p.most_parts > 16 && rows * 8 <= 148 * 64)
+    return launch(shared_merge_kernel<8>, dim3(p.n_merge, p.g.q_heads), kMergeThreads, 0, true, p, s);
+  return launch(shared_merge_kernel<1>, dim3(p.n_merge, (p.g.q_heads + 7) / 8), kMergeThreads, 0, true, p, s);
 }
 
 }  // namespace slmkv

@@ -232,6 +232,19 @@ def _stream_ptr(stream=None):
     return C.c_void_p(s.cuda_stream)
 
 
+_torch_module = None
+
+
+def _torch():
+    """torch, imported at the first use."""
+    global _torch_module
+    if _torch_module is None:
+        import torch
+
+        _torch_module = torch
+    return _torch_module
+
+
 def _ptr(t) -> C.c_void_p:
     if t is None:
         return C.c_void_p(0)
@@ -342,8 +355,7 @@ class KvPool:
         [num_layers, num_blocks, kv_heads, 16, head_dim] of its element type,
         indexed by the block ids of ``KvCache.blocks``. The views do not keep
         the pool alive; order their use with the pool's stream."""
-        import torch
-
+        torch = _torch()
         k, v, n = C.c_int64(), C.c_int64(), C.c_int64()
         self.check(lib().slm_pool_storage(self.handle, C.byref(k), C.byref(v), C.byref(n)))
         bf16 = self.config.kv_dtype == KV_BF16
@@ -533,6 +545,10 @@ class _Fast:
         self.decode = L.slm_batch_decode_layer
         self.decode_many = L.slm_batch_decode_layers
         self.decode_host = L.slm_batch_decode_layers_host
+        self.append_normed = L.slm_batch_append_layer_normed
+        self.shared_attention = L.slm_batch_shared_attention
+        self.token_probabilities = L.slm_batch_token_probabilities
+        self.verify_drafts = L.slm_batch_verify_drafts
         self.end = L.slm_batch_end
         self.submit = L.slm_batch_submit
         self.wait = L.slm_batch_wait
@@ -659,28 +675,33 @@ class Batch:
         self.pool.check(lib().slm_batch_attention_exact(self._h, int(layer), _ptr(query),
                                                         int(bool(rotate_query)), _ptr(out)))
 
-    def _tensor(self, what: str, t, shape, dtype: str = "float32", rows=False) -> int:
-        """Device address of a CUDA tensor of the pool's device with this
-        shape; ``rows``: dense rows at any distance instead of contiguous."""
-        import torch
-
+    def _tensor(self, what: str, t, shape, dtype=None, rows=False) -> int:
+        """Device address of a CUDA tensor (float32, or ``dtype``) of the
+        pool's device with this shape; ``rows``: dense rows at any distance
+        instead of contiguous."""
+        torch = _torch()
         if not isinstance(t, torch.Tensor):
             raise TypeError("expected a torch tensor")
-        if t.shape == shape and t.dtype is getattr(torch, dtype) and t.device.type == "cuda" \
-                and t.device.index == self.pool.device:
+        if t.shape == shape and t.dtype is (dtype or torch.float32) and t.is_cuda \
+                and t.get_device() == self.pool.device:
             if t.is_contiguous():
                 return t.data_ptr()
             if rows and t[0].is_contiguous() and t.stride(0) >= t[0].numel():
                 return t.data_ptr()
         raise InvalidInput(ERR_INVALID_INPUT,
                            f"invalid input for slmkv: {what} must be a "
-                           f"{'row-strided' if rows else 'contiguous'} {dtype} CUDA tensor "
-                           f"{list(shape)} on the pool's device")
+                           f"{'row-strided' if rows else 'contiguous'} {dtype or torch.float32} CUDA "
+                           f"tensor {list(shape)} on the pool's device")
 
-    def _token_rows(self) -> int:
-        if self.token_counts is None:
-            self.token_counts = list(self._counts[: len(self.caches)])
-        return sum(self.token_counts)
+    def _shapes(self):
+        """(token rows, query shape, key shape) of the batch's tensors."""
+        s = getattr(self, "_row_shapes", None)
+        if s is None:
+            if self.token_counts is None:
+                self.token_counts = list(self._counts[: len(self.caches)])
+            t, p = sum(self.token_counts), self.pool
+            s = self._row_shapes = (t, (t, p.q_heads, p.head_dim), (t, p.kv_heads, p.head_dim))
+        return s
 
     def append_layer_normed(self, layer: int, query, keys, values, query_norm, key_norm, query_out,
                             *, epsilon: float = 1e-5, rotate: bool = True) -> None:
@@ -689,58 +710,64 @@ class Batch:
         queries to ``query_out`` [tokens, q_heads, d]. query [tokens, q_heads,
         d], keys / values [tokens, kv_heads, d]: rows may be strided (slices of
         one projection's output); query_norm, key_norm [d]."""
-        p, t = self.pool, self._token_rows()
-        ins = [self._tensor("query", query, (t, p.q_heads, p.head_dim), rows=True),
-               self._tensor("keys", keys, (t, p.kv_heads, p.head_dim), rows=True),
-               self._tensor("values", values, (t, p.kv_heads, p.head_dim), rows=True)]
+        t, q_shape, k_shape = self._shapes()
+        width = q_shape[2]
+        ins = (self._tensor("query", query, q_shape, rows=True),
+               self._tensor("keys", keys, k_shape, rows=True),
+               self._tensor("values", values, k_shape, rows=True))
         # one row has no distance to a next one
-        strides = [x.stride(0) if t > 1 else x[0].numel() for x in (query, keys, values)]
-        p.check(lib().slm_batch_append_layer_normed(
-            self._h, int(layer), *ins, *strides, self._tensor("query_norm", query_norm, (p.head_dim,)),
-            self._tensor("key_norm", key_norm, (p.head_dim,)), float(epsilon), int(bool(rotate)),
-            self._tensor("query_out", query_out, (t, p.q_heads, p.head_dim))))
+        strides = ((query.stride(0), keys.stride(0), values.stride(0)) if t > 1 else
+                   (q_shape[1] * width, k_shape[1] * width, k_shape[1] * width))
+        rc = _fast.append_normed(
+            self._h, layer, *ins, *strides, self._tensor("query_norm", query_norm, (width,)),
+            self._tensor("key_norm", key_norm, (width,)), epsilon, 1 if rotate else 0,
+            self._tensor("query_out", query_out, q_shape))
+        if rc:
+            self.pool.check(rc)
 
     def shared_prefix_attention(self, layer: int, query, out, rotate_query: bool = True) -> None:
         """slm_batch_shared_attention: prefill_attention for sequences that
         share cached prefixes, whose blocks are read once for all of them;
         query / out [tokens, q_heads, d]."""
-        p, t = self.pool, self._token_rows()
-        p.check(lib().slm_batch_shared_attention(
-            self._h, int(layer), self._tensor("query", query, (t, p.q_heads, p.head_dim)),
-            int(bool(rotate_query)), self._tensor("out", out, (t, p.q_heads, p.head_dim))))
+        _, shape, _ = self._shapes()
+        rc = _fast.shared_attention(self._h, layer, self._tensor("query", query, shape),
+                                    1 if rotate_query else 0, self._tensor("out", out, shape))
+        if rc:
+            self.pool.check(rc)
 
     def token_probabilities(self, logits, probabilities, temperatures=None) -> None:
         """slm_batch_token_probabilities: softmax of logits / temperature per
         row ([tokens or sequences, vocab], rows may be strided; temperature 0:
         the first maximum), into ``probabilities`` (same shape, dense; may be
         ``logits``). temperatures: [rows] float32, or None for 1."""
-        import torch
-
-        if not isinstance(logits, torch.Tensor) or logits.dim() != 2:
+        if not isinstance(logits, _torch().Tensor) or logits.dim() != 2:
             raise InvalidInput(ERR_INVALID_INPUT, "invalid input for slmkv: logits must be [rows, vocab]")
-        rows, vocab = logits.shape
-        src = self._tensor("logits", logits, (rows, vocab), rows=True)
+        rows, vocab = shape = logits.shape
+        src = self._tensor("logits", logits, shape, rows=True)
         t = None if temperatures is None else self._tensor("temperatures", temperatures, (rows,))
-        self.pool.check(lib().slm_batch_token_probabilities(
+        rc = _fast.token_probabilities(
             self._h, src, rows, vocab, logits.stride(0) if rows > 1 else vocab, t,
-            self._tensor("probabilities", probabilities, (rows, vocab))))
+            self._tensor("probabilities", probabilities, shape))
+        if rc:
+            self.pool.check(rc)
 
     def verify_drafts(self, token_ids, target, draft, uniforms, accepted, next_tokens) -> None:
         """slm_batch_verify_drafts: token_ids [tokens] int32 (each sequence's
         last accepted token, then its drafts), target [tokens, vocab], draft
         [tokens - sequences, vocab] or None, uniforms [tokens]; accepted and
         next_tokens [sequences] int32 are written."""
-        import torch
-
+        torch = _torch()
         if not isinstance(target, torch.Tensor) or target.dim() != 2:
             raise InvalidInput(ERR_INVALID_INPUT, "invalid input for slmkv: target must be [tokens, vocab]")
-        t, n, vocab = self._token_rows(), len(self.caches), target.shape[1]
+        t, n, vocab, i32 = self._shapes()[0], len(self.caches), target.shape[1], torch.int32
         q = None if draft is None else self._tensor("draft", draft, (t - n, vocab))
-        self.pool.check(lib().slm_batch_verify_drafts(
-            self._h, vocab, self._tensor("token_ids", token_ids, (t,), "int32"),
+        rc = _fast.verify_drafts(
+            self._h, vocab, self._tensor("token_ids", token_ids, (t,), i32),
             self._tensor("target", target, (t, vocab)), q, self._tensor("uniforms", uniforms, (t,)),
-            self._tensor("accepted", accepted, (n,), "int32"),
-            self._tensor("next_tokens", next_tokens, (n,), "int32")))
+            self._tensor("accepted", accepted, (n,), i32),
+            self._tensor("next_tokens", next_tokens, (n,), i32))
+        if rc:
+            self.pool.check(rc)
 
     def end(self, raise_on_error: bool = True) -> list[int]:
         if self._h is None:
