@@ -186,7 +186,8 @@ struct slm_ctx {
   int32_t* d_counters = nullptr;
   int32_t* d_error = nullptr;
   int32_t* h_readback = nullptr;  // pinned: [1 + max_sequences]
-  CUtensorMap tmap_k{}, tmap_v{};  // bf16 pools: TMA maps for the decode kernel
+  CUtensorMap tmap_k{}, tmap_v{};  // TMA maps of the pools
+  bool have_maps = false;
   // Pinned status readback of submitted batches: kReadbackSlots slots of
   // [error word, pad, status x max_sequences], each with its event.
   int32_t* h_rb = nullptr;
@@ -685,9 +686,11 @@ slm_status upload_step(slm_ctx* c, Upload& u, cudaStream_t s, const std::vector<
   return SLM_OK;
 }
 
-// TMA maps of a bf16 pool for the decode kernel: the whole pool as rows of
-// 64 bf16 (128 B; row = ((layer * num_blocks + block) * kv_heads + head) * 16
-// + slot), a box of one 16-row chunk, 128-byte swizzle. The encoder comes
+// TMA maps of a pool: the whole pool as rows of 64 values (row = ((layer *
+// num_blocks + block) * kv_heads + head) * 16 + slot), a box of 128 bytes (64
+// bf16, half a row of f32) of one 16-row chunk, 128-byte swizzle. bf16: for the
+// decode kernel, made with the context; f32: for slm_batch_shared_attention, made
+// by its first call. The encoder comes
 // from the driver through the runtime (no link against the driver library).
 slm_status make_pool_maps(slm_ctx* c) {
   static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
@@ -705,17 +708,18 @@ slm_status make_pool_maps(slm_ctx* c) {
                         k.num_key_value_heads * kBlockTokens;
   if (rows > static_cast<uint64_t>(INT32_MAX))
     return fail(c, SLM_ERR_INVALID_CONFIGURATION,
-                "invalid configuration: a bf16 pool of %llu rows exceeds the 2^31 rows a TMA "
+                "invalid configuration: a pool of %llu rows exceeds the 2^31 rows a TMA "
                 "coordinate addresses",
                 static_cast<unsigned long long>(rows));
+  const bool bf16 = k.kv_dtype == SLM_KV_BF16;
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(k.head_dimension), rows};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(k.head_dimension) * 2};
-  const cuuint32_t box[2] = {static_cast<cuuint32_t>(k.head_dimension), kBlockTokens};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(k.head_dimension) * (bf16 ? 2 : 4)};
+  const cuuint32_t box[2] = {bf16 ? static_cast<cuuint32_t>(k.head_dimension) : 32u, kBlockTokens};
   const cuuint32_t estride[2] = {1, 1};
   void* pools[2] = {c->k_pool, c->v_pool};
   CUtensorMap* maps[2] = {&c->tmap_k, &c->tmap_v};
   for (int i = 0; i < 2; ++i) {
-    const CUresult r = encode(maps[i], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, pools[i], dims,
+    const CUresult r = encode(maps[i], bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, pools[i], dims,
                               strides, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -723,6 +727,7 @@ slm_status make_pool_maps(slm_ctx* c) {
       return fail(c, SLM_ERR_CUDA, "CUDA error: cuTensorMapEncodeTiled failed (%d)",
                   static_cast<int>(r));
   }
+  c->have_maps = true;
   return SLM_OK;
 }
 
@@ -2005,6 +2010,10 @@ void build_shared_plan(const slm_ctx* c, const slm_batch* b, SharedPlan& plan) {
 // Builds and uploads the open batch's plan (once a batch: its layers share it).
 slm_status shared_prepare(slm_batch* b) {
   slm_ctx* c = b->ctx;
+  if (!c->have_maps) {
+    const slm_status rc = make_pool_maps(c);
+    if (rc) return rc;
+  }
   SharedPlan& plan = c->shared_plan;
   build_shared_plan(c, b, plan);
   if (plan.parts > INT32_MAX || plan.items.size() + plan.units.size() > static_cast<size_t>(INT32_MAX))

@@ -263,7 +263,9 @@ struct SharedAttentionLaunch {
   int32_t most_parts;  // of a row that is joined
   const SharedItem* tc_items;  // runs that many rows see
   int32_t n_tc_items;
-  CUtensorMap tmap_k, tmap_v;  // bf16 pools: the decode kernel's pool maps
+  // boxes of 16 rows of 128 bytes: the decode kernel's maps of a bf16 pool; of an
+  // f32 pool, whose rows are two boxes wide, its own
+  CUtensorMap tmap_k, tmap_v;
   const SharedToken* tokens;
   const SharedEdge* edges;
   const SharedUnit* units;

@@ -23,13 +23,37 @@ constexpr int kThreads = 32 * kWarps;
 __device__ __forceinline__ uint32_t saddr(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+// A box of 16 rows of 128 bytes, 128-byte swizzled, at column x and row y.
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
 }
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Waits for at most about a second.
+__device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity) {
+  unsigned long long t0, t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+  for (int i = 0; i < (1 << 26); ++i) {
+    if (bar_try(bar, parity)) return true;
+    if ((i & 255) == 255) {
+      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+      if (t - t0 > 1000000000ull) return false;
+    }
+  }
+  return false;
 }
 // c += a b, 16 x 8 x 16, bf16 operands (a: rows, b: columns), f32 sums.
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -50,7 +74,7 @@ __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 
 template <int BF16>
 struct RowsCfg {
   static constexpr int kBlocks = BF16 ? 2 : 1;            // of a step
-  static constexpr int kBlockBytes = BF16 ? 4096 : 8192;   // K and V of 16 tokens
+  static constexpr int kBlockBytes = BF16 ? 4096 : 8192;  // K and V of 16 tokens, boxes of 2 KiB
   static constexpr int kStages = 2;
   static constexpr int kStageBytes = kBlocks * kBlockBytes;
   static constexpr int kWarpBytes = kStages * kStageBytes;
@@ -87,23 +111,29 @@ __device__ __forceinline__ SharedItem load_item(const SharedItem* p) {
 // exact products (f32 pages: the products of a mid or lo part with a lo part,
 // below 2^-23 of a term, are dropped).
 //
-// Each thread copies, and reads back, only its own 16-byte pieces of a block: in
-// the products' inner dimensions any order serves, so thread (g, c) of a warp
-// (g = lane / 4, c = lane % 4) takes
-//   K: tokens g and g + 8, four consecutive values a k-step (a 16-byte piece is
-//      one k-step of f32, two of bf16)
-//   V: tokens 2c, 2c+1, 2c+8, 2c+9, values 8g..8g+7; value tile j holds the
-//      values 8n + 2j and 8n + 2j + 1, so a thread ends with values 8g..8g+7 of
-//      rows 2c and 2c + 1
-// which keeps global reads full sectors and needs no barrier but a team's.
+// A block's keys and values of a head arrive as swizzled boxes, a few copies a
+// step (with sixteen 16-byte copies a thread and step, the load unit took 1000
+// cycles a step to accept them, and 5000 to fill the stages at the start). Thread
+// (g, c) of a warp (g = lane / 4, c = lane % 4) reads
+//   K: rows t(g) and t(g) + 8, four consecutive values a k-step
+//   V: rows t(2c), t(2c+1) and those + 8, values 8 v(g) .. 8 v(g) + 7; value tile j
+//      holds the values 8 v + 2j and 8 v + 2j + 1
+// in the products' inner dimensions any order serves; t and v are such that the
+// eight threads of a 16-byte access meet eight different banks of the swizzle. A
+// thread ends with values 8 v(g) .. 8 v(g) + 7 of rows 2c and 2c + 1.
 //
-// Bound by memory at the start, when every warp asks for its first stages, and
-// by the latency of a step's chain of products, maximum and powers after that.
+// Bound by memory while every warp's first stages are on their way, and by the
+// latency of a step's chain of products, maximum and powers after that.
 template <int BF16, int G>
-__global__ void __launch_bounds__(kThreads, 3) shared_rows_kernel(const SharedAttentionLaunch p) {
+__global__ void __launch_bounds__(kThreads, 3) shared_rows_kernel(const __grid_constant__ SharedAttentionLaunch p) {
   using Cfg = RowsCfg<BF16>;
   constexpr int NB = Cfg::kBlocks, kStages = Cfg::kStages;
-  extern __shared__ __align__(16) uint8_t sm[];
+  extern __shared__ __align__(1024) uint8_t sm[];
+  __shared__ __align__(8) uint64_t bars[kWarps][kStages];
+  if (saddr(sm) & 1023u) {  // uniform: report instead of misreading boxes
+    if (threadIdx.x == 0) atomicOr(p.g.error, kErrLayout);
+    return;
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   let_next_start();
   const bool team = p.team != 0;
@@ -112,13 +142,17 @@ __global__ void __launch_bounds__(kThreads, 3) shared_rows_kernel(const SharedAt
   const int item0 = p.list_start[list], item1 = p.list_start[list + 1];
   const int offset = team ? warp * NB : 0, stride = team ? kWarps * NB : NB;  // the warp's steps of an item
   const int Hkv = p.g.kv_heads, Hq = p.g.q_heads;
-  constexpr size_t esz = BF16 ? 2 : 4;
-  constexpr size_t chunk = static_cast<size_t>(kBlockTokens) * D * esz;
-  const size_t layer = static_cast<size_t>(p.layer) * p.g.layer_elems * esz;
-  const uint8_t* kbase = static_cast<const uint8_t*>(p.g.k) + layer + g * (D * esz) + 16 * c;
-  const uint8_t* vbase = static_cast<const uint8_t*>(p.g.v) + layer + 2 * c * (D * esz) + g * (8 * esz);
   uint8_t* stage0 = sm + warp * Cfg::kWarpBytes;
-  const uint32_t stage_addr = saddr(stage0) + lane * 16;
+  const uint32_t stage_addr = saddr(stage0), bar0 = saddr(&bars[warp][0]);
+  if (lane == 0) {
+    for (int n = 0; n < kStages; ++n)
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar0 + 8 * n) : "memory");
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncwarp();
+  // t and v above; adjacent threads differ by four in t and, of bf16, in v
+  auto token_row = [](int i) { return (i & 1) * 4 + (i >> 1); };
+  const int tg = token_row(g), vg = BF16 ? tg : (g & 4) + (g & 1) * 2 + ((g >> 1) & 1);
 
   // The copies run ahead of the products, across the ends of items: their own
   // place in the list, the next item's record and first block ids at hand.
@@ -130,6 +164,15 @@ __global__ void __launch_bounds__(kThreads, 3) shared_rows_kernel(const SharedAt
   SharedItem ahead = cur, ahead_next = load_item(p.items + min(item0 + 1, item1 - 1));
   int ahead_at = item0, block = offset;  // the copies' item and its next block
   int32_t ids = first_ids(ahead), ids_next = first_ids(ahead_next), window = 0;
+  int issued = 0, taken = 0;  // steps
+  bool lost = false;           // a wait ran out: no more are waited for
+  auto arrived = [&](int n) {
+    const uint32_t bar = bar0 + 8 * (n % kStages), parity = static_cast<uint32_t>((n / kStages) & 1);
+    if (!lost && !bar_try(bar, parity) && !bar_wait_slow(bar, parity)) {
+      lost = true;
+      atomicOr(p.g.error, kErrTimeout);
+    }
+  };
   auto issue = [&](int stage) {  // the next step's blocks, or nothing at the end
     while (block >= ahead.n_blocks) {  // (an item may have no step for a warp of a team)
       if (ahead_at + 1 >= item1) return;
@@ -141,46 +184,33 @@ __global__ void __launch_bounds__(kThreads, 3) shared_rows_kernel(const SharedAt
       ahead_next = load_item(p.items + min(ahead_at + 1, item1 - 1));
       ids_next = first_ids(ahead_next);
     }
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      // a step's block past the run repeats the last one (masked below)
-      const int j = min(block + b, ahead.n_blocks - 1);
-      // the ids at hand are those of a window of 32 blocks
-      if ((j >> 5) != window) {
-        window = j >> 5;
-        const int at = 32 * window + lane;
-        ids = at < ahead.n_blocks ? table_of(ahead)[at] : 0;
-      }
-      const int32_t id = pool_block(p.g, __shfl_sync(kFullMask, ids, j & 31));
-      const size_t at = (static_cast<size_t>(id) * Hkv + ahead.head) * chunk;
-      const uint32_t dst = stage_addr + stage * Cfg::kStageBytes + b * Cfg::kBlockBytes;
-      constexpr int kP = BF16 ? 2 : 4;  // 16-byte pieces of K a token and thread
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int i = 0; i < kP; ++i)
-          copy16(dst + (u * kP + i) * 512, kbase + at + u * (8 * D * esz) + 64 * i);
-      constexpr int kW = BF16 ? 1 : 2;  // of V
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int i = 0; i < kW; ++i)
-          copy16(dst + Cfg::kBlockBytes / 2 + (t * kW + i) * 512,
-                 vbase + at + ((t & 1) + 8 * (t >> 1)) * (D * esz) + 16 * i);
+    // lanes 0..3 ask for a box each: bf16 K and V of two blocks (one past the run
+    // repeats the last one: masked below), f32 the halves of K's and V's rows
+    const int j = min(block + (BF16 ? (lane >> 1) & 1 : 0), ahead.n_blocks - 1);
+    if ((min(block + NB - 1, ahead.n_blocks - 1) >> 5) != window) {  // the ids at hand are of 32 blocks
+      window = min(block + NB - 1, ahead.n_blocks - 1) >> 5;
+      const int at = 32 * window + lane;
+      ids = at < ahead.n_blocks ? table_of(ahead)[at] : 0;
     }
+    const int32_t id = pool_block(p.g, __shfl_sync(kFullMask, ids, j & 31));
+    const int y = ((p.layer * p.g.num_blocks + id) * Hkv + ahead.head) * kBlockTokens;
+    const uint32_t bar = bar0 + 8 * stage;
+    if (lane == 0)
+      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(Cfg::kStageBytes)
+                   : "memory");
+    __syncwarp();
+    if (lane < 4)
+      tma_box(stage_addr + stage * Cfg::kStageBytes + lane * 2048,
+              (BF16 ? lane & 1 : lane >> 1) ? &p.tmap_v : &p.tmap_k, BF16 ? 0 : 32 * (lane & 1), y, bar);
+    ++issued;
     block += stride;
   };
-#pragma unroll
-  for (int n = 0; n < kStages; ++n) {
-    issue(n);
-    copy_commit();
-  }
+  for (int n = 0; n < kStages; ++n) issue(n);
 
   // the token of an item's row g
   auto row_token = [&](const SharedItem& it) { return p.tokens[it.token0 + min(g / G, it.n_tokens - 1)]; };
   SharedToken tk, tk_next = row_token(cur);
   SharedItem next = cur;
-  int stage = 0;
 
   for (int at = item0; at < item1; ++at) {
     cur = next;
@@ -224,8 +254,10 @@ __global__ void __launch_bounds__(kThreads, 3) shared_rows_kernel(const SharedAt
     for (int j = 0; j < 4; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
 
     for (int n = offset; n < cur.n_blocks; n += stride) {
-      copy_wait<kStages - 1>();
-      const uint8_t* st0 = stage0 + stage * Cfg::kStageBytes + lane * 16;
+      arrived(taken);
+      __syncwarp();
+      const int stage = taken % kStages;
+      const uint8_t* st0 = stage0 + stage * Cfg::kStageBytes;
       // scores: the products with a mid or lo part apart from those of two hi
       // parts, since a tensor core's sum is cut off at each step
       float s[NB][4], small[NB][4];
@@ -240,8 +272,9 @@ __global__ void __launch_bounds__(kThreads, 3) shared_rows_kernel(const SharedAt
           uint4 k0[NB], k1[NB];
 #pragma unroll
           for (int k = 0; k < NB; ++k) {
-            k0[k] = *reinterpret_cast<const uint4*>(st0 + k * Cfg::kBlockBytes + i * 512);
-            k1[k] = *reinterpret_cast<const uint4*>(st0 + k * Cfg::kBlockBytes + (2 + i) * 512);
+            const uint8_t* at = st0 + k * Cfg::kBlockBytes + tg * 128 + (((4 * i + c) ^ tg) << 4);
+            k0[k] = *reinterpret_cast<const uint4*>(at);
+            k1[k] = *reinterpret_cast<const uint4*>(at + 8 * 128);
           }
 #pragma unroll
           for (int h = 0; h < 2; ++h)
@@ -258,8 +291,9 @@ __global__ void __launch_bounds__(kThreads, 3) shared_rows_kernel(const SharedAt
         float other[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float4 k0 = *reinterpret_cast<const float4*>(st0 + i * 512);
-          const float4 k1 = *reinterpret_cast<const float4*>(st0 + (4 + i) * 512);
+          const uint8_t* at = st0 + (i >> 1) * 2048 + tg * 128 + (((4 * (i & 1) + c) ^ tg) << 4);
+          const float4 k0 = *reinterpret_cast<const float4*>(at);
+          const float4 k1 = *reinterpret_cast<const float4*>(at + 8 * 128);
           const Parts a0 = split_pair(k0.x, k0.y), a1 = split_pair(k1.x, k1.y);
           const Parts a2 = split_pair(k0.z, k0.w), a3 = split_pair(k1.z, k1.w);
           const uint2(&x)[3] = q[i];
@@ -285,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, 3) shared_rows_kernel(const SharedAt
         for (int e = 0; e < 4; ++e) {
           float& x = s[k][e];
           x += small[k][e];
-          const int pos = kp + 16 * k + g + 8 * (e >> 1);
+          const int pos = kp + 16 * k + tg + 8 * (e >> 1);
           const bool seen = !masked || (pos <= qpos[e & 1] && pos < end);
           fin[e & 1] = fmaf(seen ? x : 0.f, 0.f, fin[e & 1]);
           if (!seen) x = -INFINITY;
@@ -334,7 +368,10 @@ __global__ void __launch_bounds__(kThreads, 3) shared_rows_kernel(const SharedAt
         for (int k = 0; k < NB; ++k) {
           uint4 v[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint4*>(sv + k * Cfg::kBlockBytes + i * 512);
+          for (int i = 0; i < 4; ++i) {
+            const int t = token_row(2 * c + (i & 1));
+            v[i] = *reinterpret_cast<const uint4*>(sv + k * Cfg::kBlockBytes + (t + 8 * (i >> 1)) * 128 + ((vg ^ t) << 4));
+          }
 #pragma unroll
           for (int part = 2; part >= 0; --part)
 #pragma unroll
@@ -345,14 +382,19 @@ __global__ void __launch_bounds__(kThreads, 3) shared_rows_kernel(const SharedAt
         }
       } else {
         const uint32_t(&x)[3][2] = pt[0];
+        float4 v[4];  // half of the values of the four tokens
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          float2 v[4];  // values 8g + 2j, 8g + 2j + 1 of the four tokens
+          if ((j & 1) == 0)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            v[i] = *reinterpret_cast<const float2*>(sv + (2 * i + (j >> 1)) * 512 + 8 * (j & 1));
-          const Parts a0 = split_pair(v[0].x, v[1].x), a1 = split_pair(v[0].y, v[1].y);
-          const Parts a2 = split_pair(v[2].x, v[3].x), a3 = split_pair(v[2].y, v[3].y);
+            for (int i = 0; i < 4; ++i) {
+              const int t = token_row(2 * c + (i & 1)), u = 2 * (vg & 3) + (j >> 1);
+              v[i] = *reinterpret_cast<const float4*>(sv + (vg >> 2) * 2048 + (t + 8 * (i >> 1)) * 128 + ((u ^ t) << 4));
+            }
+          auto pair = [&](const float4& f) { return (j & 1) ? make_float2(f.z, f.w) : make_float2(f.x, f.y); };
+          const float2 v0 = pair(v[0]), v1 = pair(v[1]), v2 = pair(v[2]), v3 = pair(v[3]);
+          const Parts a0 = split_pair(v0.x, v1.x), a1 = split_pair(v0.y, v1.y);
+          const Parts a2 = split_pair(v2.x, v3.x), a3 = split_pair(v2.y, v3.y);
           mma(acc[j], a0.lo, a1.lo, a2.lo, a3.lo, x[0][0], x[0][1]);
           mma(acc[j], a0.hi, a1.hi, a2.hi, a3.hi, x[2][0], x[2][1]);
           mma(acc[j], a0.mid, a1.mid, a2.mid, a3.mid, x[1][0], x[1][1]);
@@ -365,9 +407,9 @@ __global__ void __launch_bounds__(kThreads, 3) shared_rows_kernel(const SharedAt
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[j][e] = fmaf(o[j][e], corr[e & 1], acc[j][e]);
+      __syncwarp();  // the stage has been read
+      ++taken;
       issue(stage);
-      copy_commit();
-      stage = stage + 1 == kStages ? 0 : stage + 1;
     }
     // Deliver the rows: to the output where the run holds all that they see,
     // else as parts. softmax.rs:17-22: a score that is not finite fails the
@@ -395,10 +437,10 @@ __global__ void __launch_bounds__(kThreads, 3) shared_rows_kernel(const SharedAt
         const float4 x = make_float4(o[0][e], o[0][e + 2], o[1][e], o[1][e + 2]);
         const float4 y = make_float4(o[2][e], o[2][e + 2], o[3][e], o[3][e + 2]);
         if (!team) {
-          deliver(r, out_row, 8 * g, x, y, m[e], l[e]);
+          deliver(r, out_row, 8 * vg, x, y, m[e], l[e]);
         } else {
           uint8_t* mine = parts + warp * Cfg::kPartBytes;
-          float4* d4 = reinterpret_cast<float4*>(mine + r * (D * 4) + 32 * g);
+          float4* d4 = reinterpret_cast<float4*>(mine + r * (D * 4) + 32 * vg);
           d4[0] = x;
           d4[1] = y;
           if (g == 0) reinterpret_cast<float2*>(mine + 8 * D * 4)[r] = make_float2(m[e], l[e]);
@@ -435,7 +477,9 @@ __global__ void __launch_bounds__(kThreads, 3) shared_rows_kernel(const SharedAt
       __syncthreads();
     }
   }
-  copy_wait<0>();
+  if (lost)  // every copy lands before the CTA's shared memory is released
+    for (int n = max(0, issued - kStages); n < issued; ++n)
+      bar_wait_slow(bar0 + 8 * (n % kStages), static_cast<uint32_t>((n / kStages) & 1));
   // The tensor-core kernel, under which this one may have run (it reads nothing
   // of it), is part of what the joining kernel waits for.
   wait_for_previous();
@@ -449,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, 3) shared_rows_kernel(const SharedAt
 constexpr int kMergeThreads = 256;
 constexpr int kMergeDepth = 4;  // edges whose units are read ahead
 template <int W>
-__global__ void __launch_bounds__(kMergeThreads) shared_merge_kernel(const SharedAttentionLaunch p) {
+__global__ void __launch_bounds__(kMergeThreads, 4) shared_merge_kernel(const SharedAttentionLaunch p) {
   __shared__ float2 s_ml[8];
   __shared__ float2 s_acc[8][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, share = warp % W;
@@ -577,7 +621,16 @@ cudaError_t launch_shared_attention(const SharedAttentionLaunch& p, cudaStream_t
   auto run = [&](auto kernel, int v, int smem, int team_smem) {
     if (p.team) smem = team_smem;
     if (dev >= 64 || !(configured[v] & (1ull << dev))) {
-      const cudaError_t a = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, team_smem);
+      // all kernels of a call want the same split of the SMs' memory: an SM
+      // changes it only when it is empty
+      cudaError_t a = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, team_smem);
+      auto all_shared = [&](auto k) {
+        if (a == cudaSuccess)
+          a = cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+      };
+      all_shared(kernel);
+      all_shared(shared_merge_kernel<1>);
+      all_shared(shared_merge_kernel<8>);
       if (a != cudaSuccess) return a;
       if (dev < 64) configured[v] |= 1ull << dev;
     }

@@ -59,7 +59,8 @@ struct TcCfg {
     kBarVFull = kBarKFull + kStages,
     kBarKFree = kBarVFull + kStages,
     kBarVFree = kBarKFree + kStages,
-    kBarSFull = kBarVFree + kStages,  // one a buffer
+    kBarQFull = kBarVFree + kStages,
+    kBarSFull,  // one a buffer
     kBarPFull = kBarSFull + 2,
     kBarODone,
     kBarDrain,
@@ -220,6 +221,7 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
   const uint32_t abort = sbase + Cfg::kOffMisc + 4;
   if (tid == 0) {
     for (int s = 0; s < 4 * kStages; ++s) bar_init(bar(s), s < 2 * kStages ? Cfg::kLoaders : 1);
+    bar_init(bar(Cfg::kBarQFull), BF16 ? 8 : 4);
     bar_init(bar(Cfg::kBarSFull), 1);
     bar_init(bar(Cfg::kBarSFull + 1), 1);
     bar_init(bar(Cfg::kBarPFull), 4);
@@ -234,12 +236,13 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  {
-    // Q rows: a warp writes sixteen, one per step, lane l elements 2l and 2l + 1
-    // (one rotation pair): rotated, scaled into the exp2 domain, split. All loads
-    // first: rows beyond the item's tokens load a last one's, and are written as
-    // zeros.
-    constexpr int kEach = kRows / 8;
+  // Q rows: a warp writes N of them, one per step, lane l elements 2l and 2l + 1
+  // (one rotation pair): rotated, scaled into the exp2 domain, split. All loads
+  // first: rows beyond the item's tokens load a last one's, and are written as
+  // zeros. bf16: all warps write sixteen, the first copies under way; f32: the
+  // softmax warps write 32, beside the loaders.
+  auto write_q = [&](auto n_rows) {
+    constexpr int kEach = decltype(n_rows)::value;
     const SharedItem it = p.tc_items[cta_index()];
     const int Hq = p.g.q_heads, r0 = warp * kEach;
     // of row r0 + lane
@@ -270,7 +273,25 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
       *reinterpret_cast<uint32_t*>(dst + 2 * kQBytes) = s.lo;
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  }
+    __syncwarp();
+    if (lane == 0) bar_arrive(bar(Cfg::kBarQFull));
+  };
+  // bf16: tile j's keys, then its values, a lane a block (a last tile's blocks
+  // past the run repeat the last one: masked)
+  auto copy_tile = [&](const SharedItem& it, int j, bool keys) {
+    const int st = j % kStages;
+    const int32_t* table = p.g.block_table + static_cast<size_t>(it.slot) * p.g.max_blocks_per_seq + it.first_block;
+    int32_t blk = lane < kTileBlocks ? table[min(j * kTileBlocks + lane, it.n_blocks - 1)] : 0;
+    blk = pool_block(p.g, blk);
+    const int y = (p.layer * p.g.num_blocks * p.g.kv_heads + it.head + blk * p.g.kv_heads) * kBlockTokens;
+    const int full = (keys ? Cfg::kBarKFull : Cfg::kBarVFull) + st;
+    if (lane == 0) bar_expect(bar(full), kTileBytes);
+    __syncwarp();
+    if (lane < kTileBlocks)
+      tma_block(sbase + (keys ? Cfg::kOffK : Cfg::kOffV) + static_cast<uint32_t>(st * kStageBytes + lane * kBlockTokens * 128),
+                keys ? &p.tmap_k : &p.tmap_v, y, bar(full));
+    __syncwarp();
+  };
   fence_before();
   __syncthreads();
   fence_after();
@@ -281,6 +302,18 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
     }
   };
 
+  if (BF16) {
+    if (warp == kLoadWarp) {
+      const SharedItem it = p.tc_items[cta_index()];
+      const int first = min(kStages, (it.n_blocks + kTileBlocks - 1) / kTileBlocks);
+      for (int j = 0; j < first; ++j) {
+        copy_tile(it, j, true);
+        copy_tile(it, j, false);
+      }
+    }
+    write_q(std::integral_constant<int, kRows / 8>{});
+  }
+
   if (warp < 4) {
     // ================= softmax: thread = row =================
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsSoftmax) : "memory");
@@ -290,6 +323,7 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
     auto wait = [&](int b, uint32_t parity) {
       return __all_sync(kFullMask, bar_wait(bar(b), parity, abort));
     };
+    if (!BF16) write_q(std::integral_constant<int, kRows / 4>{});
     float o[D];
 #pragma unroll
     for (int i = 0; i < D; ++i) o[i] = 0.f;
@@ -344,18 +378,28 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
       m = mx;
       const uint64_t neg = pack2(-mx, -mx);
       uint64_t sums[2] = {0ull, 0ull};
-#pragma unroll
-      for (int ks = 0; ks < kTokens / 16; ++ks) {
-        uint32_t hi[8], mid[8], lo[8];
+      // the next sixteen powers are taken while the last ones are split: the two
+      // keep different units busy
+      uint64_t w[2][8];
+      auto powers = [&](int ks) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const uint64_t x = pack2(s[16 * ks + 2 * i], s[16 * ks + 2 * i + 1]);
           fin = fma2(x, 0ull, fin);  // +0 per finite score, NaN from a non-finite one on
           float a, b;
           unpack2(add2(x, neg), a, b);
-          const uint64_t w = pack2(exp2_fast(a), exp2_fast(b));
-          sums[i & 1] = add2(sums[i & 1], w);
-          const Parts q = split_pair(w);
+          w[ks & 1][i] = pack2(exp2_fast(a), exp2_fast(b));
+        }
+      };
+      powers(0);
+#pragma unroll
+      for (int ks = 0; ks < kTokens / 16; ++ks) {
+        if (ks + 1 < kTokens / 16) powers(ks + 1);
+        uint32_t hi[8], mid[8], lo[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          sums[i & 1] = add2(sums[i & 1], w[ks & 1][i]);
+          const Parts q = split_pair(w[ks & 1][i]);
           hi[i] = q.hi;
           mid[i] = q.mid;
           lo[i] = q.lo;
@@ -404,30 +448,16 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
     auto pbar = bar;
     auto wait = [&](int b, uint32_t parity) { return __all_sync(kFullMask, bar_wait(pbar(b), parity, abort)); };
     if (BF16 && warp == kLoadWarp) {
-      // ================= loader: a lane a block =================
-      const int32_t* table = p.g.block_table + static_cast<size_t>(it.slot) * p.g.max_blocks_per_seq + it.first_block;
-      const int row0 = p.layer * p.g.num_blocks * p.g.kv_heads + it.head;
-      int k_issued = 0, v_issued = 0;
+      // ================= loader (the first tiles are on their way) =================
+      int k_issued = min(kStages, n_tiles), v_issued = k_issued;
       bool ok = true;
-      for (int j = 0; ok && j < n_tiles; ++j) {
-        const int st = j % kStages;
-        // a last tile's blocks past the run repeat the last one (masked)
-        int32_t blk = lane < kTileBlocks ? table[min(j * kTileBlocks + lane, it.n_blocks - 1)] : 0;
-        blk = pool_block(p.g, blk);
-        const int y = (row0 + blk * p.g.kv_heads) * kBlockTokens;
-        const uint32_t off = static_cast<uint32_t>(st * kStageBytes + lane * kBlockTokens * 128);
+      for (int j = kStages; ok && j < n_tiles; ++j) {
         const uint32_t parity = static_cast<uint32_t>((j / kStages - 1) & 1);
-        if (j >= kStages && !(ok = wait(Cfg::kBarKFree + st, parity))) break;
-        if (lane == 0) bar_expect(pbar(Cfg::kBarKFull + st), kTileBytes);
-        __syncwarp();
-        if (lane < kTileBlocks) tma_block(sbase + Cfg::kOffK + off, &p.tmap_k, y, pbar(Cfg::kBarKFull + st));
-        __syncwarp();
+        if (!(ok = wait(Cfg::kBarKFree + j % kStages, parity))) break;
+        copy_tile(it, j, true);
         k_issued = j + 1;
-        if (j >= kStages && !(ok = wait(Cfg::kBarVFree + st, parity))) break;
-        if (lane == 0) bar_expect(pbar(Cfg::kBarVFull + st), kTileBytes);
-        __syncwarp();
-        if (lane < kTileBlocks) tma_block(sbase + Cfg::kOffV + off, &p.tmap_v, y, pbar(Cfg::kBarVFull + st));
-        __syncwarp();
+        if (!(ok = wait(Cfg::kBarVFree + j % kStages, parity))) break;
+        copy_tile(it, j, false);
         v_issued = j + 1;
       }
       if (!ok) raise();
@@ -514,7 +544,7 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
         __syncwarp();
         return true;
       };
-      bool ok = scores(0) && (n_tiles < 2 || scores(1));
+      bool ok = wait(Cfg::kBarQFull, 0) && scores(0) && (n_tiles < 2 || scores(1));
       for (int j = 0; ok && j < n_tiles; ++j) {
         const int st = j % kStages;
         if (!(ok = wait(Cfg::kBarPFull, j & 1)) || !(ok = wait(Cfg::kBarVFull + st, (j / kStages) & 1))) break;
@@ -566,6 +596,9 @@ cudaError_t launch_shared_tc(const SharedAttentionLaunch& p, cudaStream_t s) {
       if (a != cudaSuccess) return a;
       if (fa.numRegs < kRegsLaunch) return cudaErrorInvalidConfiguration;
       a = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      // the same split of the SMs' memory as the kernels that run beside this one
+      if (a == cudaSuccess)
+        a = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
       if (a != cudaSuccess) return a;
       if (dev < 64) configured[v] |= 1ull << dev;
     }
