@@ -4,9 +4,11 @@
 // keys and values go into the pages (the append of kv_cache.rs:182-230 with the
 // rotation of attention.rs:422-482), queries to a dense buffer.
 //
-// Bound by memory: T (2 Hq + 2 Hkv) rows of 256 B plus the page writes. Sixteen
-// lanes hold a head's row, four values (two rotation pairs) a lane, so the
-// square sum is four shuffles and nothing goes through shared memory.
+// Bound by memory: T (2 Hq + 2 Hkv) rows of 256 B plus the page writes. Eight
+// lanes hold a head's row, eight values (four rotation pairs) a lane, so the
+// square sum is three shuffles and nothing goes through shared memory. One row a
+// lane group: with two (76 registers), or with 256 threads a CTA, fewer rows are
+// in flight on an SM (8191 tokens of 32 + 8 heads, bf16: 45 and 41 us against 35).
 #include <cuda_bf16.h>
 
 #include "slmkv_device.h"
@@ -15,85 +17,93 @@ namespace slmkv {
 namespace {
 
 constexpr int D = kHeadDim;
-constexpr int kThreads = 256;  // 16 row groups of 16 lanes
+constexpr int kThreads = 128;
+constexpr int kGroups = kThreads / 8;
 
-__device__ __forceinline__ float4 normed(float4 x, float4 w, float eps) {
-  float ss = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w;
+struct Row {  // eight consecutive values of a row
+  float4 a, b;
+};
+__device__ __forceinline__ Row load_row(const float* p, uint32_t l8) {
+  return {reinterpret_cast<const float4*>(p)[2 * l8], reinterpret_cast<const float4*>(p)[2 * l8 + 1]};
+}
+__device__ __forceinline__ void store_row(float* p, uint32_t l8, const Row& x) {
+  reinterpret_cast<float4*>(p)[2 * l8] = x.a;
+  reinterpret_cast<float4*>(p)[2 * l8 + 1] = x.b;
+}
+__device__ __forceinline__ float4 scaled(float4 x, float s, float4 w) {
+  return make_float4(x.x * s * w.x, x.y * s * w.y, x.z * s * w.z, x.w * s * w.w);
+}
+__device__ __forceinline__ Row normed(const Row& x, const Row& w, float eps) {
+  float ss = x.a.x * x.a.x + x.a.y * x.a.y + x.a.z * x.a.z + x.a.w * x.a.w;
+  ss += x.b.x * x.b.x + x.b.y * x.b.y + x.b.z * x.b.z + x.b.w * x.b.w;
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(kFullMask, ss, o);
+  for (int o = 4; o > 0; o >>= 1) ss += __shfl_xor_sync(kFullMask, ss, o);
   // a square sum past f32 would scale the row to zero: it counts as not finite
-  const float inv = isfinite(ss) ? __frsqrt_rn(ss * (1.f / D) + eps) : __int_as_float(0x7fc00000);
-  return make_float4(x.x * inv * w.x, x.y * inv * w.y, x.z * inv * w.z, x.w * inv * w.w);
+  const float inv = isfinite(ss) ? rsqrtf(ss * (1.f / D) + eps) : __int_as_float(0x7fc00000);
+  return {scaled(x.a, inv, w.a), scaled(x.b, inv, w.b)};
+}
+__device__ __forceinline__ uint32_t bf16_pair(float x, float y) {
+  const __nv_bfloat162 r = __floats2bfloat162_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// A word of two bf16 of which one is not finite.
+__device__ __forceinline__ bool not_finite(uint32_t w) {
+  return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
 }
 
 // A row is one query head of a token, or one key/value head (both halves).
-// R rows a lane group, every input load issued before the first use.
-template <int BF16, int R>
-__global__ void __launch_bounds__(kThreads) normed_append_kernel(const NormedAppendLaunch p) {
-  const int Hq = p.g.q_heads, Hkv = p.g.kv_heads, heads = Hq + Hkv;
-  const int64_t n_rows = static_cast<int64_t>(p.total_tokens) * heads;
-  const int grp = threadIdx.x >> 4, l16 = threadIdx.x & 15;
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * (16 * R) + grp;
-  float4 x[R], v[R];
-  int tok[R], head[R];
-#pragma unroll
-  for (int j = 0; j < R; ++j) {
-    // rows past the end repeat the last one: every lane takes part in the shuffles
-    const int64_t row = min(row0 + 16 * j, n_rows - 1);
-    tok[j] = static_cast<int>(row / heads);
-    head[j] = static_cast<int>(row - static_cast<int64_t>(tok[j]) * heads);
-    const int h = head[j] - Hq;
-    const float* src = h < 0 ? p.q + tok[j] * p.q_stride + head[j] * D : p.k + tok[j] * p.k_stride + h * D;
-    x[j] = reinterpret_cast<const float4*>(src)[l16];
-    v[j] = h < 0 ? make_float4(0.f, 0.f, 0.f, 0.f)
-                 : reinterpret_cast<const float4*>(p.v + tok[j] * p.v_stride + h * D)[l16];
+template <int BF16>
+__global__ void __launch_bounds__(kThreads, 12) normed_append_kernel(const NormedAppendLaunch p) {
+  // (rows fit 31 bits: as many of 256 bytes fill no device)
+  const uint32_t Hq = p.g.q_heads, Hkv = p.g.kv_heads, heads = Hq + Hkv;
+  const uint32_t n_rows = static_cast<uint32_t>(p.total_tokens) * heads;
+  const uint32_t l8 = threadIdx.x & 7, row = blockIdx.x * kGroups + (threadIdx.x >> 3);
+  // rows past the end repeat the last one: every lane takes part in the shuffles
+  const uint32_t tok = min(row, n_rows - 1) / heads, head = min(row, n_rows - 1) - tok * heads;
+  const bool query = head < Hq;
+  const Row x = load_row(query ? p.q + tok * p.q_stride + head * D : p.k + tok * p.k_stride + (head - Hq) * D, l8);
+  Row v = x;
+  if (!query) v = load_row(p.v + tok * p.v_stride + (head - Hq) * D, l8);
+  // where the row goes and how it turns, asked for before the norm is ready
+  const int si = find_sequence(p.seqs, p.n_seq, static_cast<int>(tok));
+  const SeqEntry se = p.seqs[si];
+  const int pos = se.base + (static_cast<int>(tok) - se.row_offset);
+  Row cs{};
+  if (p.rotate) cs = load_row(reinterpret_cast<const float*>(p.g.rope + static_cast<size_t>(pos) * (D / 2)), l8);
+  const int32_t blk =
+      query ? 0 : p.g.block_table[static_cast<size_t>(se.slot) * p.g.max_blocks_per_seq + pos / kBlockTokens];
+  Row y = normed(x, load_row(query ? p.q_norm : p.k_norm, l8), p.eps);
+  if (p.rotate) y = {rotate_quad(y.a, cs.a), rotate_quad(y.b, cs.b)};
+  if (row >= n_rows) return;
+  if (query) {
+    store_row(p.q_out + (static_cast<size_t>(tok) * Hq + head) * D, l8, y);
+    return;
   }
-  const float4 gq = reinterpret_cast<const float4*>(p.q_norm)[l16];
-  const float4 gk = reinterpret_cast<const float4*>(p.k_norm)[l16];
-  int si = find_sequence(p.seqs, p.n_seq, tok[0]);
-#pragma unroll
-  for (int j = 0; j < R; ++j) {
-    while (si + 1 < p.n_seq && p.seqs[si + 1].row_offset <= tok[j]) ++si;  // rows ascend
-    const SeqEntry se = p.seqs[si];
-    const int pos = se.base + (tok[j] - se.row_offset);
-    const bool query = head[j] < Hq;
-    float4 y = normed(x[j], query ? gq : gk, p.eps);
-    if (p.rotate)
-      y = rotate_quad(y, reinterpret_cast<const float4*>(p.g.rope + static_cast<size_t>(pos) * (D / 2))[l16]);
-    if (row0 + 16 * j >= n_rows) continue;
-    if (query) {
-      reinterpret_cast<float4*>(p.q_out + (static_cast<int64_t>(tok[j]) * Hq + head[j]) * D)[l16] = y;
-      continue;
+  const size_t dst = static_cast<size_t>(p.layer) * p.g.layer_elems +
+                     ((static_cast<size_t>(pool_block(p.g, blk)) * Hkv + (head - Hq)) * kBlockTokens +
+                      pos % kBlockTokens) * D;
+  // The pool never holds a non-finite value: such a row's lanes store zeros
+  // and its sequence's step fails.
+  if constexpr (BF16) {
+    uint4 ks = make_uint4(bf16_pair(y.a.x, y.a.y), bf16_pair(y.a.z, y.a.w), bf16_pair(y.b.x, y.b.y),
+                          bf16_pair(y.b.z, y.b.w));
+    uint4 vs = make_uint4(bf16_pair(v.a.x, v.a.y), bf16_pair(v.a.z, v.a.w),
+                          bf16_pair(v.b.x, v.b.y), bf16_pair(v.b.z, v.b.w));
+    if (not_finite(ks.x) || not_finite(ks.y) || not_finite(ks.z) || not_finite(ks.w) || not_finite(vs.x) ||
+        not_finite(vs.y) || not_finite(vs.z) || not_finite(vs.w)) {
+      ks = vs = make_uint4(0u, 0u, 0u, 0u);
+      atomicOr(&p.status[si], kStatusNonFinite);
     }
-    const int32_t blk = pool_block(
-        p.g, p.g.block_table[static_cast<size_t>(se.slot) * p.g.max_blocks_per_seq + pos / kBlockTokens]);
-    const size_t dst =
-        static_cast<size_t>(p.layer) * p.g.layer_elems +
-        ((static_cast<size_t>(blk) * Hkv + (head[j] - Hq)) * kBlockTokens + pos % kBlockTokens) * D;
-    // The pool never holds a non-finite value: such a row's lanes store zeros
-    // and its sequence's step fails.
-    if constexpr (BF16) {
-      __nv_bfloat162 kq[2] = {__floats2bfloat162_rn(y.x, y.y), __floats2bfloat162_rn(y.z, y.w)};
-      __nv_bfloat162 vq[2] = {__floats2bfloat162_rn(v[j].x, v[j].y), __floats2bfloat162_rn(v[j].z, v[j].w)};
-      const float2 a = __bfloat1622float2(kq[0]), b = __bfloat1622float2(kq[1]);
-      const float2 c = __bfloat1622float2(vq[0]), d = __bfloat1622float2(vq[1]);
-      const bool fin = all_finite(make_float4(a.x, a.y, b.x, b.y)) && all_finite(make_float4(c.x, c.y, d.x, d.y));
-      uint2 ks = *reinterpret_cast<uint2*>(kq), vs = *reinterpret_cast<uint2*>(vq);
-      if (!fin) {
-        ks = vs = make_uint2(0u, 0u);
-        atomicOr(&p.status[si], kStatusNonFinite);
-      }
-      reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.g.k) + dst)[l16] = ks;
-      reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.g.v) + dst)[l16] = vs;
-    } else {
-      float4 vs = v[j];
-      if (!all_finite(y) || !all_finite(vs)) {
-        y = vs = make_float4(0.f, 0.f, 0.f, 0.f);
-        atomicOr(&p.status[si], kStatusNonFinite);
-      }
-      reinterpret_cast<float4*>(static_cast<float*>(p.g.k) + dst)[l16] = y;
-      reinterpret_cast<float4*>(static_cast<float*>(p.g.v) + dst)[l16] = vs;
+    reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.g.k) + dst)[l8] = ks;
+    reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.g.v) + dst)[l8] = vs;
+  } else {
+    Row vs = v;
+    if (!all_finite(y.a) || !all_finite(y.b) || !all_finite(vs.a) || !all_finite(vs.b)) {
+      y.a = y.b = vs.a = vs.b = make_float4(0.f, 0.f, 0.f, 0.f);
+      atomicOr(&p.status[si], kStatusNonFinite);
     }
+    store_row(static_cast<float*>(p.g.k) + dst, l8, y);
+    store_row(static_cast<float*>(p.g.v) + dst, l8, vs);
   }
 }
 
@@ -102,11 +112,10 @@ __global__ void __launch_bounds__(kThreads) normed_append_kernel(const NormedApp
 cudaError_t launch_normed_append(const NormedAppendLaunch& p, cudaStream_t s) {
   const int64_t rows = static_cast<int64_t>(p.total_tokens) * (p.g.q_heads + p.g.kv_heads);
   if (rows <= 0) return cudaSuccess;
-  auto run = [&](auto kernel, int r) {
-    kernel<<<static_cast<unsigned>((rows + 16 * r - 1) / (16 * r)), kThreads, 0, s>>>(p);
-    return cudaGetLastError();
-  };
-  return p.g.bf16 ? run(normed_append_kernel<1, 1>, 1) : run(normed_append_kernel<0, 1>, 1);
+  const unsigned grid = static_cast<unsigned>((rows + kGroups - 1) / kGroups);
+  if (p.g.bf16) normed_append_kernel<1><<<grid, kThreads, 0, s>>>(p);
+  else normed_append_kernel<0><<<grid, kThreads, 0, s>>>(p);
+  return cudaGetLastError();
 }
 
 }  // namespace slmkv

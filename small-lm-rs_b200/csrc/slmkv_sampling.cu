@@ -15,6 +15,8 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
+// (without ordering of memory: that all CTAs of the cluster have started)
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // Writes a 16-byte record to CTA `rank`'s shared memory, at the same place as p
@@ -74,7 +76,7 @@ __global__ void __launch_bounds__(kProbThreads, 4) probabilities_kernel(const Pr
   __shared__ int red_first[kProbThreads / 32], red_bad[kProbThreads / 32];
   __shared__ __align__(16) ProbSlice slices[kMaxCluster];
   const int ctas = p.cluster, rank = static_cast<int>(cluster_rank()), row = blockIdx.x / ctas, V = p.vocab;
-  if (ctas > 1) cluster_arrive();  // the row's CTAs have all started once the wait below returns
+  if (ctas > 1) cluster_arrive_relaxed();  // the row's CTAs have all started once the wait below returns
   const float* x = p.logits + row * p.logits_stride;
   float* y = p.out + static_cast<int64_t>(row) * V;
   const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(x) >> 2) & 3);
@@ -141,6 +143,7 @@ __global__ void __launch_bounds__(kProbThreads, 4) probabilities_kernel(const Pr
 #pragma unroll 4
     for (int i = begin + threadIdx.x; i < end; i += kProbThreads) {
       const float4 a = power(load(i));
+      if constexpr (KEEP) kept[i - begin] = a;
       sum += (a.x + a.y) + (a.z + a.w);
     }
   } else {
@@ -188,7 +191,7 @@ __global__ void __launch_bounds__(kProbThreads, 4) probabilities_kernel(const Pr
     const float f = m == -INFINITY ? 0.f : exp2_fast((m - top) * c) / total;
 #pragma unroll 4
     for (int i = begin + threadIdx.x; i < end; i += kProbThreads) {
-      const float4 a = power(load(i));
+      const float4 a = KEEP ? load(i) : power(load(i));
       store(i, make_float4(a.x * f, a.y * f, a.z * f, a.w * f));
     }
   }
@@ -223,7 +226,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyL
   __shared__ int s_first, s_flags;
   const int ctas = p.cluster, rank = static_cast<int>(cluster_rank()), i = blockIdx.x / ctas, V = p.vocab;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (ctas > 1) cluster_arrive();  // the row's CTAs have all started once the wait below returns
+  if (ctas > 1) cluster_arrive_relaxed();  // the row's CTAs have all started once the wait below returns
   const SeqEntry se = p.seqs[i];
   const int k = se.count - 1;              // drafts
   const int r0 = se.row_offset;            // target rows of the sequence
