@@ -262,7 +262,8 @@ slm_status slm_batch_append_layer_normed(slm_batch* batch, int32_t layer, const 
  * through slm_batch_prefill_attention. A batch's first call plans it for all
  * layers; plan buffers and the joined parts' scratch are allocated by the
  * context's first call and grow when a call needs more (which waits for the
- * device). */
+ * device). A batch's first call is refused while its stream is being captured
+ * into a graph. */
 slm_status slm_batch_shared_attention(slm_batch* batch, int32_t layer, const float* d_query,
                                       int32_t rotate_query, float* d_out);
 /* Probabilities of logit rows (no reference counterpart: greedy.rs takes the
@@ -271,7 +272,8 @@ slm_status slm_batch_shared_attention(slm_batch* batch, int32_t layer, const flo
  * `rows` rows of vocab_size f32, logits_stride values apart; rows is the batch's
  * number of tokens (slm_model_score) or of sequences (slm_model_prefill,
  * slm_model_decode). d_temperatures: [rows], or NULL for 1. d_probabilities:
- * [rows, vocab_size], dense; it may be d_logits when those are dense. A logit of
+ * [rows, vocab_size], dense; it may be d_logits when those are dense. vocab_size
+ * up to 2^30. A logit of
  * -inf is a masked token. A row with a NaN or +inf logit, with nothing but -inf,
  * or with a temperature that is negative or not finite becomes zeros and its
  * sequence fails with SLM_ERR_NON_FINITE when the batch ends. */
@@ -291,7 +293,7 @@ slm_status slm_batch_token_probabilities(slm_batch* batch, const float* d_logits
  * rejected draft's row (from its p where nothing of that is left), or after the
  * last draft from its row's p: the first token whose running sum of weights in
  * token order exceeds u times their total. Outside [0, 1) u counts as the nearer
- * end. Kept cache lengths: slm_seqs_truncate_all to base + 1 + accepted after
+ * end, NaN as 0. The outputs overlap nothing else. Kept cache lengths: slm_seqs_truncate_all to base + 1 + accepted after
  * the batch's end. A drafted token outside the vocabulary fails its sequence with
  * SLM_ERR_INVALID_INPUT when the batch ends, a row it reads that is negative, not
  * finite or all zero with SLM_ERR_NON_FINITE; both give 0 accepted and next token

@@ -11,6 +11,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <exception>
 #include <memory>
 #include <new>
 #include <random>
@@ -224,6 +225,9 @@ struct slm_ctx {
     float* part_acc = nullptr;
     float2* part_ml = nullptr;
     size_t part_cap = 0;  // row slots
+    // The batch that used the parts last: its descriptor slot and stream.
+    int32_t last_slot = -1;
+    cudaStream_t last_stream = nullptr;
   } shared;
   size_t upd_cap = 0, copy_cap = 0;
 
@@ -1767,7 +1771,9 @@ slm_status slm_batch_append_layer_normed(slm_batch* b, int32_t layer, const floa
   const bool in_place = d_query_out == d_query && query_stride == qw;
   if ((!in_place && ranges_overlap(d_query_out, out_bytes, d_query, span(query_stride, qw))) ||
       ranges_overlap(d_query_out, out_bytes, d_keys, span(key_stride, kw)) ||
-      ranges_overlap(d_query_out, out_bytes, d_values, span(value_stride, kw)))
+      ranges_overlap(d_query_out, out_bytes, d_values, span(value_stride, kw)) ||
+      ranges_overlap(d_query_out, out_bytes, d_query_norm, kHeadDim * sizeof(float)) ||
+      ranges_overlap(d_query_out, out_bytes, d_key_norm, kHeadDim * sizeof(float)))
     return input_error(ctx, SLM_ERR_INVALID_INPUT, what, "the output may not overlap the inputs");
   rc = flush_excess(ctx, b->stream, 0, 0);  // the append reads the device block table
   if (rc) return rc;
@@ -2010,12 +2016,21 @@ void build_shared_plan(const slm_ctx* c, const slm_batch* b, SharedPlan& plan) {
 // Builds and uploads the open batch's plan (once a batch: its layers share it).
 slm_status shared_prepare(slm_batch* b) {
   slm_ctx* c = b->ctx;
+  // Planning waits for the slot's last upload, and the plan is one batch's.
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  CU(c, cudaStreamIsCapturing(b->stream, &capture));
+  if (capture != cudaStreamCaptureStatusNone)
+    return input_error(c, SLM_ERR_INVALID_INPUT, "shared prefix attention", "a batch's first call cannot be captured");
   if (!c->have_maps) {
     const slm_status rc = make_pool_maps(c);
     if (rc) return rc;
   }
   SharedPlan& plan = c->shared_plan;
-  build_shared_plan(c, b, plan);
+  try {
+    build_shared_plan(c, b, plan);
+  } catch (const std::exception&) {  // (no exception crosses the C boundary)
+    return input_error(c, SLM_ERR_INVALID_INPUT, "shared prefix attention", "no host memory for the step's plan");
+  }
   if (plan.parts > INT32_MAX || plan.items.size() + plan.units.size() > static_cast<size_t>(INT32_MAX))
     return input_error(c, SLM_ERR_INVALID_INPUT, "shared prefix attention", "the step has too many rows");
   size_t bytes = 0;
@@ -2074,6 +2089,11 @@ slm_status shared_prepare(slm_batch* b) {
   put(o_merge, plan.merge);
   // the kernels that last read the slot's device buffer are done
   CU(c, cudaStreamWaitEvent(b->stream, c->up_batch.consumed[k], 0));
+  // and so are those that last used the parts, of a batch on another stream too
+  if (io.last_slot >= 0 && io.last_stream != b->stream)
+    CU(c, cudaStreamWaitEvent(b->stream, c->up_batch.consumed[io.last_slot], 0));
+  io.last_slot = k;
+  io.last_stream = b->stream;
   CU(c, cudaMemcpyAsync(io.d[k], h, bytes, cudaMemcpyHostToDevice, b->stream));
   CU(c, cudaEventRecord(io.copied[k], b->stream));
   SharedAttentionLaunch& p = b->shared;
@@ -2136,6 +2156,8 @@ slm_status batch_open_check(slm_batch* b) {
     return input_error(b->ctx, SLM_ERR_INVALID_INPUT, "batch", "the batch is not open");
   return need_device(b->ctx);
 }
+// Of token probabilities: lines of a row and their values count in 32 bits.
+constexpr int32_t kMaxVocab = 1 << 30;
 bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 }  // namespace
 
@@ -2154,9 +2176,9 @@ slm_status slm_batch_token_probabilities(slm_batch* b, const float* d_logits, in
   if (rows != n && rows != b->total_tokens)
     return input_error(ctx, SLM_ERR_INVALID_INPUT, what,
                        "%d rows are neither one a sequence (%d) nor one a token (%d)", rows, n, b->total_tokens);
-  if (vocab_size <= 0 || logits_stride < vocab_size)
+  if (vocab_size <= 0 || vocab_size > kMaxVocab || logits_stride < vocab_size)
     return input_error(ctx, SLM_ERR_INVALID_INPUT, what,
-                       "the vocabulary must be positive and no wider than the logits' row stride");
+                       "the vocabulary must be in 1..=%d and no wider than the logits' row stride", kMaxVocab);
   const size_t in = static_cast<size_t>((rows - 1) * logits_stride + vocab_size) * sizeof(float);
   const size_t out = static_cast<size_t>(rows) * vocab_size * sizeof(float);
   const bool in_place = d_logits == d_probabilities && (rows == 1 || logits_stride == vocab_size);
@@ -2198,6 +2220,14 @@ slm_status slm_batch_verify_drafts(slm_batch* b, int32_t vocab_size, const int32
   if (vocab_size <= 0 || vocab_size > verify_max_vocab())
     return input_error(ctx, SLM_ERR_INVALID_INPUT, what, "vocabulary size %d is outside 1..=%lld", vocab_size,
                        static_cast<long long>(verify_max_vocab()));
+  const size_t n = b->seq_ids.size(), rows = static_cast<size_t>(b->total_tokens), row_bytes = sizeof(float) * vocab_size;
+  for (const void* o : {d_accepted, d_next_tokens})
+    if (ranges_overlap(o, 4 * n, d_token_ids, 4 * rows) || ranges_overlap(o, 4 * n, d_target, rows * row_bytes) ||
+        (d_draft && ranges_overlap(o, 4 * n, d_draft, (rows - n) * row_bytes)) ||
+        ranges_overlap(o, 4 * n, d_uniforms, 4 * rows))
+      return input_error(ctx, SLM_ERR_INVALID_INPUT, what, "the outputs may not overlap the inputs");
+  if (ranges_overlap(d_accepted, 4 * n, d_next_tokens, 4 * n))
+    return input_error(ctx, SLM_ERR_INVALID_INPUT, what, "the outputs may not overlap each other");
   VerifyLaunch p{};
   p.seqs = b->dev.seqs;
   p.n_seq = static_cast<int32_t>(b->seq_ids.size());

@@ -236,6 +236,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyL
     s_flags = 0;
   }
   __syncthreads();
+  auto uniform = [&](int r) { return fmin(fmax(static_cast<double>(p.uniforms[r]), 0.0), 1.0); };  // (NaN: 0)
   for (int j = tid; j < k; j += kVerifyThreads) {
     const int x = p.token_ids[r0 + j + 1];
     if (static_cast<uint32_t>(x) >= static_cast<uint32_t>(V)) {
@@ -244,9 +245,9 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyL
     }
     const float pt = p.target[static_cast<int64_t>(r0 + j) * V + x];
     const float qt = p.draft ? p.draft[(q0 + j) * V + x] : 1.f;
-    if (!(static_cast<double>(p.uniforms[r0 + j]) * qt < static_cast<double>(pt))) atomicMin(&s_first, j);
+    if (!(uniform(r0 + j) * qt < static_cast<double>(pt))) atomicMin(&s_first, j);
   }
-  const double u = fmax(static_cast<double>(p.uniforms[r0 + k]), 0.0);
+  const double u = uniform(r0 + k);
   __syncthreads();
   const int a = s_first;
   const int skip = !p.draft && a < k ? p.token_ids[r0 + a + 1] : -1;  // a draft without probabilities: q = 1 there

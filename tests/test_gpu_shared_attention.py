@@ -300,3 +300,52 @@ def test_refusals():
     b.shared_prefix_attention(0, q, out)
     b.end()
     assert slmkv.lib().slm_batch_shared_attention(None, 0, None, 0, None) == slmkv.ERR_INVALID_INPUT
+
+
+def test_captured_and_replayed():
+    """A batch's first call plans and is refused under capture; later ones are
+    captured, and a replay reads the buffers' new contents."""
+    f = Forest(8, 2, [path((1, 160), (50 * i, 9)) for i in range(2, 30)], [2] * 28, seed=12, dtype="bf16")
+    stream = torch.cuda.Stream()
+    q, k, v = f.new_rows()
+    out, first = torch.empty_like(q), torch.empty_like(q)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        b = f.pool.begin(f.caches, f.counts)
+        b.append_layer(0, k, v, rotate_keys=False)
+        empty, graph = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(empty, stream=stream):
+            torch.ones(1, device="cuda")  # (a graph of something)
+            with pytest.raises(slmkv.InvalidInput, match="captured"):
+                b.shared_prefix_attention(0, q, out, rotate_query=False)
+        b.shared_prefix_attention(0, q, first, rotate_query=False)
+        with torch.cuda.graph(graph, stream=stream):
+            b.shared_prefix_attention(0, q, out, rotate_query=False)
+        graph.replay()
+        stream.synchronize()
+        ref, tol = f.reference(0, q, k, v)
+        assert torch.equal(out, first) and (out.double() - ref).abs().max().item() <= tol
+        q.copy_(f.randn(*q.shape))
+        graph.replay()
+        stream.synchronize()
+        ref, tol = f.reference(0, q, k, v)
+        assert (out.double() - ref).abs().max().item() <= tol
+        b.end()
+
+
+def test_a_rolled_back_step_and_the_next_on_another_stream():
+    """Both use the context's scratch for joined parts."""
+    f = Forest(4, 2, [path((1, 640), (9000 * (i + 1), 5)) for i in range(32)], [1] * 32, seed=13)
+    rows = f.new_rows()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    outs = []
+    for turn in range(4):
+        with torch.cuda.stream(streams[turn % 2]):
+            b = f.pool.begin(f.caches, f.counts)
+            outs.append(f.attend(b, 0, rows))
+            b.rollback()
+    torch.cuda.synchronize()
+    ref, tol = f.reference(0, *rows)
+    for out in outs:
+        assert (out.double() - ref).abs().max().item() <= tol

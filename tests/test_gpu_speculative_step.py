@@ -461,6 +461,45 @@ def test_verify_refusals():
     b.rollback()
 
 
+def test_verify_uniforms_outside_their_range():
+    """They count as the nearer end, for the drafts as for the draw."""
+    p = torch.tensor([[0.0, 0.5, 0.5], [1.0, 0.0, 0.0]], device="cuda")
+    q = torch.tensor([[0.25, 0.375, 0.375]], device="cuda")
+    for draft, u, acc, nxt in ((0, -1.0, 0, 1),       # 0 < p fails: p = 0
+                               (1, 2.0, 1, 0),        # q < p, though 2 q > p
+                               (1, -math.inf, 1, 0), (1, math.inf, 1, 0), (0, math.inf, 0, 2),
+                               (1, math.nan, 1, 0)):  # as 0
+        ids = torch.tensor([0, draft], dtype=torch.int32, device="cuda")
+        uniforms = torch.tensor([u, u], device="cuda")
+        assert run_verify([2], ids, p, q, uniforms)[:2] == ([acc], [nxt]), (draft, u)
+
+
+def test_outputs_over_inputs_are_refused():
+    pool, b = rows_batch([2, 1])
+    words = torch.zeros(64, dtype=torch.int32, device="cuda")
+    floats = words.view(torch.float32)
+    good = dict(token_ids=words[:3], target=floats[8:32].view(3, 8), draft=floats[32:40].view(1, 8),
+                uniforms=floats[40:43], accepted=words[44:46], next_tokens=words[46:48])
+    for bad in (dict(accepted=words[2:4]), dict(next_tokens=words[30:32]), dict(accepted=words[39:41]),
+                dict(next_tokens=words[42:44]), dict(next_tokens=words[45:47])):
+        with pytest.raises(slmkv.InvalidInput, match="overlap"):
+            b.verify_drafts(**{**good, **bad})
+    fn = slmkv.lib().slm_batch_token_probabilities
+    assert fn(b._h, floats[:4].data_ptr(), 3, 2**30 + 1, 2**30 + 1, None, 4) == slmkv.ERR_INVALID_INPUT
+    b.rollback()
+    g = gen(4)
+    pool = make_pool()
+    q, k, v = randn(g, 2, 4, D), randn(g, 2, 2, D), randn(g, 2, 2, D)
+    buf = torch.ones(q.numel() + D, device="cuda")
+    b = pool.begin([pool.allocate_kv_cache(64)], 2)
+    for at in (0, q.numel() - D):
+        w = buf[at:at + D]
+        for norms in ((w, buf[-D:]), (buf[-D:], w)):
+            with pytest.raises(slmkv.InvalidInput, match="overlap"):
+                b.append_layer_normed(0, q, k, v, *norms, buf[:-D].view(q.shape))
+    b.rollback()
+
+
 # ---- together ------------------------------------------------------------------
 
 
