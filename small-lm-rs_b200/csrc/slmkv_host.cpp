@@ -1811,6 +1811,12 @@ constexpr int32_t kSharedMinBlocks = 4;
 // Rows (tokens x query heads of a KV head) from which a shared run goes to the
 // tensor cores' 128-row tiles.
 constexpr int32_t kSharedTcMinRows = 48;
+// And only where a batch has enough such work, as eight-row units x blocks for
+// each warp of the other kernel: below, a launch more costs more than it saves.
+// Batches of 16 and 64 over 64 to 4096 shared tokens, with and without: at 0.6 a
+// warp 12.3 and 10.5 us, at 1.2 14.4 and 12.3, at 2.3 18.4 and 20.1 (or alike),
+// at 4.6 16.4 and 27.0, at 37 28.7 and 43.0.
+constexpr int32_t kSharedTcMinWork = 2;
 
 // The tree below the members order[lo, hi), which share their blocks before
 // `start` (edge `parent` ends there) and, beyond it, those before `probe`.
@@ -1876,12 +1882,16 @@ void build_shared_plan(const slm_ctx* c, const slm_batch* b, SharedPlan& plan) {
   // Tensor-core runs are cut into items that fill the SMs (two CTAs each) about
   // once, of two tiles at least, or of one while those do not fill the SMs.
   plan.on_tc.assign(n_edges, 0);
+  int64_t shared_work = 0;
   for (int32_t i = 0; i < n_edges; ++i) {
     const auto& e = plan.tree[i];
     const int32_t rows = (plan.token0[e.seq1] - plan.token0[e.seq0]) * G;
-    plan.on_tc[i] = e.seq1 - e.seq0 > 1 && rows >= kSharedTcMinRows &&
-                    e.last_block - e.first_block >= 2 * kSharedTcBlocks;
+    const int32_t nb = e.last_block - e.first_block;
+    plan.on_tc[i] = e.seq1 - e.seq0 > 1 && rows >= kSharedTcMinRows && nb >= 2 * kSharedTcBlocks;
+    if (plan.on_tc[i]) shared_work += static_cast<int64_t>((rows + kSharedRows - 1) / kSharedRows) * Hkv * nb;
   }
+  const int64_t ctas = static_cast<int64_t>(kSharedCtasPerSm) * c->num_sms;
+  if (shared_work < kSharedTcMinWork * 4 * ctas) plan.on_tc.assign(n_edges, 0);
   const int32_t tile = kSharedRows / G, tc_tile = kSharedTcRows / G;
   auto tiles_of = [&](int32_t i) {
     const auto& e = plan.tree[i];
@@ -1915,12 +1925,15 @@ void build_shared_plan(const slm_ctx* c, const slm_batch* b, SharedPlan& plan) {
     tc_room += kSharedTcBlocks;
   }
   // The other runs form one stream of (edge, head, row tile) units that the
-  // warps of one wave share evenly, or its CTAs as teams of four warps where a
-  // warp would get fewer than kTeamBelow blocks. A list's budget counts blocks,
-  // and for each piece of a unit what starting and delivering it costs.
-  constexpr int32_t kTeamBelow = 6, kPieceCost = 3;
-  const int64_t ctas = static_cast<int64_t>(kSharedCtasPerSm) * c->num_sms;
-  plan.team = work < kTeamBelow * 4 * ctas;
+  // warps of one wave share evenly, or its CTAs as teams of four warps: few units,
+  // of which a warp would get fewer than kTeamBelow blocks, finish sooner as
+  // teams, and need less joining (64 units of 30 tokens 6 against 9 us, 128 of
+  // 2000 20 against 23); of many units, or long ones, teams only add their joins
+  // (1600 of 30 tokens 23 against 11 us, 200 of 2000 33 against 25). A list's
+  // budget counts blocks, and for each piece of a unit what starting and
+  // delivering it costs.
+  constexpr int32_t kTeamBelow = 12, kPieceCost = 3;
+  plan.team = n_units <= ctas && work < kTeamBelow * 4 * ctas;
   const int64_t lists = plan.team ? ctas : 4 * ctas;
   const int32_t step = plan.team ? 8 : 2;  // blocks of a step, at most
   const int32_t budget = static_cast<int32_t>(

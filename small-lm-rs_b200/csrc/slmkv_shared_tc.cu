@@ -3,24 +3,28 @@
 //
 // A CTA takes 128 rows (128/G tokens x the G query heads of one KV head) over a
 // run of 64-token tiles. Per tile
-//   S = Q K^T     tcgen05.mma kind::f16, M = 128, N = 64, Q in three bf16 parts
-//                 that hold the scaled f32 query exactly (K = 3 x 64)
-//   P = 2^(S - m) one thread a row (TMEM lane), running maximum m; P in three
-//                 bf16 parts into TMEM, in the place of S and 32 columns more
-//   O = P V       M = 128, N = 64, the three parts summed, V from shared memory
-//                 as an MN-major operand
+//   S = Q K^T     tcgen05.mma kind::f16, M = 128, N = 64
+//   P = 2^(S - m) one thread a row (TMEM lane), running maximum m
+//   O = P V       M = 128, N = 64, V from shared memory as an MN-major operand
 // and the thread adds the tile's O to its row's 64 f32 registers: the tensor
 // cores cut off their running sums, so none of them runs over more than a tile.
-// That makes the result as exact as f32 arithmetic at six bf16 products' cost
-// instead of two. Keys and values of f32 pools are split the same way on their
-// way into shared memory, by three loading warps, and take twelve products (those
-// of a mid or lo part with a lo part, below 2^-23 of a term, are left out).
+//
+// All operands are f16 parts under power-of-two scales that bring the largest
+// value of a query row, of a key or value block (16 tokens of a head) and the
+// weights to 2^14..2^15: a bf16 value has one part, exact, an f32 value two, hi
+// and lo, that hold it to 2^-22 (what lies more than 2^25 below the largest value
+// keeps 2^-39 of that one instead). So a tile takes two products a sum where keys
+// and values are bf16 and three where they are f32 (lo times lo, below 2^-22 of a
+// term, is left out). With three bf16 parts, which need no scales, it were three
+// and six; f16 parts of Q also fit into TMEM beside the rest, and a product with
+// its first operand there takes 34 cycles instead of the 51 that reading both
+// from shared memory takes. Keys and values arrive as swizzled boxes by the copy
+// engine and are turned into parts where they lie, by a warp a block.
 //
 // Scores have two buffers, so a tile's softmax runs under the last one's P V and
-// the next one's Q K^T; two CTAs an SM (256 TMEM columns and 113 KiB each).
-// (With one buffer of 128-token tiles a CTA's steps waited on each other: 3400
-// cycles a tile and SM, against the products' 1536.) Bound by the tensor cores,
-// and nearly as much by the powers and their splitting.
+// the next one's Q K^T; two CTAs an SM (256 TMEM columns and 97 KiB each).
+#include <cuda_fp16.h>
+
 #include <cfloat>
 #include <type_traits>
 
@@ -34,52 +38,64 @@ constexpr float kScaleLog2e = 0.125f * 1.4426950408889634f;
 constexpr int kRows = 128;
 constexpr int kTokens = 64;  // of a tile: 4 blocks
 constexpr int kTileBlocks = kTokens / kBlockTokens;
-constexpr int kQBytes = kRows * D * 2;       // 16 KiB a part
-constexpr int kTileBytes = kTokens * D * 2;  // 8 KiB
-constexpr int kThreads = 256;                // softmax warpgroup, producer warpgroup
-constexpr int kRegsLaunch = 128;
-constexpr int kMmaWarp = 4, kLoadWarp = 5;  // bf16: one loading warp; f32: three
-// TMEM columns: two buffers of S (64), each with the P parts (96) in its place; O
-constexpr int kTmemCols = 256, kBufCols = 96, kOCol = 192;
+constexpr int kTileBytes = kTokens * D * 2;  // 8 KiB: of a part
+constexpr int kBlockBytes = kBlockTokens * D * 2;
+constexpr int kThreads = 384;  // softmax warpgroup; one that makes parts; products and copies
+constexpr int kRegsLaunch = 80, kRegsSoftmax = 168, kRegsParts = 40, kRegsIssue = 32;
+static_assert(kRegsSoftmax + kRegsParts + kRegsIssue <= 3 * kRegsLaunch,
+              "the setmaxnreg split must fit the registers the CTA is launched with");
+constexpr int kMmaWarp = 8, kLoadWarp = 9;
+// TMEM columns: Q's parts; two buffers of S (64), each with the P parts in its
+// place; O
+constexpr int kTmemCols = 256, kQCol = 0, kBufCol = 64, kBufCols = 64, kOCol = 192;
+struct Scales {  // of a tile's blocks
+  float key[4];   // 2^-b: of the scores
+  int value[4];   // c + 127: values are times 2^c
+};
 template <int BF16>
 struct TcCfg {
-  static constexpr int kStages = BF16 ? 4 : 1;  // of K and of V
-  static constexpr int kParts = BF16 ? 1 : 3;   // of K and of V
+  static constexpr int kStages = BF16 ? 6 : 3;  // of K and of V
+  static constexpr int kParts = BF16 ? 1 : 2;   // of K and of V
   static constexpr int kStageBytes = kParts * kTileBytes;
-  static constexpr int kLoaders = BF16 ? 1 : 3;
-  static constexpr int kRegsSoftmax = BF16 ? 208 : 168, kRegsProducer = BF16 ? 48 : 88;
-  static_assert(128 * (kRegsSoftmax + kRegsProducer) <= kThreads * kRegsLaunch,
-                "the setmaxnreg split must fit the registers the CTA is launched with");
-  static constexpr int kOffQ = 0;  // three parts
-  static constexpr int kOffK = kOffQ + 3 * kQBytes;
+  static constexpr int kOffK = 0;
   static constexpr int kOffV = kOffK + kStages * kStageBytes;
-  static constexpr int kOffBar = kOffV + kStages * kStageBytes;
+  static constexpr int kOffQ = kOffV + kStages * kStageBytes;  // bf16: Q's lo part
+  static constexpr int kOffBar = kOffQ + (BF16 ? kRows * D * 2 : 0);
+  // Q's rows in f32 pass through the last stages of V at first.
+  static constexpr int kQStageBytes = kRows * D * 4;
+  static constexpr int kFirstQStage = kStages - kQStageBytes / kStageBytes;
+  static_assert(kFirstQStage >= 1, "the first tile's values have a place of their own");
   enum : int {
-    kBarKFull = 0,
-    kBarVFull = kBarKFull + kStages,
-    kBarKFree = kBarVFull + kStages,
+    kBarKRaw = 0,  // copied
+    kBarVRaw = kBarKRaw + kStages,
+    kBarKFree = kBarVRaw + kStages,
     kBarVFree = kBarKFree + kStages,
-    kBarQFull = kBarVFree + kStages,
+    kBarKFull = kBarVFree + kStages,  // in parts
+    kBarVFull = kBarKFull + kStages,
+    kBarQFull = kBarVFull + kStages,
     kBarSFull,  // one a buffer
     kBarPFull = kBarSFull + 2,
     kBarODone,
     kBarDrain,
     kBars
   };
-  static constexpr int kOffMisc = kOffBar + 8 * kBars;  // TMEM base, abort flag
+  // A tile's scales are read before its P is handed over, those of the tile
+  // kStages + 2 later are written after.
+  static constexpr int kRing = 8;
+  static_assert(kRing >= kStages + 2, "scales overwritten while they are read");
+  static constexpr int kOffRing = (kOffBar + 8 * kBars + 15) / 16 * 16;
+  static constexpr int kOffMisc = kOffRing + kRing * static_cast<int>(sizeof(Scales));  // TMEM base, abort flag
   static constexpr int kSmem = kOffMisc + 16;
   static_assert(2 * (kSmem + 1024) <= 228 * 1024, "two CTAs an SM");
 };
-// The products of one sum, as (part of the first operand, part of the second),
-// small ones first.
+// The products of one sum of f32 pools, as (part of the first operand, part of
+// the second), small ones first.
 struct Product {
   int a, b;
 };
-template <int BF16>
 __device__ __forceinline__ constexpr Product product(int i) {
-  constexpr Product kBf16[3] = {{2, 0}, {1, 0}, {0, 0}};
-  constexpr Product kF32[6] = {{2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};
-  return BF16 ? kBf16[i < 3 ? i : 0] : kF32[i];
+  constexpr Product k[3] = {{1, 0}, {0, 1}, {0, 0}};
+  return k[i];
 }
 constexpr unsigned long long kWaitNs = 1000000000ull;  // 1 s
 constexpr int kWaitSpins = 1 << 26;
@@ -131,11 +147,11 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, uint32_t
   }
   return false;
 }
-__device__ __forceinline__ void tma_block(uint32_t dst, const CUtensorMap* map, int y, uint32_t bar) {
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
           dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(y), "r"(bar)
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
 // Shared-memory matrix descriptor, 128-byte swizzle; leading and stride byte
@@ -144,9 +160,9 @@ __device__ __forceinline__ uint64_t matrix(uint32_t addr, uint32_t leading, uint
   return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(leading & 0x3FFFu) << 16) |
          (static_cast<uint64_t>(stride & 0x3FFFu) << 32) | (1ull << 46) | (2ull << 61);
 }
-// Instruction descriptor: kind::f16, f32 sums, bf16 operands, A K-major.
-constexpr uint32_t instruction(int m, int n, bool b_mn_major) {
-  return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn_major ? 1u : 0u) << 16) |
+// Instruction descriptor: kind::f16, f32 sums, bf16 or f16 operands, A K-major.
+constexpr uint32_t instruction(int m, int n, bool bf16, bool b_mn_major) {
+  return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | ((b_mn_major ? 1u : 0u) << 16) |
          (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t add) {
@@ -178,10 +194,13 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[32]) {
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr));
 }
-__device__ __forceinline__ void tmem_store8(uint32_t addr, const uint32_t* v) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(v[0]),
-               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t* a, const uint32_t* b) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(addr),
+      "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(a[4]), "r"(a[5]), "r"(a[6]), "r"(a[7]), "r"(b[0]), "r"(b[1]),
+      "r"(b[2]), "r"(b[3]), "r"(b[4]), "r"(b[5]), "r"(b[6]), "r"(b[7])
+      : "memory");
 }
 __device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -189,9 +208,41 @@ __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::
 __device__ __forceinline__ uint32_t swizzled(int r, int u) {
   return static_cast<uint32_t>(((r >> 3) << 10) + ((r & 7) << 7) + (((u ^ r) & 7) << 4));
 }
-// TMEM column of part q (0: hi) of the 16 tokens ks of a tile: the parts take the
-// place of the scores, which are all in registers by then, and the next 64 columns.
-__device__ __forceinline__ constexpr int part_col(int ks, int q) { return 24 * ks + 8 * q; }
+// TMEM column of part q (0: hi) of the 16 inner values ks of Q or P: P's take the
+// place of the scores, which are all in registers by then.
+__device__ __forceinline__ constexpr int part_col(int ks, int q) { return 16 * ks + 8 * q; }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// An f32 pair as two f16 pairs, to 2^-22 of each value in f16's normal range.
+struct Halves {
+  uint32_t hi, lo;
+};
+__device__ __forceinline__ uint32_t half_pair(uint64_t xy) {
+  float x, y;
+  unpack2(xy, x, y);
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+  return r;
+}
+__device__ __forceinline__ Halves split_halves(uint64_t xy) {
+  Halves r;
+  r.hi = half_pair(xy);
+  float x, y;  // what is left, exact
+  unpack2(xy, x, y);
+  asm("{\n\t.reg .b16 h0, h1, n;\n\tmov.b32 {h0, h1}, %4;\n\tmov.b16 n, 0xBC00;\n\t"  // n = -1
+      "fma.rn.f32.f16 %0, h0, n, %2;\n\tfma.rn.f32.f16 %1, h1, n, %3;\n\t}"
+      : "=f"(x), "=f"(y)
+      : "f"(x), "f"(y), "r"(r.hi));
+  r.lo = half_pair(pack2(x, y));
+  return r;
+}
+// The scale 2^c that brings values with this largest exponent field to
+// 2^14..2^15, as c + 127; a block or row of zeros, or nearly, gets 2^126.
+__device__ __forceinline__ int scale_field(int exponent) { return min(268 - exponent, 253); }
+__device__ __forceinline__ float power_of_field(int field) { return __int_as_float(field << 23); }
 // One lane of the warp, in a form that keeps the issued operands uniform: under
 // `lane == 0` each product took 100 to 200 cycles to issue.
 __device__ __forceinline__ bool elect_one() {
@@ -208,7 +259,7 @@ __device__ __forceinline__ int cta_index() {
 template <int BF16, int G>
 __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_constant__ SharedAttentionLaunch p) {
   using Cfg = TcCfg<BF16>;
-  constexpr int kStages = Cfg::kStages, kStageBytes = Cfg::kStageBytes, kProducts = BF16 ? 3 : 6;
+  constexpr int kStages = Cfg::kStages, kStageBytes = Cfg::kStageBytes;
   extern __shared__ __align__(1024) uint8_t sm[];
   const uint32_t sbase = saddr(sm);
   if (sbase & 1023u) {  // uniform: report instead of misreading tiles
@@ -219,9 +270,10 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   auto bar = [&](int i) { return sbase + Cfg::kOffBar + 8u * static_cast<uint32_t>(i); };
   const uint32_t abort = sbase + Cfg::kOffMisc + 4;
+  Scales* ring = reinterpret_cast<Scales*>(sm + Cfg::kOffRing);
   if (tid == 0) {
-    for (int s = 0; s < 4 * kStages; ++s) bar_init(bar(s), s < 2 * kStages ? Cfg::kLoaders : 1);
-    bar_init(bar(Cfg::kBarQFull), BF16 ? 8 : 4);
+    for (int s = 0; s < 6 * kStages; ++s) bar_init(bar(s), s < 4 * kStages ? 1 : 4);
+    bar_init(bar(Cfg::kBarQFull), 4);
     bar_init(bar(Cfg::kBarSFull), 1);
     bar_init(bar(Cfg::kBarSFull + 1), 1);
     bar_init(bar(Cfg::kBarPFull), 4);
@@ -236,62 +288,6 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  // Q rows: a warp writes N of them, one per step, lane l elements 2l and 2l + 1
-  // (one rotation pair): rotated, scaled into the exp2 domain, split. All loads
-  // first: rows beyond the item's tokens load a last one's, and are written as
-  // zeros. bf16: all warps write sixteen, the first copies under way; f32: the
-  // softmax warps write 32, beside the loaders.
-  auto write_q = [&](auto n_rows) {
-    constexpr int kEach = decltype(n_rows)::value;
-    const SharedItem it = p.tc_items[cta_index()];
-    const int Hq = p.g.q_heads, r0 = warp * kEach;
-    // of row r0 + lane
-    const SharedToken tk = p.tokens[it.token0 + min((r0 + (lane & (kEach - 1))) / G, it.n_tokens - 1)];
-    float2 xv[kEach], cv[kEach];
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int row = __shfl_sync(kFullMask, tk.row, i);
-      xv[i] = reinterpret_cast<const float2*>(
-          p.q + (static_cast<size_t>(row) * Hq + it.head * G + (r0 + i) % G) * D)[lane];
-    }
-    if (p.rotate) {
-#pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        const int pos = __shfl_sync(kFullMask, tk.pos, i);
-        cv[i] = p.g.rope[static_cast<size_t>(pos) * (D / 2) + lane];
-      }
-#pragma unroll
-      for (int i = 0; i < kEach; ++i) xv[i] = rotate_pair(xv[i], cv[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const bool live = (r0 + i) / G < it.n_tokens;
-      const Parts s = split_pair(live ? xv[i].x * kScaleLog2e : 0.f, live ? xv[i].y * kScaleLog2e : 0.f);
-      uint8_t* dst = sm + Cfg::kOffQ + swizzled(r0 + i, lane >> 2) + (lane & 3) * 4;
-      *reinterpret_cast<uint32_t*>(dst) = s.hi;
-      *reinterpret_cast<uint32_t*>(dst + kQBytes) = s.mid;
-      *reinterpret_cast<uint32_t*>(dst + 2 * kQBytes) = s.lo;
-    }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncwarp();
-    if (lane == 0) bar_arrive(bar(Cfg::kBarQFull));
-  };
-  // bf16: tile j's keys, then its values, a lane a block (a last tile's blocks
-  // past the run repeat the last one: masked)
-  auto copy_tile = [&](const SharedItem& it, int j, bool keys) {
-    const int st = j % kStages;
-    const int32_t* table = p.g.block_table + static_cast<size_t>(it.slot) * p.g.max_blocks_per_seq + it.first_block;
-    int32_t blk = lane < kTileBlocks ? table[min(j * kTileBlocks + lane, it.n_blocks - 1)] : 0;
-    blk = pool_block(p.g, blk);
-    const int y = (p.layer * p.g.num_blocks * p.g.kv_heads + it.head + blk * p.g.kv_heads) * kBlockTokens;
-    const int full = (keys ? Cfg::kBarKFull : Cfg::kBarVFull) + st;
-    if (lane == 0) bar_expect(bar(full), kTileBytes);
-    __syncwarp();
-    if (lane < kTileBlocks)
-      tma_block(sbase + (keys ? Cfg::kOffK : Cfg::kOffV) + static_cast<uint32_t>(st * kStageBytes + lane * kBlockTokens * 128),
-                keys ? &p.tmap_k : &p.tmap_v, y, bar(full));
-    __syncwarp();
-  };
   fence_before();
   __syncthreads();
   fence_after();
@@ -302,48 +298,119 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
     }
   };
 
-  if (BF16) {
-    if (warp == kLoadWarp) {
-      const SharedItem it = p.tc_items[cta_index()];
-      const int first = min(kStages, (it.n_blocks + kTileBlocks - 1) / kTileBlocks);
-      for (int j = 0; j < first; ++j) {
-        copy_tile(it, j, true);
-        copy_tile(it, j, false);
-      }
-    }
-    write_q(std::integral_constant<int, kRows / 8>{});
-  }
-
   if (warp < 4) {
     // ================= softmax: thread = row =================
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsSoftmax) : "memory");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax) : "memory");
     const SharedItem it = p.tc_items[cta_index()];
-    const uint32_t tmem = ld_flag(sbase + Cfg::kOffMisc);
-    const uint32_t trow = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+    const uint32_t trow = ld_flag(sbase + Cfg::kOffMisc) + (static_cast<uint32_t>(warp * 32) << 16);
     auto wait = [&](int b, uint32_t parity) {
       return __all_sync(kFullMask, bar_wait(bar(b), parity, abort));
     };
-    if (!BF16) write_q(std::integral_constant<int, kRows / 4>{});
-    float o[D];
+    float fin = 0.f;         // NaN once a score is not finite
+    uint64_t fin2 = 0ull;    // (of bf16 pools, two chains)
+    float q_scale = 1.f;     // f32 pools: 2^-a, of the scores
+    {
+      // Q: a warp's 32 rows, read two at a time (rows beyond the item's tokens
+      // read a last one's), rotated, scaled into the exp2 domain, and through
+      // shared memory to their threads
+      const SharedToken tk = p.tokens[it.token0 + min(tid / G, it.n_tokens - 1)];
+      uint8_t* rows = sm + Cfg::kOffV + Cfg::kFirstQStage * kStageBytes + warp * (32 * D * 4);
+      const int u = lane & 15;
 #pragma unroll
-    for (int i = 0; i < D; ++i) o[i] = 0.f;
-    float m = -INFINITY, l = 0.f, corr = 0.f;
-    uint64_t fin = 0ull;
+      for (int b = 0; b < 2; ++b) {
+        float4 x[8], cs[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = 2 * (8 * b + i) + (lane >> 4);
+          const size_t row = __shfl_sync(kFullMask, tk.row, r);
+          x[i] = reinterpret_cast<const float4*>(
+              p.q + (row * p.g.q_heads + it.head * G + (warp * 32 + r) % G) * D)[u];
+          const int pos = __shfl_sync(kFullMask, tk.pos, r);
+          if (p.rotate) cs[i] = reinterpret_cast<const float4*>(p.g.rope + static_cast<size_t>(pos) * (D / 2))[u];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = 2 * (8 * b + i) + (lane >> 4);
+          float4 y = x[i];
+          if (p.rotate) y = rotate_quad(y, cs[i]);
+          *reinterpret_cast<float4*>(rows + r * (D * 4) + ((u ^ (r & 15)) << 4)) =
+              make_float4(y.x * kScaleLog2e, y.y * kScaleLog2e, y.z * kScaleLog2e, y.w * kScaleLog2e);
+        }
+      }
+      __syncwarp();
+      const bool live = tid / G < it.n_tokens;
+      float4 x[D / 4];
+      float most = 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 4; ++i) {
+        x[i] = *reinterpret_cast<const float4*>(rows + lane * (D * 4) + ((i ^ (lane & 15)) << 4));
+        if (!live) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (!BF16) most = fmax3(most, fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
+        fin = fmaf(x[i].x, 0.f, fmaf(x[i].y, 0.f, fmaf(x[i].z, 0.f, fmaf(x[i].w, 0.f, fin))));
+      }
+      const int field = fin == 0.f ? scale_field(__float_as_int(most) >> 23) : 127;
+      if (!BF16) q_scale = power_of_field(254 - field);
+      const uint64_t f2 = pack2(power_of_field(field), power_of_field(field));
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        uint32_t first[8], second[8], third[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float4& v = x[4 * ks + i / 2];
+          const uint64_t w = i & 1 ? pack2(v.z, v.w) : pack2(v.x, v.y);
+          if constexpr (BF16) {
+            const Parts a = split_pair(w);
+            first[i] = a.hi;
+            second[i] = a.mid;
+            third[i] = a.lo;
+          } else {
+            const Halves a = split_halves(mul2(w, f2));
+            first[i] = a.hi;
+            second[i] = a.lo;
+          }
+        }
+        tmem_store16(trow + kQCol + part_col(ks, 0), first, second);
+        if constexpr (BF16) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+            *reinterpret_cast<uint4*>(sm + Cfg::kOffQ + swizzled(tid, 2 * ks + n)) =
+                make_uint4(third[4 * n], third[4 * n + 1], third[4 * n + 2], third[4 * n + 3]);
+        }
+      }
+      tmem_wait_store();
+      fence_before();
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) bar_arrive(bar(Cfg::kBarQFull));
+    }
+    uint64_t o[D / 2];
+#pragma unroll
+    for (int i = 0; i < D / 2; ++i) o[i] = 0ull;
+    float m = -INFINITY, l = 0.f, corr = 0.f, unit = 0.f;
     const int n_tiles = (it.n_blocks + kTileBlocks - 1) / kTileBlocks;
     bool ok = true;  // warp-uniform
-    auto add_o = [&]() {  // o = o corr + O, O of the last product
+    auto add_o = [&]() {  // o = o corr + O unit, O of the last product
+      const uint64_t c2 = pack2(corr, corr), u2 = pack2(unit, unit);
+      const bool same = __all_sync(kFullMask, corr == 1.f);  // most tiles: no row's maximum moved
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         uint32_t v[32];
         tmem_load(trow + kOCol + 32 * c, v);
         tmem_wait_load();
+        if (!same) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[32 * c + i] = fmaf(o[32 * c + i], corr, __uint_as_float(v[i]));
+          for (int i = 0; i < 16; ++i) o[16 * c + i] = mul2(o[16 * c + i], c2);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          o[16 * c + i] = fma2(pack2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), u2, o[16 * c + i]);
       }
     };
     for (int j = 0; j < n_tiles; ++j) {
-      const uint32_t buf = trow + (j & 1) * kBufCols;
+      const uint32_t buf = trow + kBufCol + (j & 1) * kBufCols;
       if (!(ok = wait(Cfg::kBarSFull + (j & 1), (j >> 1) & 1))) break;
+      // the values' scales: bf16, with six stages, has its scores taken after them
+      if (!BF16 && !(ok = wait(Cfg::kBarVFull + j % kStages, (j / kStages) & 1))) break;
       fence_after();
       float s[kTokens];
       {
@@ -354,14 +421,35 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
 #pragma unroll
         for (int i = 0; i < kTokens; ++i) s[i] = __uint_as_float(v[i >> 5][i & 31]);
       }
-      // the run ends in a last tile: what lies beyond gets no weight, and a
-      // finite score for the check below
+      const Scales& sc = ring[j % Cfg::kRing];
+      const int4 vf = *reinterpret_cast<const int4*>(sc.value);
+      float f[4] = {1.f, 1.f, 1.f, 1.f};
+      if constexpr (!BF16) {
+        const float4 ks4 = *reinterpret_cast<const float4*>(sc.key);
+        auto scale = [&](float k) { return fminf(fmaxf(q_scale * k, FLT_MIN), FLT_MAX); };
+        f[0] = scale(ks4.x);
+        f[1] = scale(ks4.y);
+        f[2] = scale(ks4.z);
+        f[3] = scale(ks4.w);
+        // Finite queries give finite S (below 2^36); times a large scale they need
+        // not stay so.
+        if (fmax3(fmaxf(f[0], f[1]), f[2], f[3]) > 0x1p90f) {
+#pragma unroll
+          for (int i = 0; i < kTokens; ++i) fin = fmaf(s[i] * f[i / 16], 0.f, fin);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kTokens / 2; ++i) fin2 = fma2(pack2(s[2 * i], s[2 * i + 1]), 0ull, fin2);
+      }
+      // the run ends in a last tile: what lies beyond gets no weight
       const int valid = (it.n_blocks - j * kTileBlocks) * kBlockTokens;
       if (valid < kTokens) {
 #pragma unroll
         for (int i = 0; i < kTokens; ++i)
-          if (i >= valid) s[i] = -FLT_MAX;
+          if (i >= valid) s[i] = -INFINITY;
       }
+      // the running maximum, rounded up to a whole number: its differences and the
+      // exponents below are exact
       float mx;
       {  // four chains
         float m4[4];
@@ -370,48 +458,46 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
           float x = fmax3(s[16 * k], s[16 * k + 1], s[16 * k + 2]);
 #pragma unroll
           for (int i = 3; i < 15; i += 2) x = fmax3(x, s[16 * k + i], s[16 * k + i + 1]);
-          m4[k] = fmaxf(x, s[16 * k + 15]);
+          m4[k] = fmaxf(x, s[16 * k + 15]) * f[k];
         }
-        mx = fmax3(fmaxf(m, m4[0]), fmaxf(m4[1], m4[2]), m4[3]);
+        mx = ceilf(fmax3(fmaxf(m, m4[0]), fmaxf(m4[1], m4[2]), m4[3]));
       }
       const float next_corr = exp2_fast(m - mx);  // 0 on the first tile
       m = mx;
-      const uint64_t neg = pack2(-mx, -mx);
-      uint64_t sums[2] = {0ull, 0ull};
-      // the next sixteen powers are taken while the last ones are split: the two
-      // keep different units busy
-      uint64_t w[2][8];
-      auto powers = [&](int ks) {
+      float ref = mx;
+      if (fabsf(mx) > 0x1p22f) {  // 15 and the like would be lost beside it
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint64_t x = pack2(s[16 * ks + 2 * i], s[16 * ks + 2 * i + 1]);
-          fin = fma2(x, 0ull, fin);  // +0 per finite score, NaN from a non-finite one on
-          float a, b;
-          unpack2(add2(x, neg), a, b);
-          w[ks & 1][i] = pack2(exp2_fast(a), exp2_fast(b));
-        }
-      };
-      powers(0);
+        for (int i = 0; i < kTokens; ++i) s[i] = fmaf(s[i], f[i / 16], -mx);
+        f[0] = f[1] = f[2] = f[3] = 1.f;
+        ref = 0.f;
+      }
+      // Weights are times 2^15, and a block's by what its values' scale is above
+      // the tile's least (at most 2^60: beyond, the values are nothing beside the
+      // largest ones), so that the products are all in one unit.
+      const int least = min(min(vf.x, vf.y), min(vf.z, vf.w));
+      const int above[4] = {min(vf.x - least, 60), min(vf.y - least, 60), min(vf.z - least, 60), min(vf.w - least, 60)};
+      l *= next_corr;
 #pragma unroll
       for (int ks = 0; ks < kTokens / 16; ++ks) {
-        if (ks + 1 < kTokens / 16) powers(ks + 1);
-        uint32_t hi[8], mid[8], lo[8];
+        const float add = 15.f - ref - static_cast<float>(above[ks]);
+        const uint64_t f2 = pack2(f[ks], f[ks]), up = pack2(add, add);
+        uint64_t sum = 0ull;
+        uint32_t hi[8], lo[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          sums[i & 1] = add2(sums[i & 1], w[ks & 1][i]);
-          const Parts q = split_pair(w[ks & 1][i]);
-          hi[i] = q.hi;
-          mid[i] = q.mid;
-          lo[i] = q.lo;
+          float a, b;
+          const uint64_t x = pack2(s[16 * ks + 2 * i], s[16 * ks + 2 * i + 1]);
+          unpack2(BF16 ? add2(x, up) : fma2(x, f2, up), a, b);
+          const uint64_t w = pack2(exp2_fast(a), exp2_fast(b));
+          sum = add2(sum, w);
+          const Halves h = split_halves(w);
+          hi[i] = h.hi;
+          lo[i] = h.lo;
         }
-        tmem_store8(buf + part_col(ks, 0), hi);
-        tmem_store8(buf + part_col(ks, 1), mid);
-        tmem_store8(buf + part_col(ks, 2), lo);
-      }
-      {
+        tmem_store16(buf + part_col(ks, 0), hi, lo);
         float a, b;
-        unpack2(add2(sums[0], sums[1]), a, b);
-        l = fmaf(l, next_corr, a + b);
+        unpack2(sum, a, b);
+        l = fmaf(a + b, power_of_field(127 + above[ks]), l);
       }
       if (j > 0) {  // the last tile's O, before the next product takes its place
         if (!(ok = wait(Cfg::kBarODone, (j - 1) & 1))) break;
@@ -419,6 +505,7 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
         add_o();
       }
       corr = next_corr;
+      unit = power_of_field(254 - least);
       tmem_wait_store();
       fence_before();
       __syncwarp();
@@ -433,113 +520,171 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
     } else if (tid / G < it.n_tokens) {
       // softmax.rs:17-22: a score that is not finite fails the row's sequence
       float f0, f1;
-      unpack2(fin, f0, f1);
-      if (!(f0 == 0.f && f1 == 0.f) && p.status) atomicOr(&p.status[p.tokens[it.token0 + tid / G].seq], kStatusNonFiniteScore);
+      unpack2(fin2, f0, f1);
+      if (!(fin == 0.f && f0 == 0.f && f1 == 0.f) && p.status) atomicOr(&p.status[p.tokens[it.token0 + tid / G].seq], kStatusNonFiniteScore);
       const size_t slot = static_cast<size_t>(it.part) + tid;
-      p.part_ml[slot] = make_float2(m, l);
-      float4* dst = reinterpret_cast<float4*>(p.part_acc + slot * D);
+      const uint64_t down = pack2(0x1p-15f, 0x1p-15f);
+      p.part_ml[slot] = make_float2(m, l * 0x1p-15f);
+      ulonglong2* dst = reinterpret_cast<ulonglong2*>(p.part_acc + slot * D);
 #pragma unroll
-      for (int i = 0; i < D / 4; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+      for (int i = 0; i < D / 4; ++i) dst[i] = make_ulonglong2(mul2(o[2 * i], down), mul2(o[2 * i + 1], down));
     }
+  } else if (warp < 8) {
+    // ================= parts: block `warp - 4` of every tile, where it lies =================
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsParts) : "memory");
+    const int n_tiles = (p.tc_items[cta_index()].n_blocks + kTileBlocks - 1) / kTileBlocks;
+    const int block = warp - 4;
+    auto wait = [&](int b, uint32_t parity) { return __all_sync(kFullMask, bar_wait(bar(b), parity, abort)); };
+    // Scales one block's values; the scale's field.
+    auto make_parts = [&](uint8_t* base) {
+      if constexpr (BF16) {
+        uint4 x[4];
+        uint32_t most = 0;  // of both halves
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          x[n] = *reinterpret_cast<const uint4*>(base + 512 * n + 16 * lane);
+          most = __vmaxu2(most, __vmaxu2(__vmaxu2(x[n].x & 0x7fff7fffu, x[n].y & 0x7fff7fffu),
+                                         __vmaxu2(x[n].z & 0x7fff7fffu, x[n].w & 0x7fff7fffu)));
+        }
+        const uint32_t top = __reduce_max_sync(kFullMask, max(most & 0xffffu, most >> 16));
+        const int field = scale_field(static_cast<int>(top >> 7));
+        const uint64_t f2 = pack2(power_of_field(field), power_of_field(field));
+        auto part = [&](uint32_t w) {  // exact: eight bits, scaled
+          return half_pair(mul2(pack2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)), f2));
+        };
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+          *reinterpret_cast<uint4*>(base + 512 * n + 16 * lane) =
+              make_uint4(part(x[n].x), part(x[n].y), part(x[n].z), part(x[n].w));
+        return field;
+      } else {
+        // a row's two 128-byte halves lie where its parts go
+        uint32_t most = 0;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+          const uint4 x = *reinterpret_cast<const uint4*>(base + (n >> 2) * kTileBytes + 512 * (n & 3) + 16 * lane);
+          most = max(most, max(max(x.x & 0x7fffffffu, x.y & 0x7fffffffu), max(x.z & 0x7fffffffu, x.w & 0x7fffffffu)));
+        }
+        const int field = scale_field(static_cast<int>(__reduce_max_sync(kFullMask, most) >> 23));
+        const uint64_t f2 = pack2(power_of_field(field), power_of_field(field));
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const int row = 4 * n + (lane >> 3), u = lane & 7;
+          const uint8_t* src = base + (u >> 2) * kTileBytes;
+          const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(src + swizzled(row, 2 * (u & 3)));
+          const ulonglong2 y = *reinterpret_cast<const ulonglong2*>(src + swizzled(row, 2 * (u & 3) + 1));
+          const Halves a = split_halves(mul2(x.x, f2)), b = split_halves(mul2(x.y, f2));
+          const Halves c = split_halves(mul2(y.x, f2)), d = split_halves(mul2(y.y, f2));
+          __syncwarp();  // the four rows have been read
+          *reinterpret_cast<uint4*>(base + swizzled(row, u)) = make_uint4(a.hi, b.hi, c.hi, d.hi);
+          *reinterpret_cast<uint4*>(base + kTileBytes + swizzled(row, u)) = make_uint4(a.lo, b.lo, c.lo, d.lo);
+        }
+        return field;
+      }
+    };
+    bool ok = true;
+    for (int j = 0; ok && j < n_tiles; ++j) {
+      const int st = j % kStages;
+      const uint32_t parity = (j / kStages) & 1;
+      uint8_t* stage = sm + st * kStageBytes + block * kBlockBytes;
+      if constexpr (!BF16) {
+        if (!(ok = wait(Cfg::kBarKRaw + st, parity))) break;
+        const int key = make_parts(stage + Cfg::kOffK);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+          ring[j % Cfg::kRing].key[block] = power_of_field(254 - key);
+          bar_arrive(bar(Cfg::kBarKFull + st));
+        }
+      }
+      if (!(ok = wait(Cfg::kBarVRaw + st, parity))) break;
+      const int value = make_parts(stage + Cfg::kOffV);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+        ring[j % Cfg::kRing].value[block] = value;
+        bar_arrive(bar(Cfg::kBarVFull + st));
+      }
+    }
+    if (!ok) raise();
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsProducer) : "memory");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue) : "memory");
     const SharedItem it = p.tc_items[cta_index()];
     const int n_tiles = (it.n_blocks + kTileBlocks - 1) / kTileBlocks;
-    auto pbar = bar;
-    auto wait = [&](int b, uint32_t parity) { return __all_sync(kFullMask, bar_wait(pbar(b), parity, abort)); };
-    if (BF16 && warp == kLoadWarp) {
-      // ================= loader (the first tiles are on their way) =================
-      int k_issued = min(kStages, n_tiles), v_issued = k_issued;
+    auto wait = [&](int b, uint32_t parity) { return __all_sync(kFullMask, bar_wait(bar(b), parity, abort)); };
+    if (warp == kLoadWarp) {
+      // ================= copies: a lane a box (a last tile's blocks past the run repeat the last one) ==========
+      const int32_t* table = p.g.block_table + static_cast<size_t>(it.slot) * p.g.max_blocks_per_seq + it.first_block;
+      constexpr int kBoxes = BF16 ? 1 : 2;  // of a block, side by side
+      const int block = lane / kBoxes, half = lane % kBoxes;
+      auto copy = [&](int j, int y, bool keys) {
+        const int st = j % kStages;
+        const uint32_t full = bar((keys ? Cfg::kBarKRaw : Cfg::kBarVRaw) + st);
+        if (lane == 0) bar_expect(full, kStageBytes);
+        __syncwarp();
+        if (block < kTileBlocks)
+          tma_box(sbase + (keys ? Cfg::kOffK : Cfg::kOffV) +
+                      static_cast<uint32_t>(st * kStageBytes + half * kTileBytes + block * kBlockBytes),
+                  keys ? &p.tmap_k : &p.tmap_v, 32 * half, y, full);
+        __syncwarp();
+      };
+      int k_issued = 0, v_issued = 0;
       bool ok = true;
-      for (int j = kStages; ok && j < n_tiles; ++j) {
+      for (int j = 0; j < n_tiles; ++j) {
+        int32_t id = block < kTileBlocks ? table[min(j * kTileBlocks + block, it.n_blocks - 1)] : 0;
+        id = pool_block(p.g, id);
+        const int y = ((p.layer * p.g.num_blocks + id) * p.g.kv_heads + it.head) * kBlockTokens;
         const uint32_t parity = static_cast<uint32_t>((j / kStages - 1) & 1);
-        if (!(ok = wait(Cfg::kBarKFree + j % kStages, parity))) break;
-        copy_tile(it, j, true);
+        if (j >= kStages && !(ok = wait(Cfg::kBarKFree + j % kStages, parity))) break;
+        copy(j, y, true);
         k_issued = j + 1;
-        if (!(ok = wait(Cfg::kBarVFree + j % kStages, parity))) break;
-        copy_tile(it, j, false);
+        if (j >= Cfg::kFirstQStage && j < kStages && !(ok = wait(Cfg::kBarQFull, 0))) break;
+        if (j >= kStages && !(ok = wait(Cfg::kBarVFree + j % kStages, parity))) break;
+        copy(j, y, false);
         v_issued = j + 1;
       }
       if (!ok) raise();
       // every copy lands before the CTA's shared memory is released
       for (int j = max(0, k_issued - kStages); j < k_issued; ++j)
-        bar_wait(pbar(Cfg::kBarKFull + j % kStages), (j / kStages) & 1, 0);
+        bar_wait(bar(Cfg::kBarKRaw + j % kStages), (j / kStages) & 1, 0);
       for (int j = max(0, v_issued - kStages); j < v_issued; ++j)
-        bar_wait(pbar(Cfg::kBarVFull + j % kStages), (j / kStages) & 1, 0);
+        bar_wait(bar(Cfg::kBarVRaw + j % kStages), (j / kStages) & 1, 0);
       __syncwarp();
-    } else if (!BF16 && warp >= kLoadWarp) {
-      // ================= loaders: eight values a thread at a time, split =================
-      const int32_t* table = p.g.block_table + static_cast<size_t>(it.slot) * p.g.max_blocks_per_seq + it.first_block;
-      const size_t layer = static_cast<size_t>(p.layer) * p.g.layer_elems;
-      const float* kpool = static_cast<const float*>(p.g.k) + layer;
-      const float* vpool = static_cast<const float*>(p.g.v) + layer;
-      const int i0 = tid - 32 * kLoadWarp;
-      constexpr int kPieces = kTokens * (D / 8), kStep = 96, kEach = (kPieces + kStep - 1) / kStep;
-      auto fetch = [&](const float* pool, int32_t blk, float4 (&x)[kEach][2]) {
-#pragma unroll
-        for (int n = 0; n < kEach; ++n) {
-          const int i = min(i0 + n * kStep, kPieces - 1), row = i >> 3, u = i & 7;
-          const int32_t id = __shfl_sync(kFullMask, blk, row / kBlockTokens);
-          const float* src =
-              pool + ((static_cast<size_t>(id) * p.g.kv_heads + it.head) * kBlockTokens + row % kBlockTokens) * D + 8 * u;
-          x[n][0] = reinterpret_cast<const float4*>(src)[0];
-          x[n][1] = reinterpret_cast<const float4*>(src)[1];
-        }
-      };
-      auto store = [&](int off, const float4 (&x)[kEach][2]) {
-#pragma unroll
-        for (int n = 0; n < kEach; ++n) {
-          const int i = i0 + n * kStep, row = i >> 3, u = i & 7;
-          const Parts a = split_pair(x[n][0].x, x[n][0].y), b = split_pair(x[n][0].z, x[n][0].w);
-          const Parts c = split_pair(x[n][1].x, x[n][1].y), d = split_pair(x[n][1].z, x[n][1].w);
-          if (i < kPieces) {
-            uint8_t* dst = sm + off + swizzled(row, u);
-            *reinterpret_cast<uint4*>(dst) = make_uint4(a.hi, b.hi, c.hi, d.hi);
-            *reinterpret_cast<uint4*>(dst + kTileBytes) = make_uint4(a.mid, b.mid, c.mid, d.mid);
-            *reinterpret_cast<uint4*>(dst + 2 * kTileBytes) = make_uint4(a.lo, b.lo, c.lo, d.lo);
-          }
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-      };
-      bool ok = true;
-      for (int j = 0; ok && j < n_tiles; ++j) {
-        int32_t blk = lane < kTileBlocks ? table[min(j * kTileBlocks + lane, it.n_blocks - 1)] : 0;
-        blk = pool_block(p.g, blk);
-        const uint32_t parity = static_cast<uint32_t>((j - 1) & 1);
-        float4 x[kEach][2];
-        fetch(kpool, blk, x);
-        if (j > 0 && !(ok = wait(Cfg::kBarKFree, parity))) break;
-        store(Cfg::kOffK, x);
-        if (lane == 0) bar_arrive(pbar(Cfg::kBarKFull));
-        fetch(vpool, blk, x);
-        if (j > 0 && !(ok = wait(Cfg::kBarVFree, parity))) break;
-        store(Cfg::kOffV, x);
-        if (lane == 0) bar_arrive(pbar(Cfg::kBarVFull));
-      }
-      if (!ok) raise();
     } else if (warp == kMmaWarp) {
-      // ================= the products (lane 0 issues, the warp waits) =================
+      // ================= the products (one lane issues, the warp waits) =================
       const uint32_t tmem = ld_flag(sbase + Cfg::kOffMisc);
-      constexpr uint32_t kIdS = instruction(kRows, kTokens, false), kIdO = instruction(kRows, D, true);
+      constexpr uint32_t kIdS = instruction(kRows, kTokens, BF16, false), kIdO = instruction(kRows, D, false, true);
       const bool one = elect_one();
       const uint64_t q_desc = matrix(sbase + Cfg::kOffQ, 1, 64), k_desc = matrix(sbase + Cfg::kOffK, 1, 64);
       const uint64_t v_desc = matrix(sbase + Cfg::kOffV, kTileBytes >> 4, 64);
       auto scores = [&](int j) {  // S of tile j into buffer j & 1
         const int st = j % kStages;
-        if (!wait(Cfg::kBarKFull + st, (j / kStages) & 1)) return false;
+        const uint32_t parity = (j / kStages) & 1;
+        if (!wait((BF16 ? Cfg::kBarKRaw : Cfg::kBarKFull) + st, parity) || (BF16 && !wait(Cfg::kBarVFull + st, parity)))
+          return false;
         fence_after();
         if (one) {
           const uint64_t k = k_desc + static_cast<uint64_t>(st * (kStageBytes >> 4));
+          const uint32_t to = tmem + kBufCol + (j & 1) * kBufCols;
+          if constexpr (BF16) {
 #pragma unroll
-          for (int i = 0; i < kProducts; ++i)
+            for (int kk = 0; kk < D / 16; ++kk)
+              mma_ss(to, q_desc + static_cast<uint64_t>(2 * kk), k + static_cast<uint64_t>(2 * kk), kIdS, kk > 0);
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              mma_ss(tmem + (j & 1) * kBufCols,
-                     q_desc + static_cast<uint64_t>(product<BF16>(i).a * (kQBytes >> 4) + 2 * kk),
-                     k + static_cast<uint64_t>(product<BF16>(i).b * (kTileBytes >> 4) + 2 * kk), kIdS, i > 0 || kk > 0);
-          mma_commit(pbar(Cfg::kBarSFull + (j & 1)));
-          mma_commit(pbar(Cfg::kBarKFree + st));
+            for (int part = 1; part >= 0; --part)
+#pragma unroll
+              for (int kk = 0; kk < D / 16; ++kk)
+                mma_ts(to, tmem + kQCol + part_col(kk, part), k + static_cast<uint64_t>(2 * kk), kIdS, 1);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+#pragma unroll
+              for (int kk = 0; kk < D / 16; ++kk)
+                mma_ts(to, tmem + kQCol + part_col(kk, product(i).a),
+                       k + static_cast<uint64_t>(product(i).b * (kTileBytes >> 4) + 2 * kk), kIdS, i > 0 || kk > 0);
+          }
+          mma_commit(bar(Cfg::kBarSFull + (j & 1)));
+          mma_commit(bar(Cfg::kBarKFree + st));
         }
         __syncwarp();
         return true;
@@ -547,18 +692,20 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
       bool ok = wait(Cfg::kBarQFull, 0) && scores(0) && (n_tiles < 2 || scores(1));
       for (int j = 0; ok && j < n_tiles; ++j) {
         const int st = j % kStages;
-        if (!(ok = wait(Cfg::kBarPFull, j & 1)) || !(ok = wait(Cfg::kBarVFull + st, (j / kStages) & 1))) break;
+        if (!(ok = wait(Cfg::kBarPFull, j & 1) && (BF16 || wait(Cfg::kBarVFull + st, (j / kStages) & 1)))) break;
         fence_after();
         if (one) {
           const uint64_t v = v_desc + static_cast<uint64_t>(st * (kStageBytes >> 4));
 #pragma unroll
-          for (int i = 0; i < kProducts; ++i)
+          for (int i = BF16 ? 1 : 0; i < 3; ++i)  // (bf16 values have one part: lo and hi of P)
 #pragma unroll
             for (int ks = 0; ks < kTokens / 16; ++ks)
-              mma_ts(tmem + kOCol, tmem + (j & 1) * kBufCols + part_col(ks, product<BF16>(i).a),
-                     v + static_cast<uint64_t>(product<BF16>(i).b * (kTileBytes >> 4) + 128 * ks), kIdO, i > 0 || ks > 0);
-          mma_commit(pbar(Cfg::kBarODone));
-          mma_commit(pbar(Cfg::kBarVFree + st));
+              mma_ts(tmem + kOCol,
+                     tmem + kBufCol + (j & 1) * kBufCols + part_col(ks, BF16 ? 2 - i : product(i).a),
+                     v + static_cast<uint64_t>((BF16 ? 0 : product(i).b) * (kTileBytes >> 4) + 128 * ks), kIdO,
+                     i > (BF16 ? 1 : 0) || ks > 0);
+          mma_commit(bar(Cfg::kBarODone));
+          mma_commit(bar(Cfg::kBarVFree + st));
         }
         __syncwarp();
         // the next scores of this buffer take the place of the P just read
@@ -566,8 +713,8 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
       }
       if (!ok) raise();
       // every product completes before TMEM is released
-      if (lane == 0) mma_commit(pbar(Cfg::kBarDrain));
-      bar_wait(pbar(Cfg::kBarDrain), 0, 0);
+      if (lane == 0) mma_commit(bar(Cfg::kBarDrain));
+      bar_wait(bar(Cfg::kBarDrain), 0, 0);
       __syncwarp();
     }
   }

@@ -349,3 +349,94 @@ def test_a_rolled_back_step_and_the_next_on_another_stream():
     ref, tol = f.reference(0, *rows)
     for out in outs:
         assert (out.double() - ref).abs().max().item() <= tol
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("hq,hkv", [(8, 1), (8, 2), (4, 2)])
+@pytest.mark.parametrize("prefix", [1040, 1504])
+def test_runs_on_the_tensor_cores(hq, hkv, prefix, dtype):
+    """Enough rows and shared blocks for the 128-row tiles, whose last tile ends
+    inside; drafts, so that rows end in a last row tile too."""
+    n = 40
+    Forest(hq, hkv, [path((1, prefix), (70 * i, 1 + i % 7)) for i in range(2, 2 + n)], [1 + i % 4 for i in range(n)],
+           dtype, seed=prefix).check()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_magnitudes_on_the_tensor_cores(dtype):
+    """Blocks and rows of very different sizes: values from 1e-12 to 1e12 with
+    a block of zeros, keys and queries whose product stays of order one."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    n, prefix, hq, hkv = 48, 1024, 8, 2
+    f = Forest(hq, hkv, [path((1, prefix), (70 * i, 3)) for i in range(2, 2 + n)], [1] * n, dtype, seed=21)
+    key, value = f.pool.storage()
+    ids = torch.tensor(f.caches[0].blocks()[:prefix // 16], device="cuda", dtype=torch.long)
+    for scale_k, size_v in ((1e-20, 1e12), (1e20, 1e-12), (1.0, 1.0)):
+        k = torch.randn((prefix // 16, hkv, 16, D), generator=g, device="cuda") * scale_k
+        v = torch.randn((prefix // 16, hkv, 16, D), generator=g, device="cuda") * size_v
+        v[5:9] *= 1e-3
+        v[9] = 0
+        key[0, ids], value[0, ids] = k.to(key.dtype), v.to(value.dtype)
+        k, v = key[0, ids].transpose(1, 2).reshape(prefix, hkv, D), value[0, ids].transpose(1, 2).reshape(prefix, hkv, D)
+        for i in range(prefix):
+            f.kv[(0, tuple(f.paths[0][:i + 1]))] = (k[i].float(), v[i].float())
+        q, nk, nv = f.new_rows()
+        q, nk, nv = q / scale_k, nk * scale_k, nv * size_v
+        for p in f.paths:  # the few own cached tokens are zeros
+            for j in range(prefix, len(p)):
+                f.kv[(0, tuple(p[:j + 1]))] = (torch.zeros((hkv, D), device="cuda"),) * 2
+        for i, c in enumerate(f.caches):
+            last = c.blocks()[prefix // 16]
+            key[0, last], value[0, last] = 0, 0
+        with f.pool.begin(f.caches, f.counts) as b:
+            out = f.attend(b, 0, (q, nk, nv))
+        ref, tol = f.reference(0, q, nk, nv)
+        assert (out.double() - ref).abs().max().item() <= tol, (scale_k, size_v)
+        f.pool.truncate_many(f.caches, [prefix + 3] * n)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_scores_far_from_zero_on_the_tensor_cores(dtype):
+    """Scores of 2^30 and beyond, ties among them: one key for all tokens of the
+    prefix, zeros for the others, so that every row is the mean of the one's or
+    of the others' values."""
+    n, prefix, hq, hkv = 48, 1024, 8, 2
+    f = Forest(hq, hkv, [path((1, prefix), (70 * i, 3)) for i in range(2, 2 + n)], [1] * n, dtype, seed=22)
+    key, _ = f.pool.storage()
+    shared = torch.tensor(f.caches[0].blocks()[:prefix // 16], device="cuda", dtype=torch.long)
+    for at in (2.0**15, -(2.0**15), 2.0**40, -(2.0**40)):
+        key[0] = 0
+        key[0, shared] = at
+        for x in f.kv:
+            f.kv[x] = (torch.full((hkv, D), at if len(x[1]) <= prefix else 0.0, device="cuda"), f.kv[x][1])
+        q, nk, nv = f.new_rows()
+        q, nk = torch.full_like(q, 2.0**14), torch.zeros_like(nk)
+        with f.pool.begin(f.caches, f.counts) as b:
+            out = f.attend(b, 0, (q, nk, nv))
+        ref, _ = f.reference(0, q, nk, nv)
+        # equal scores are equal whatever they are: a mean, of weights of one
+        # size. At most 12 sums cut at 2^-23 a tile of 64, values in parts to
+        # 2^-22, 16 tiles and their joins each rounded at 2^-24.
+        vmax = max(x.abs().max().item() for _, x in f.kv.values())
+        assert (out.double() - ref).abs().max().item() <= 32 * 2.0**-22 * max(vmax, nv.abs().max().item()), at
+        f.pool.truncate_many(f.caches, [prefix + 3] * n)
+
+
+def test_a_score_past_f32_fails_its_sequence_on_the_tensor_cores():
+    n, prefix, hq, hkv = 48, 1024, 8, 2
+    f = Forest(hq, hkv, [path((1, prefix), (70 * i, 3)) for i in range(2, 2 + n)], [1] * n, "f32", seed=23)
+    key, _ = f.pool.storage()
+    ids = f.caches[0].blocks()[:prefix // 16]
+    key[0, ids[20], :, 3, 7] = 1e30
+    q, nk, nv = f.new_rows()
+    q[:, :, 7] = 0.5
+    q[4, 2, 7] = 1e20
+    q[9, 5, 1] = math.inf
+    b = f.pool.begin(f.caches, f.counts)
+    out = f.attend(b, 0, (q, nk, nv))
+    status = b.end(raise_on_error=False)
+    assert [i for i, s in enumerate(status) if s] == [4, 9]
+    assert set(status) == {0, slmkv.ERR_NON_FINITE}
+    good = [i for i in range(n) if i not in (4, 9)]
+    assert torch.isfinite(out[good]).all()
