@@ -257,12 +257,12 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyL
   const int first_tile = rank * per, n_tiles = max(0, min(tiles, first_tile + per) - first_tile);
   bool rest = a < k;  // the residual; the row itself when nothing of it is left
   auto usable = [](float w) { return w >= 0.f && w <= FLT_MAX; };
-  auto weight = [&](float pv, float qv, int x) -> double {
-    if (!rest) return pv;
-    if (!qr) return x == skip ? 0.0 : pv;
-    return fmax(static_cast<double>(pv) - static_cast<double>(qv), 0.0);
+  // of token x; q is zero where there is none
+  auto weight = [&](float pv, float qv, int x) {
+    return fmax(static_cast<double>(rest && x == skip ? 0.f : pv) - static_cast<double>(qv), 0.0);
   };
-  double total = 0.0, run_sum = 0.0, run_upto = 0.0;  // runs: of warp 0's lanes
+  double total = 0.0, part = 0.0, upto_part = 0.0;  // parts: of the row's CTAs
+  double run_sum = 0.0, run_upto = 0.0;             // runs: of warp 0's lanes
   int flags = 0, round = 0;
   const int run = (n_tiles + 31) >> 5;  // tiles of a lane
   for (; round < 2; ++round) {
@@ -275,23 +275,41 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyL
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int tt = t + n * (kVerifyThreads / 32), x = (first_tile + tt) * kTile + 32 * e + lane;
-          const bool in = tt < n_tiles && x < V;
-          pv[n][e] = in ? pr[x] : 0.f;
-          qv[n][e] = in && qr && rest ? qr[x] : 0.f;
+          pv[n][e] = tt < n_tiles && x < V ? pr[x] : 0.f;
+          qv[n][e] = 0.f;
         }
+      if (qr && rest) {
+#pragma unroll
+        for (int n = 0; n < kUnroll; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int tt = t + n * (kVerifyThreads / 32), x = (first_tile + tt) * kTile + 32 * e + lane;
+            if (tt < n_tiles && x < V) qv[n][e] = qr[x];
+          }
+      }
+      double sum[kUnroll];
 #pragma unroll
       for (int n = 0; n < kUnroll; ++n) {
-        const int tt = t + n * (kVerifyThreads / 32);
-        double s = 0.0;
+        double w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           bad |= !usable(pv[n][e]) | !usable(qv[n][e]);
-          s += weight(pv[n][e], qv[n][e], (first_tile + tt) * kTile + 32 * e + lane);
+          w[e] = weight(pv[n][e], qv[n][e],
+                        (first_tile + t + n * (kVerifyThreads / 32)) * kTile + 32 * e + lane);
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kFullMask, s, o);
-        if (lane == 0 && tt < n_tiles) tile_sum[tt] = s;
+        sum[n] = (w[0] + w[1]) + (w[2] + w[3]);
       }
+      // across the warp, the four tiles at once: at the first two steps a lane keeps
+      // half of its tiles and gives the others away
+      static_assert(kUnroll == 4, "two halvings");
+      const bool h16 = lane & 16, h8 = lane & 8;
+      const double x0 = (h16 ? sum[2] : sum[0]) + __shfl_xor_sync(kFullMask, h16 ? sum[0] : sum[2], 16);
+      const double x1 = (h16 ? sum[3] : sum[1]) + __shfl_xor_sync(kFullMask, h16 ? sum[1] : sum[3], 16);
+      double y = (h8 ? x1 : x0) + __shfl_xor_sync(kFullMask, h8 ? x0 : x1, 8);
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) y += __shfl_xor_sync(kFullMask, y, o);
+      const int mine = t + (lane >> 3) * (kVerifyThreads / 32);
+      if ((lane & 7) == 0 && mine < n_tiles) tile_sum[mine] = y;
     }
     if (bad) atomicOr(&s_flags, kStatusProbability);
     if (ctas > 1 && round == 0) cluster_wait();
@@ -317,12 +335,16 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyL
     } else {
       __syncthreads();
     }
-    total = 0.0;
-    flags = 0;
-    for (int r = 0; r < ctas; ++r) {
-      total += slices[round][r].total;
-      flags |= slices[round][r].flags;
+    // lanes 0 .. 7: the CTAs' totals, summed up to theirs (the same in every warp)
+    const VerifySlice mine = lane < ctas ? slices[round][lane] : VerifySlice{0.0, 0, 0};
+    part = upto_part = mine.total;
+#pragma unroll
+    for (int o = 1; o < kMaxCluster; o <<= 1) {
+      const double up = __shfl_up_sync(kFullMask, upto_part, o);
+      if (lane >= o) upto_part += up;
     }
+    total = __shfl_sync(kFullMask, upto_part, kMaxCluster - 1);
+    flags = static_cast<int>(__reduce_or_sync(kFullMask, static_cast<unsigned>(mine.flags)));
     if (flags || total > 0.0 || !rest) break;  // the same in every CTA of the row
     rest = false;
   }
@@ -339,22 +361,15 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyL
   // does (u is 1 or more) the last with a weight. The same rule then finds the
   // lane's run of tiles, the tile and the value.
   const double point = u * total;
-  double before = 0.0, upto = 0.0;
-  int owner = 0;
-  for (int r = 0; r < ctas; ++r) {
-    const double w = slices[round][r].total;
-    if (w > 0.0) {
-      owner = r;
-      before = upto;
-      if (upto + w > point) break;
-    }
-    upto += w;
-  }
+  unsigned over = __ballot_sync(kFullMask, part > 0.0 && upto_part > point);
+  unsigned live = __ballot_sync(kFullMask, part > 0.0);
+  const int owner = over ? __ffs(over) - 1 : 31 - __clz(live);
+  double before = __shfl_sync(kFullMask, upto_part - part, owner);
   if (rank != owner) return;
-  unsigned over = __ballot_sync(kFullMask, run_sum > 0.0 && before + run_upto > point);
-  unsigned live = __ballot_sync(kFullMask, run_sum > 0.0);
+  over = __ballot_sync(kFullMask, run_sum > 0.0 && before + run_upto > point);
+  live = __ballot_sync(kFullMask, run_sum > 0.0);
   const int src = over ? __ffs(over) - 1 : 31 - __clz(live);
-  upto = before + __shfl_sync(kFullMask, run_upto - run_sum, src);
+  double upto = before + __shfl_sync(kFullMask, run_upto - run_sum, src);
   int tile = src * run;
   for (int t = src * run; t < min(n_tiles, (src + 1) * run); ++t) {
     const double w = tile_sum[t];
