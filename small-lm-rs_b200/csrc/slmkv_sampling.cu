@@ -1,6 +1,7 @@
 // Token probabilities of logit rows, and the verification of drafted tokens
 // against them. Both spread a row over a thread-block cluster and read it once.
 #include <cfloat>
+#include <type_traits>
 
 #include "slmkv_device.h"
 
@@ -68,6 +69,12 @@ struct ProbSlice {  // exchanged between the CTAs of a row
 };
 static_assert(sizeof(ProbSlice) == 16, "written as one uint4");
 
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // KEEP: the slice stays in shared memory; otherwise it is read again.
 template <bool KEEP>
 __global__ void __launch_bounds__(kProbThreads, 4) probabilities_kernel(const ProbabilitiesLaunch p) {
@@ -84,74 +91,92 @@ __global__ void __launch_bounds__(kProbThreads, 4) probabilities_kernel(const Pr
   const int n_lines = (V + shift + 3) >> 2, per = (n_lines + ctas - 1) / ctas;
   const int begin = rank * per, end = min(n_lines, begin + per);
 
-  auto inside = [&](int e) { return e >= 0 && e + 4 <= V; };
-  auto edge = [&](int e) {  // a line of which some values lie outside the row: -inf there
+  // Whole lines, in a loop that checks nothing, and the first and last ones that
+  // are not: f(line, whole). A thread meets the same lines every time.
+  const int whole0 = max(begin, shift ? 1 : 0), whole1 = min(end, (V + shift) >> 2), last = n_lines - 1;
+  auto for_lines = [&](auto f) {
+#pragma unroll 4
+    for (int i = whole0 + static_cast<int>(threadIdx.x); i < whole1; i += kProbThreads) f(i, std::true_type{});
+    if (threadIdx.x == 0 && shift && begin == 0 && end > 0) f(0, std::false_type{});
+    if (threadIdx.x == 32 && ((V + shift) & 3) && last >= (shift ? 1 : 0) && begin <= last && last < end)
+      f(last, std::false_type{});
+  };
+  auto edge = [&](int i) {  // -inf outside the row
+    const int e = 4 * i - shift;
     return make_float4(e >= 0 ? x[e] : -INFINITY, e + 1 >= 0 && e + 1 < V ? x[e + 1] : -INFINITY,
                        e + 2 >= 0 && e + 2 < V ? x[e + 2] : -INFINITY,
                        e + 3 >= 0 && e + 3 < V ? x[e + 3] : -INFINITY);
   };
+  const float4* x4 = reinterpret_cast<const float4*>(x - shift);
+  float4* y4 = reinterpret_cast<float4*>(y - shift);  // (whole lines of y where `lines` holds)
   if constexpr (KEEP) {
-    for (int i = begin + threadIdx.x; i < end; i += kProbThreads) {
-      const int e = 4 * i - shift;
-      if (inside(e))
+    for_lines([&](int i, auto whole) {
+      if constexpr (decltype(whole)::value)
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
                          static_cast<uint32_t>(__cvta_generic_to_shared(kept + (i - begin)))),
-                     "l"(x + e)
+                     "l"(x4 + i)
                      : "memory");
       else
-        kept[i - begin] = edge(e);
-    }
+        kept[i - begin] = edge(i);
+    });
     asm volatile("cp.async.wait_all;" ::: "memory");
   }
-  auto load = [&](int i) -> float4 {
+  auto load = [&](int i, auto whole) -> float4 {
     if constexpr (KEEP) return kept[i - begin];
-    const int e = 4 * i - shift;
-    return inside(e) ? *reinterpret_cast<const float4*>(x + e) : edge(e);
+    else if constexpr (decltype(whole)::value) return x4[i];
+    else return edge(i);
   };
-  auto store = [&](int i, float4 v) {
-    const int e = 4 * i - shift;
-    if (lines && inside(e)) {
-      *reinterpret_cast<float4*>(y + e) = v;
+  auto store = [&](int i, auto whole, float4 v) {
+    if (decltype(whole)::value && lines) {
+      y4[i] = v;
       return;
     }
+    const int e = 4 * i - shift;
     if (e >= 0) y[e] = v.x;
     if (e + 1 >= 0 && e + 1 < V) y[e + 1] = v.y;
     if (e + 2 >= 0 && e + 2 < V) y[e + 2] = v.z;
     if (e + 3 >= 0 && e + 3 < V) y[e + 3] = v.w;
   };
   const float t = p.temperatures ? p.temperatures[row] : 1.f;
-  int bad = !(t >= 0.f && t <= FLT_MAX);
-  float m = -INFINITY;
-#pragma unroll 4
-  for (int i = begin + threadIdx.x; i < end; i += kProbThreads) {
-    const float4 a = load(i);
-    m = fmaxf(fmaxf(m, fmaxf(a.x, a.y)), fmaxf(a.z, a.w));
-    // not a number, or +inf
-    bad |= !(a.x <= FLT_MAX) | !(a.y <= FLT_MAX) | !(a.z <= FLT_MAX) | !(a.w <= FLT_MAX);
-  }
+  float m = -INFINITY;  // NaN once a value is not a number
+  for_lines([&](int i, auto whole) {
+    const float4 a = load(i, whole);
+    m = max3_nan(max3_nan(m, a.x, a.y), a.z, a.w);
+  });
+  int bad = !(t >= 0.f && t <= FLT_MAX) | !(m <= FLT_MAX);  // or a value is +inf
   m = block_reduce<float, kProbThreads>(m, red_max, [](float a, float b) { return fmaxf(a, b); });
   const float base = m == -INFINITY ? 0.f : m;
   // the least T whose reciprocal is in range keeps 0 * c = 0 at the maximum
   const float c = t > 0.f ? fminf(kLog2e / t, FLT_MAX) : 0.f;
+  const uint64_t base2 = pack2(-base, -base), c2 = pack2(c, c);
+  struct Line {
+    uint64_t xy, zw;
+  };
   auto power = [&](const float4& a) {
-    return make_float4(exp2_fast((a.x - base) * c), exp2_fast((a.y - base) * c), exp2_fast((a.z - base) * c),
-                       exp2_fast((a.w - base) * c));
+    float x0, x1, x2, x3;
+    unpack2(mul2(add2(pack2(a.x, a.y), base2), c2), x0, x1);
+    unpack2(mul2(add2(pack2(a.z, a.w), base2), c2), x2, x3);
+    return Line{pack2(exp2_fast(x0), exp2_fast(x1)), pack2(exp2_fast(x2), exp2_fast(x3))};
   };
   float sum = 0.f;
   int first = INT32_MAX;
   if (t > 0.f) {
-#pragma unroll 4
-    for (int i = begin + threadIdx.x; i < end; i += kProbThreads) {
-      const float4 a = power(load(i));
-      if constexpr (KEEP) kept[i - begin] = a;
-      sum += (a.x + a.y) + (a.z + a.w);
-    }
+    uint64_t sums[2] = {0ull, 0ull};
+    for_lines([&](int i, auto whole) {
+      const Line a = power(load(i, whole));
+      if constexpr (KEEP) reinterpret_cast<Line*>(kept)[i - begin] = a;
+      sums[0] = add2(sums[0], a.xy);
+      sums[1] = add2(sums[1], a.zw);
+    });
+    float s0, s1;
+    unpack2(add2(sums[0], sums[1]), s0, s1);
+    sum = s0 + s1;
   } else {
-    for (int i = begin + threadIdx.x; i < end; i += kProbThreads) {
-      const float4 a = load(i);
+    for_lines([&](int i, auto whole) {
+      const float4 a = load(i, whole);
       const int at = a.x == m ? 0 : a.y == m ? 1 : a.z == m ? 2 : a.w == m ? 3 : -1;
       if (at >= 0) first = min(first, 4 * i - shift + at);
-    }
+    });
     first = block_reduce<int, kProbThreads>(first, red_first, [](int a, int b) { return min(a, b); });
   }
   sum = block_reduce<float, kProbThreads>(sum, red_sum, [](float a, float b) { return a + b; });
@@ -179,21 +204,26 @@ __global__ void __launch_bounds__(kProbThreads, 4) probabilities_kernel(const Pr
     }
   }
   if (bad || top == -INFINITY) {
-    for (int i = begin + threadIdx.x; i < end; i += kProbThreads) store(i, make_float4(0.f, 0.f, 0.f, 0.f));
+    for_lines([&](int i, auto whole) { store(i, whole, make_float4(0.f, 0.f, 0.f, 0.f)); });
     if (rank == 0 && threadIdx.x == 0)
       atomicOr(&p.status[p.rows == p.n_seq ? row : find_sequence(p.seqs, p.n_seq, row)], kStatusLogits);
   } else if (t == 0.f) {
-    for (int i = begin + threadIdx.x; i < end; i += kProbThreads) {
+    for_lines([&](int i, auto whole) {
       const int e = 4 * i - shift;
-      store(i, make_float4(e == first, e + 1 == first, e + 2 == first, e + 3 == first));
-    }
+      store(i, whole, make_float4(e == first, e + 1 == first, e + 2 == first, e + 3 == first));
+    });
   } else {
     const float f = m == -INFINITY ? 0.f : exp2_fast((m - top) * c) / total;
-#pragma unroll 4
-    for (int i = begin + threadIdx.x; i < end; i += kProbThreads) {
-      const float4 a = KEEP ? load(i) : power(load(i));
-      store(i, make_float4(a.x * f, a.y * f, a.z * f, a.w * f));
-    }
+    const uint64_t f2 = pack2(f, f);
+    for_lines([&](int i, auto whole) {
+      Line a;
+      if constexpr (KEEP) a = reinterpret_cast<const Line*>(kept)[i - begin];
+      else a = power(load(i, whole));
+      float4 v;
+      unpack2(mul2(a.xy, f2), v.x, v.y);
+      unpack2(mul2(a.zw, f2), v.z, v.w);
+      store(i, whole, v);
+    });
   }
 }
 

@@ -211,11 +211,6 @@ __device__ __forceinline__ uint32_t swizzled(int r, int u) {
 // TMEM column of part q (0: hi) of the 16 inner values ks of Q or P: P's take the
 // place of the scores, which are all in registers by then.
 __device__ __forceinline__ constexpr int part_col(int ks, int q) { return 16 * ks + 8 * q; }
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 // An f32 pair as two f16 pairs, to 2^-22 of each value in f16's normal range.
 struct Halves {
   uint32_t hi, lo;
