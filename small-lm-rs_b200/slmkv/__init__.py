@@ -686,8 +686,16 @@ class Batch:
                 and t.get_device() == self.pool.device:
             if t.is_contiguous():
                 return t.data_ptr()
-            if rows and t[0].is_contiguous() and t.stride(0) >= t[0].numel():
-                return t.data_ptr()
+            if rows:
+                apart, *inner = t.stride()
+                width = 1  # of a dense row's dimensions so far
+                for size, stride in zip(reversed(shape[1:]), reversed(inner)):
+                    if size != 1 and stride != width:
+                        break
+                    width *= size
+                else:
+                    if apart >= width:
+                        return t.data_ptr()
         raise InvalidInput(ERR_INVALID_INPUT,
                            f"invalid input for slmkv: {what} must be a "
                            f"{'row-strided' if rows else 'contiguous'} {dtype or torch.float32} CUDA "
