@@ -486,14 +486,15 @@ __global__ void __launch_bounds__(kThreads, 3) shared_rows_kernel(const __grid_c
 }
 
 // Joins rows' parts: a CTA takes one token and 8 / W query heads, W warps a row
-// (the more parts a row has, the more), lane l holding values 2l, 2l + 1. The
-// parts of a row are those of the edges from its own up to the root. The plan is
-// read while the kernels before finish; what is left then is one round of reads
-// for a row of up to kBatch parts an edge.
+// (the more parts a row has, the more). The parts of a row are those of the edges
+// from its own up to the root; a warp takes 32 of them at a time, lane l the
+// maximum and sum of the l-th, and values 2l and 2l + 1 of all. The plan is read
+// while the kernels before finish; what is left then is one round of reads for up
+// to 8 W parts.
 constexpr int kMergeThreads = 256;
 constexpr int kMergeDepth = 4;  // edges whose units are read ahead
 template <int W>
-__global__ void __launch_bounds__(kMergeThreads, 4) shared_merge_kernel(const SharedAttentionLaunch p) {
+__global__ void __launch_bounds__(kMergeThreads, 5) shared_merge_kernel(const SharedAttentionLaunch p) {
   __shared__ float2 s_ml[8];
   __shared__ float2 s_acc[8][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, share = warp % W;
@@ -502,69 +503,70 @@ __global__ void __launch_bounds__(kMergeThreads, 4) shared_merge_kernel(const Sh
   const bool live = hq < Hq;
   const int head = min(hq, Hq - 1) / G, gq = min(hq, Hq - 1) % G;
   const SharedToken tk = p.tokens[k];
-  // parts of the row on one edge: the first slot, their number and their distance
-  struct Run {
-    size_t slot0;
-    int n_parts, n_rows;
-  };
-  auto run_of = [&](int e, int& parent) {
-    const SharedEdge ed = p.edges[e];
-    parent = ed.parent;
-    const int tile = (k - ed.token0) / ed.tile_tokens;
-    const SharedUnit u = p.units[ed.unit0 + head * ed.n_tiles + tile];
-    return Run{static_cast<size_t>(u.part0) + (k - ed.token0 - tile * ed.tile_tokens) * G + gq, u.n_parts, u.n_rows};
-  };
-  Run runs[kMergeDepth];
-  int e = tk.edge, depth = 0;
-#pragma unroll
-  for (int d = 0; d < kMergeDepth; ++d) {
-    if (e < 0) break;
-    int parent;
-    runs[d] = run_of(e, parent);
-    e = parent;
-    depth = d + 1;
-  }
-  wait_for_previous();
   float m = -INFINITY, l = 0.f;
   float2 a = make_float2(0.f, 0.f);
-  bool any = false;
-  auto add = [&](const Run& u) {
-    any = any || u.n_parts > 0;
-    constexpr int kBatch = 8;  // parts in flight
-    for (int s = share; s < u.n_parts; s += W * kBatch) {
-      float2 ml[kBatch], v[kBatch];
+  bool any = false, first = true;
+  for (int e = tk.edge; e >= 0; first = false) {
+    // parts of the row on the next edges: first slot, number, distance
+    uint32_t slot0[kMergeDepth];
+    int n_parts[kMergeDepth], n_rows[kMergeDepth], total = 0;
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const bool in = s + i * W < u.n_parts;
-        const size_t slot = u.slot0 + static_cast<size_t>(in ? s + i * W : s) * u.n_rows;
-        ml[i] = in ? p.part_ml[slot] : make_float2(-INFINITY, 0.f);
-        v[i] = in ? reinterpret_cast<const float2*>(p.part_acc + slot * D)[lane] : make_float2(0.f, 0.f);
+    for (int d = 0; d < kMergeDepth; ++d) {
+      n_parts[d] = 0;
+      if (e < 0) continue;
+      const SharedEdge ed = p.edges[e];
+      const int tile = (k - ed.token0) / ed.tile_tokens;
+      const SharedUnit u = p.units[ed.unit0 + head * ed.n_tiles + tile];
+      slot0[d] = static_cast<uint32_t>(u.part0 + (k - ed.token0 - tile * ed.tile_tokens) * G + gq);
+      n_parts[d] = u.n_parts;
+      n_rows[d] = u.n_rows;
+      total += u.n_parts;
+      e = ed.parent;
+    }
+    if (first) wait_for_previous();
+    any = any || total > 0;
+    for (int at = share; at < total; at += 32 * W) {
+      int i = at + lane * W;
+      const bool in = i < total;
+      uint32_t slot = 0;
+#pragma unroll
+      for (int d = 0; d < kMergeDepth; ++d) {
+        if (i >= 0 && i < n_parts[d]) slot = slot0[d] + static_cast<uint32_t>(i) * n_rows[d];
+        i -= n_parts[d];
       }
-      float mx = m;
+      const float2 ml = in ? p.part_ml[slot] : make_float2(-INFINITY, 0.f);
+      const int count = min(32, (total - at + W - 1) / W);
+      constexpr int kBatch = 8;  // parts in flight
+      float2 v[kBatch];
+      auto load = [&](int s0) {
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) mx = fmaxf(mx, ml[i].x);
-      const float base = mx == -INFINITY ? 0.f : mx, w0 = exp2_fast(m - base);
+        for (int n = 0; n < kBatch; ++n) {
+          const size_t part = __shfl_sync(kFullMask, slot, (s0 + n) & 31);
+          v[n] = s0 + n < count ? reinterpret_cast<const float2*>(p.part_acc + part * D)[lane] : make_float2(0.f, 0.f);
+        }
+      };
+      load(0);
+      float mx = fmaxf(m, ml.x);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(kFullMask, mx, o));
+      const float base = mx == -INFINITY ? 0.f : mx, w0 = exp2_fast(m - base), w = exp2_fast(ml.x - base);
+      float sum = ml.y * w;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
       m = mx;
-      l *= w0;
+      l = fmaf(l, w0, sum);
       a.x *= w0;
       a.y *= w0;
+      for (int s0 = 0; s0 < count; s0 += kBatch) {
+        if (s0) load(s0);
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const float w = exp2_fast(ml[i].x - base);
-        l = fmaf(ml[i].y, w, l);
-        a.x = fmaf(v[i].x, w, a.x);
-        a.y = fmaf(v[i].y, w, a.y);
+        for (int n = 0; n < kBatch; ++n) {
+          const float wn = __shfl_sync(kFullMask, w, (s0 + n) & 31);
+          a.x = fmaf(v[n].x, wn, a.x);
+          a.y = fmaf(v[n].y, wn, a.y);
+        }
       }
     }
-  };
-#pragma unroll
-  for (int d = 0; d < kMergeDepth; ++d)
-    if (d < depth) add(runs[d]);
-  while (e >= 0) {  // deeper trees
-    int parent;
-    const Run u = run_of(e, parent);
-    e = parent;
-    add(u);
   }
   if constexpr (W > 1) {
     if (lane == 0) s_ml[warp] = make_float2(m, l);
@@ -630,6 +632,8 @@ cudaError_t launch_shared_attention(const SharedAttentionLaunch& p, cudaStream_t
       };
       all_shared(kernel);
       all_shared(shared_merge_kernel<1>);
+      all_shared(shared_merge_kernel<2>);
+      all_shared(shared_merge_kernel<4>);
       all_shared(shared_merge_kernel<8>);
       if (a != cudaSuccess) return a;
       if (dev < 64) configured[v] |= 1ull << dev;
@@ -652,11 +656,18 @@ cudaError_t launch_shared_attention(const SharedAttentionLaunch& p, cudaStream_t
   };
   e = p.g.bf16 ? of_group(std::integral_constant<int, 1>{}, 4) : of_group(std::integral_constant<int, 0>{}, 0);
   if (e != cudaSuccess || p.n_merge == 0) return e;
-  // a warp a row while rows fill the SMs or have few parts
+  // more warps a row while the SMs hold them all at once and there are parts for
+  // them
   const int64_t rows = static_cast<int64_t>(p.n_merge) * p.g.q_heads;
-  if (p.most_parts > 16 && rows * 8 <= 148 * 64)
-    return launch(shared_merge_kernel<8>, dim3(p.n_merge, p.g.q_heads), kMergeThreads, 0, true, p, s);
-  return launch(shared_merge_kernel<1>, dim3(p.n_merge, (p.g.q_heads + 7) / 8), kMergeThreads, 0, true, p, s);
+  int w = 1;
+  while (w < 8 && rows * w * 2 <= 148 * 40 && p.most_parts > 8 * w) w *= 2;
+  const dim3 grid(p.n_merge, (p.g.q_heads * w + 7) / 8);
+  switch (w) {
+    case 1: return launch(shared_merge_kernel<1>, grid, kMergeThreads, 0, true, p, s);
+    case 2: return launch(shared_merge_kernel<2>, grid, kMergeThreads, 0, true, p, s);
+    case 4: return launch(shared_merge_kernel<4>, grid, kMergeThreads, 0, true, p, s);
+    default: return launch(shared_merge_kernel<8>, grid, kMergeThreads, 0, true, p, s);
+  }
 }
 
 }  // namespace slmkv
