@@ -1805,12 +1805,19 @@ slm_status slm_batch_append_layer_normed(slm_batch* b, int32_t layer, const floa
 }
 
 namespace {
-// A run of blocks that several sequences share becomes an edge of its own from
-// this many blocks on: a shorter one costs more in joining than it saves.
-constexpr int32_t kSharedMinBlocks = 4;
+// A run of blocks that n sequences share becomes an edge of its own where that
+// saves each of them, on average, this many blocks: joining costs about as much.
+// Groups of 8 with 40 tokens of their own, shared and not: 8 blocks 10.3 and 6.7
+// us, 12 blocks 10.3 and 8.2, 16 blocks alike; 200 sequences, bf16: 22.5 and 18.5
+// at 12 blocks, alike at 16.
+constexpr int32_t kSharedMinSaved = 12;
 // Rows (tokens x query heads of a KV head) from which a shared run goes to the
-// tensor cores' 128-row tiles.
-constexpr int32_t kSharedTcMinRows = 48;
+// tensor cores' 128-row tiles: a tile costs the same for any number, and about as
+// much as eight rows do on the other kernel (16 rows over 16384 tokens of 8 heads
+// 23 against 33 us, 32 rows 24 against 37; 8 rows 22 against 25). A tile's start
+// there needs rows x blocks to pay: 25 groups of 32 rows over 16 blocks 28.7
+// against 26.6 us without, over 64 blocks 41 against 45.
+constexpr int32_t kSharedTcMinRows = 16, kSharedTcMinRowBlocks = 2048;
 // And only where a batch has enough such work, as eight-row units x blocks for
 // each warp of the other kernel: below, a launch more costs more than it saves.
 // Batches of 16 and 64 over 64 to 4096 shared tokens, with and without: at 0.6 a
@@ -1845,7 +1852,7 @@ void shared_tree(const slm_ctx* c, const slm_batch* b, SharedPlan& plan, int32_t
         while (j < n && x[j] == y[j]) ++j;
         same = j;
       }
-      if (same - start >= kSharedMinBlocks) {
+      if (static_cast<int64_t>(same - start) * (end - at - 1) >= static_cast<int64_t>(kSharedMinSaved) * (end - at)) {
         plan.tree.push_back({parent, start, same, at, end});
         shared_tree(c, b, plan, static_cast<int32_t>(plan.tree.size()) - 1, at, end, same, same);
       } else {
@@ -1887,7 +1894,8 @@ void build_shared_plan(const slm_ctx* c, const slm_batch* b, SharedPlan& plan) {
     const auto& e = plan.tree[i];
     const int32_t rows = (plan.token0[e.seq1] - plan.token0[e.seq0]) * G;
     const int32_t nb = e.last_block - e.first_block;
-    plan.on_tc[i] = e.seq1 - e.seq0 > 1 && rows >= kSharedTcMinRows && nb >= 2 * kSharedTcBlocks;
+    plan.on_tc[i] = e.seq1 - e.seq0 > 1 && rows >= kSharedTcMinRows && nb >= 2 * kSharedTcBlocks &&
+                    static_cast<int64_t>(rows) * nb >= kSharedTcMinRowBlocks;
     if (plan.on_tc[i]) shared_work += static_cast<int64_t>((rows + kSharedRows - 1) / kSharedRows) * Hkv * nb;
   }
   const int64_t ctas = static_cast<int64_t>(kSharedCtasPerSm) * c->num_sms;
