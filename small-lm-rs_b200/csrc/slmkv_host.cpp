@@ -94,11 +94,13 @@ struct SharedPlan {
   struct Edge {
     int32_t parent, first_block, last_block;  // blocks [first, last)
     int32_t seq0, seq1;                       // members order[seq0 .. seq1)
+    bool leaf;                                // one sequence's, up to its new tokens
   };
   std::vector<int32_t> order;  // batch rows, members of an edge next to each other
   std::vector<Edge> tree;
   std::vector<int32_t> token0;  // first token of order[i]
   std::vector<uint8_t> on_tc;   // per edge
+  bool split = false;           // long caches of one sequence are edges of their own
   std::vector<SharedItem> items, tc_items;
   std::vector<int32_t> list_start;  // first item of a warp's or team's list, and the end
   std::vector<SharedToken> tokens;
@@ -1825,6 +1827,18 @@ constexpr int32_t kSharedTcMinRows = 16, kSharedTcMinRowBlocks = 2048;
 // at 4.6 16.4 and 27.0, at 37 28.7 and 43.0.
 constexpr int32_t kSharedTcMinWork = 2;
 
+bool runs_on_tc(int32_t rows, int32_t blocks) {
+  return rows >= kSharedTcMinRows && blocks >= 2 * kSharedTcBlocks &&
+         static_cast<int64_t>(rows) * blocks >= kSharedTcMinRowBlocks;
+}
+// One sequence's cache, read for its new tokens' rows: cutting it off for the
+// tensor cores adds parts that a shared run has anyway (8 requests with 6 drafts,
+// f32: over 2000 tokens 20.5 us cut and 16.4 not, over 8000 26.7 and 48.7).
+bool cut_pays(int32_t rows, int32_t blocks) {
+  return runs_on_tc(rows, blocks) && static_cast<int64_t>(rows) * blocks >= 2 * kSharedTcMinRowBlocks;
+}
+int64_t units_of_eight(int32_t rows) { return (rows + kSharedRows - 1) / kSharedRows; }
+
 // The tree below the members order[lo, hi), which share their blocks before
 // `start` (edge `parent` ends there) and, beyond it, those before `probe`.
 void shared_tree(const slm_ctx* c, const slm_batch* b, SharedPlan& plan, int32_t parent, int32_t lo,
@@ -1842,7 +1856,14 @@ void shared_tree(const slm_ctx* c, const slm_batch* b, SharedPlan& plan, int32_t
       while (end < hi && key(plan.order[end]) == block) ++end;
     if (end - at == 1) {  // the sequence's own run, to its last new token
       const int32_t stop = blocks_for(b->base[first] + b->counts[first]);
-      plan.tree.push_back({parent, start, stop, at, end});
+      int32_t above = parent, from = start;
+      if (plan.split && cut_pays(b->counts[first] * c->group, limit(first) - start)) {
+        // what all its new tokens see goes to the tensor cores
+        plan.tree.push_back({parent, start, limit(first), at, end, false});
+        above = static_cast<int32_t>(plan.tree.size()) - 1;
+        from = limit(first);
+      }
+      plan.tree.push_back({above, from, stop, at, end, true});
     } else {
       int32_t same = limit(first);
       for (int32_t i = at + 1; i < end; ++i) {
@@ -1853,7 +1874,7 @@ void shared_tree(const slm_ctx* c, const slm_batch* b, SharedPlan& plan, int32_t
         same = j;
       }
       if (static_cast<int64_t>(same - start) * (end - at - 1) >= static_cast<int64_t>(kSharedMinSaved) * (end - at)) {
-        plan.tree.push_back({parent, start, same, at, end});
+        plan.tree.push_back({parent, start, same, at, end, false});
         shared_tree(c, b, plan, static_cast<int32_t>(plan.tree.size()) - 1, at, end, same, same);
       } else {
         shared_tree(c, b, plan, parent, at, end, start, same);
@@ -1869,6 +1890,14 @@ void build_shared_plan(const slm_ctx* c, const slm_batch* b, SharedPlan& plan) {
   plan.order.resize(n);
   for (int32_t i = 0; i < n; ++i) plan.order[i] = i;
   plan.tree.clear();
+  const int64_t ctas = static_cast<int64_t>(kSharedCtasPerSm) * c->num_sms;
+  const int64_t tc_from = kSharedTcMinWork * 4 * ctas;
+  int64_t long_work = 0;
+  for (int32_t i = 0; i < n; ++i) {
+    const int32_t rows = b->counts[i] * G, nb = b->base[i] / kBlockTokens;
+    if (cut_pays(rows, nb)) long_work += units_of_eight(rows) * Hkv * nb;
+  }
+  plan.split = long_work >= tc_from;
   shared_tree(c, b, plan, -1, 0, n, 0, 0);
 
   const int32_t n_edges = static_cast<int32_t>(plan.tree.size());
@@ -1894,12 +1923,10 @@ void build_shared_plan(const slm_ctx* c, const slm_batch* b, SharedPlan& plan) {
     const auto& e = plan.tree[i];
     const int32_t rows = (plan.token0[e.seq1] - plan.token0[e.seq0]) * G;
     const int32_t nb = e.last_block - e.first_block;
-    plan.on_tc[i] = e.seq1 - e.seq0 > 1 && rows >= kSharedTcMinRows && nb >= 2 * kSharedTcBlocks &&
-                    static_cast<int64_t>(rows) * nb >= kSharedTcMinRowBlocks;
-    if (plan.on_tc[i]) shared_work += static_cast<int64_t>((rows + kSharedRows - 1) / kSharedRows) * Hkv * nb;
+    plan.on_tc[i] = !e.leaf && runs_on_tc(rows, nb);
+    if (plan.on_tc[i]) shared_work += units_of_eight(rows) * Hkv * nb;
   }
-  const int64_t ctas = static_cast<int64_t>(kSharedCtasPerSm) * c->num_sms;
-  if (shared_work < kSharedTcMinWork * 4 * ctas) plan.on_tc.assign(n_edges, 0);
+  if (shared_work < tc_from) plan.on_tc.assign(n_edges, 0);
   const int32_t tile = kSharedRows / G, tc_tile = kSharedTcRows / G;
   auto tiles_of = [&](int32_t i) {
     const auto& e = plan.tree[i];
@@ -1959,7 +1986,7 @@ void build_shared_plan(const slm_ctx* c, const slm_batch* b, SharedPlan& plan) {
   for (int32_t i = 0; i < n_edges; ++i) {
     const auto& e = plan.tree[i];
     const int32_t end = plan.token0[e.seq1], n_tiles = tiles_of(i);
-    const bool own = e.seq1 - e.seq0 == 1;
+    const bool own = e.leaf;
     SharedEdge& d = plan.edges[i];
     d.parent = e.parent;
     d.token0 = plan.token0[e.seq0];
@@ -2027,7 +2054,7 @@ void build_shared_plan(const slm_ctx* c, const slm_batch* b, SharedPlan& plan) {
   }
   plan.list_start.push_back(static_cast<int32_t>(plan.items.size()));
   for (int32_t i = 0; i < n_edges; ++i) {  // the most parts of a row, over its edges up to the root
-    if (plan.tree[i].seq1 - plan.tree[i].seq0 > 1) continue;
+    if (!plan.tree[i].leaf) continue;
     int32_t n_parts = 0;
     for (int32_t e = i; e >= 0; e = plan.tree[e].parent) n_parts += plan.units[plan.edges[e].unit0].n_parts;
     plan.most_parts = std::max(plan.most_parts, n_parts);

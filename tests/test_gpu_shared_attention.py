@@ -440,3 +440,20 @@ def test_a_score_past_f32_fails_its_sequence_on_the_tensor_cores():
     assert set(status) == {0, slmkv.ERR_NON_FINITE}
     good = [i for i in range(n) if i not in (4, 9)]
     assert torch.isfinite(out[good]).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("hq,hkv,lengths,counts", [
+    (8, 2, [12_005], [6]),                                             # one long cache, drafts
+    (8, 8, [0, 1600, 1601, 1615, 1616, 90], [17, 16, 16, 20, 33, 1]),  # one query head a key head; chunks
+    (16, 2, [2500, 2511, 2047, 31], [5, 8, 3, 8])])
+def test_long_caches_of_one_sequence(hq, hkv, lengths, counts, dtype):
+    """Nothing shared, but many new rows a sequence: its cache is read for all of
+    them, the rows' own blocks apart."""
+    Forest(hq, hkv, [path((1000 * i, n)) if n else [] for i, n in enumerate(lengths, 1)], counts, dtype, seed=len(lengths)).check()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_shared_and_long_runs_with_one_query_head(dtype):
+    paths = [path((1, 1600), (9000 * i, 1300 + 7 * i)) for i in range(1, 4)]
+    Forest(4, 4, paths, [40, 33, 1], dtype, seed=5).check()
