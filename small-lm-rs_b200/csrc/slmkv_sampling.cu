@@ -56,8 +56,12 @@ __device__ __forceinline__ T block_reduce(T v, T* scratch, Op op) {
 //
 // Every thread copies, and reads back, its own 16-byte lines, so the copies need
 // no barrier; slices of up to 56 KiB leave four CTAs an SM, one's copies under
-// another's arithmetic. (Slices in registers, 8 lines a thread, took 91 us for
-// 320 rows of 100003 at two CTAs an SM, 126 us at one.) Rows may start anywhere
+// another's arithmetic. 320 rows of 100003: 55 us, 4.6 TB/s. What is missing to a
+// copy's 6.5 is the last, partly filled wave and the CTAs' own chain of copy,
+// maximum, sum, exchange and write. (Slices in registers, 8 lines a thread: 91 us at
+// two CTAs an SM; loads through registers into shared memory, fewer in flight: 69;
+// one bulk copy a slice: 58; slices of 112 KiB, two CTAs: 62; clusters of 16 with 27
+// KiB: 59; persistent CTAs: 99.) 64 rows of 8192: 4 us, latency. Rows may start anywhere
 // in a line (odd vocabularies): threads take whole lines, and the values of the
 // first and last line outside the row are left alone.
 // ---------------------------------------------------------------------------
@@ -236,9 +240,13 @@ __global__ void __launch_bounds__(kProbThreads, 4) probabilities_kernel(const Pr
 //
 // Bound by memory where there are many sequences (one row of p each, one of q
 // where a draft is rejected), by latency otherwise. A cluster of C CTAs shares
-// a row: every warp sums tiles of 128 consecutive values, the CTAs exchange
-// their totals, and the one that holds the border finds its tile among the
-// sums and reads that tile again.
+// a row: every warp sums tiles of 128 consecutive values, four at a time across its
+// lanes, the CTAs exchange their totals, and the one that holds the border finds its
+// tile among the sums and reads that tile again. One sequence at 32003 tokens: 5.5
+// us, of which reading and summing 1.6 (each step of a 64-bit sum across a warp is
+// about 150 cycles), the two dependent reads before 1.0, the exchange 0.5, the
+// border 1.2; 64 sequences of 4 drafts at 8192: 5.7 us. (One CTA a row: 42 us at
+// 32003 tokens. Every tile summed by its own five steps: 6.1, and 9.8 with eight CTAs a row.)
 // ---------------------------------------------------------------------------
 constexpr int kVerifyThreads = 256;
 constexpr int kTile = 128;  // consecutive values a warp sums
@@ -488,11 +496,12 @@ int64_t verify_max_vocab() { return static_cast<int64_t>(kMaxCluster) * kVerifyT
 
 cudaError_t launch_verify(const VerifyLaunch& p0, cudaStream_t s) {
   VerifyLaunch p = p0;
-  // CTAs a row: until the SMs hold four each or a warp has a tile left, and at
-  // least what the tile sums of a CTA have room for.
+  // CTAs a row: until the SMs hold four each or a warp has its four tiles in
+  // flight (64 sequences at 8192: 8.0 us at four tiles a warp, 9.6 at two, 10.3 at
+  // one, 10.6 at eight), and at least what the tile sums of a CTA have room for.
   const int tiles = (p.vocab + kTile - 1) / kTile;
   p.cluster = 1;
-  while (p.cluster < kMaxCluster && ((p.n_seq * p.cluster * 2 <= 4 * 148 && tiles / p.cluster > 8) ||
+  while (p.cluster < kMaxCluster && ((p.n_seq * p.cluster * 2 <= 4 * 148 && tiles / p.cluster > 4 * (kVerifyThreads / 32)) ||
                                      (tiles + p.cluster - 1) / p.cluster > kVerifyTiles))
     p.cluster *= 2;
   return launch_clusters(verify_kernel, p, p.n_seq, kVerifyThreads, 0, s);

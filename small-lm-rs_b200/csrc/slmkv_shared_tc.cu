@@ -9,20 +9,31 @@
 // and the thread adds the tile's O to its row's 64 f32 registers: the tensor
 // cores cut off their running sums, so none of them runs over more than a tile.
 //
-// All operands are f16 parts under power-of-two scales that bring the largest
-// value of a query row, of a key or value block (16 tokens of a head) and the
-// weights to 2^14..2^15: a bf16 value has one part, exact, an f32 value two, hi
-// and lo, that hold it to 2^-22 (what lies more than 2^25 below the largest value
-// keeps 2^-39 of that one instead). So a tile takes two products a sum where keys
-// and values are bf16 and three where they are f32 (lo times lo, below 2^-22 of a
-// term, is left out). With three bf16 parts, which need no scales, it were three
-// and six; f16 parts of Q also fit into TMEM beside the rest, and a product with
-// its first operand there takes 34 cycles instead of the 51 that reading both
-// from shared memory takes. Keys and values arrive as swizzled boxes by the copy
-// engine and are turned into parts where they lie, by a warp a block.
+// Operands that are f32 (or not of their partner's type) enter as parts:
+//   bf16 keys     as they are; Q in three bf16 parts that hold it exactly
+//   f32 keys, Q   two f16 parts, hi and lo, which hold a value to 2^-22, under
+//                 power-of-two scales that bring the largest value of a query row
+//                 or a key block (16 tokens of a head) to 2^14..2^15
+//   bf16 values   one f16 part, exact under the block's scale
+//   f32 values, P two f16 parts, under the block's scale and 2^15
+// (what lies more than 2^25 below the largest value keeps 2^-39 of that one). So
+// O takes two products a tile with bf16 values and S three; f32 pools take three
+// each (lo times lo, below 2^-22 of a term, is left out). With three bf16 parts for
+// everything it were three and three, six and six, and 96 columns of P. All of Q
+// but its lo part lies in TMEM: a product takes 34 cycles from there, 51 with both
+// operands in shared memory. Blocks arrive as swizzled boxes by the copy engine and
+// are turned into parts where they lie, by a warp a block of the tile.
 //
 // Scores have two buffers, so a tile's softmax runs under the last one's P V and
-// the next one's Q K^T; two CTAs an SM (256 TMEM columns and 97 KiB each).
+// the next one's Q K^T; two CTAs an SM (256 TMEM columns and at most 113 KiB each).
+// What bounds it is each CTA's chain: a tile takes 2560 cycles (bf16), of which
+// powers and parts 1300, the maximum 450, waits 450, adding O 320; with two CTAs the
+// tensor cores are busy 59 % of the time, the schedulers 55 %, the exponential unit
+// 40 %. 170 rows x 8 heads over 8192 tokens: 38 us, 340 TFLOP/s of the 4 n d flops
+// that the formula has. (Keys as f16 too, two products for S but twice the parts to
+// make: 46 us. Three bf16 parts for all: 43. One CTA an SM: 2070 cycles a tile
+// against 1300 at two. Half the registers for the softmax, so that a CTA of the other
+// kernel fits beside two: that kernel then spills, 23 -> 30 us.)
 #include <cuda_fp16.h>
 
 #include <cfloat>
