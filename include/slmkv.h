@@ -263,7 +263,7 @@ slm_status slm_batch_append_layer_normed(slm_batch* batch, int32_t layer, const 
  * layers; plan buffers and the joined parts' scratch are allocated by the
  * context's first call and grow when a call needs more (which waits for the
  * device). A batch's first call is refused while its stream is being captured
- * into a graph. */
+ * into a graph; a captured later one may be replayed until the batch ends. */
 slm_status slm_batch_shared_attention(slm_batch* batch, int32_t layer, const float* d_query,
                                       int32_t rotate_query, float* d_out);
 /* Probabilities of logit rows (no reference counterpart: greedy.rs takes the

@@ -2092,6 +2092,10 @@ slm_status shared_prepare(slm_batch* b) {
                o_merge = place(plan.merge);
   slm_ctx::SharedIo& io = c->shared;
   const int k = b->up_slot;
+  auto allocated = [](cudaError_t e) {  // a failure is this call's, not the next launch's
+    if (e != cudaSuccess) cudaGetLastError();
+    return e;
+  };
   if (bytes > io.cap) {
     CU(c, cudaDeviceSynchronize());  // a slot may be in use
     for (int i = 0; i < kUploadSlots; ++i) {
@@ -2103,8 +2107,8 @@ slm_status shared_prepare(slm_batch* b) {
     io.cap = 0;
     const size_t cap = align16(bytes + bytes / 2 + 4096);
     for (int i = 0; i < kUploadSlots; ++i) {
-      CU(c, cudaMallocHost(reinterpret_cast<void**>(&io.h[i]), cap));
-      CU(c, cudaMalloc(reinterpret_cast<void**>(&io.d[i]), cap));
+      CU(c, allocated(cudaMallocHost(reinterpret_cast<void**>(&io.h[i]), cap)));
+      CU(c, allocated(cudaMalloc(reinterpret_cast<void**>(&io.d[i]), cap)));
       if (!io.copied[i]) CU(c, cudaEventCreateWithFlags(&io.copied[i], cudaEventDisableTiming));
     }
     io.cap = cap;
@@ -2120,8 +2124,8 @@ slm_status shared_prepare(slm_batch* b) {
     c->device_bytes -= static_cast<int64_t>(io.part_cap * kPart);
     io.part_cap = 0;
     const size_t cap = static_cast<size_t>(plan.parts) + static_cast<size_t>(plan.parts) / 4;
-    CU(c, cudaMalloc(reinterpret_cast<void**>(&io.part_acc), cap * kHeadDim * sizeof(float)));
-    CU(c, cudaMalloc(reinterpret_cast<void**>(&io.part_ml), cap * sizeof(float2)));
+    CU(c, allocated(cudaMalloc(reinterpret_cast<void**>(&io.part_acc), cap * kHeadDim * sizeof(float))));
+    CU(c, allocated(cudaMalloc(reinterpret_cast<void**>(&io.part_ml), cap * sizeof(float2))));
     io.part_cap = cap;
     c->device_bytes += static_cast<int64_t>(cap * kPart);
   }
