@@ -322,8 +322,8 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
       const SharedToken tk = p.tokens[it.token0 + min(tid / G, it.n_tokens - 1)];
       uint8_t* rows = sm + Cfg::kOffV + Cfg::kFirstQStage * kStageBytes + warp * (32 * D * 4);
       const int u = lane & 15;
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
+#pragma unroll 1
+      for (int b = 0; b < 2; ++b) {  // (loops: a kernel's start waits for its code)
         float4 x[8], cs[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -345,34 +345,42 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
       }
       __syncwarp();
       const bool live = tid / G < it.n_tokens;
-      float4 x[D / 4];
-      float most = 0.f;
-#pragma unroll
-      for (int i = 0; i < D / 4; ++i) {
-        x[i] = *reinterpret_cast<const float4*>(rows + lane * (D * 4) + ((i ^ (lane & 15)) << 4));
-        if (!live) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (!BF16) most = fmax3(most, fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
-        fin = fmaf(x[i].x, 0.f, fmaf(x[i].y, 0.f, fmaf(x[i].z, 0.f, fmaf(x[i].w, 0.f, fin))));
+      auto value = [&](int i) {  // 4i .. 4i + 3 of the thread's row
+        const float4 y = *reinterpret_cast<const float4*>(rows + lane * (D * 4) + ((i ^ (lane & 15)) << 4));
+        return live ? y : make_float4(0.f, 0.f, 0.f, 0.f);
+      };
+      int field = 127;
+      if constexpr (!BF16) {
+        float most = 0.f;
+#pragma unroll 4
+        for (int i = 0; i < D / 4; ++i) {
+          const float4 y = value(i);
+          most = fmax3(most, fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)));
+        }
+        field = scale_field(__float_as_int(most) >> 23);  // (of +inf too, whose row fails)
+        q_scale = power_of_field(254 - field);
       }
-      const int field = fin == 0.f ? scale_field(__float_as_int(most) >> 23) : 127;
-      if (!BF16) q_scale = power_of_field(254 - field);
       const uint64_t f2 = pack2(power_of_field(field), power_of_field(field));
-#pragma unroll
+#pragma unroll 1
       for (int ks = 0; ks < D / 16; ++ks) {
         uint32_t first[8], second[8], third[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float4& v = x[4 * ks + i / 2];
-          const uint64_t w = i & 1 ? pack2(v.z, v.w) : pack2(v.x, v.y);
-          if constexpr (BF16) {
-            const Parts a = split_pair(w);
-            first[i] = a.hi;
-            second[i] = a.mid;
-            third[i] = a.lo;
-          } else {
-            const Halves a = split_halves(mul2(w, f2));
-            first[i] = a.hi;
-            second[i] = a.lo;
+        for (int i = 0; i < 4; ++i) {
+          const float4 y = value(4 * ks + i);
+          fin = fmaf(y.x, 0.f, fmaf(y.y, 0.f, fmaf(y.z, 0.f, fmaf(y.w, 0.f, fin))));
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint64_t w = k ? pack2(y.z, y.w) : pack2(y.x, y.y);
+            if constexpr (BF16) {
+              const Parts a = split_pair(w);
+              first[2 * i + k] = a.hi;
+              second[2 * i + k] = a.mid;
+              third[2 * i + k] = a.lo;
+            } else {
+              const Halves a = split_halves(mul2(w, f2));
+              first[2 * i + k] = a.hi;
+              second[2 * i + k] = a.lo;
+            }
           }
         }
         tmem_store16(trow + kQCol + part_col(ks, 0), first, second);
@@ -523,17 +531,33 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
     }
     if (!ok) {
       raise();
-    } else if (tid / G < it.n_tokens) {
-      // softmax.rs:17-22: a score that is not finite fails the row's sequence
-      float f0, f1;
-      unpack2(fin2, f0, f1);
-      if (!(fin == 0.f && f0 == 0.f && f1 == 0.f) && p.status) atomicOr(&p.status[p.tokens[it.token0 + tid / G].seq], kStatusNonFiniteScore);
-      const size_t slot = static_cast<size_t>(it.part) + tid;
+    } else {
+      if (tid / G < it.n_tokens) {
+        // softmax.rs:17-22: a score that is not finite fails the row's sequence
+        float f0, f1;
+        unpack2(fin2, f0, f1);
+        if (!(fin == 0.f && f0 == 0.f && f1 == 0.f) && p.status)
+          atomicOr(&p.status[p.tokens[it.token0 + tid / G].seq], kStatusNonFiniteScore);
+        p.part_ml[static_cast<size_t>(it.part) + tid] = make_float2(m, l * 0x1p-15f);
+      }
+      // The rows' parts lie one after the other: through shared memory (the last
+      // product has read it), two whole rows a store. A row a thread, each store
+      // met 32 lines, 3500 cycles an item.
+      uint8_t* rows = sm + warp * (32 * D * 4);
       const uint64_t down = pack2(0x1p-15f, 0x1p-15f);
-      p.part_ml[slot] = make_float2(m, l * 0x1p-15f);
-      ulonglong2* dst = reinterpret_cast<ulonglong2*>(p.part_acc + slot * D);
 #pragma unroll
-      for (int i = 0; i < D / 4; ++i) dst[i] = make_ulonglong2(mul2(o[2 * i], down), mul2(o[2 * i + 1], down));
+      for (int i = 0; i < D / 4; ++i)
+        *reinterpret_cast<ulonglong2*>(rows + lane * (D * 4) + ((i ^ (lane & 15)) << 4)) =
+            make_ulonglong2(mul2(o[2 * i], down), mul2(o[2 * i + 1], down));
+      __syncwarp();
+      const int live = it.n_tokens * G - warp * 32, u = lane & 15;
+      float4* dst = reinterpret_cast<float4*>(p.part_acc + (static_cast<size_t>(it.part) + warp * 32) * D);
+#pragma unroll 4
+      for (int i = 0; i < 16; ++i) {
+        const int r = 2 * i + (lane >> 4);
+        const float4 y = *reinterpret_cast<const float4*>(rows + r * (D * 4) + ((u ^ (r & 15)) << 4));
+        if (r < live) dst[r * (D / 4) + u] = y;
+      }
     }
   } else if (warp < 8) {
     // ================= parts: block `warp - 4` of every tile, where it lies =================
