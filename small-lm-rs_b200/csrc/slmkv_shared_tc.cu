@@ -16,7 +16,7 @@
 //                 or a key block (16 tokens of a head) to 2^14..2^15
 //   bf16 values   one f16 part, exact under the block's scale
 //   f32 values, P two f16 parts, under the block's scale and 2^15
-// (what lies more than 2^25 below the largest value keeps 2^-39 of that one). So
+// (an f32 value more than 2^17 below the largest one keeps 2^-40 of that instead). So
 // O takes two products a tile with bf16 values and S three; f32 pools take three
 // each (lo times lo, below 2^-22 of a term, is left out). With three bf16 parts for
 // everything it were three and three, six and six, and 96 columns of P. All of Q

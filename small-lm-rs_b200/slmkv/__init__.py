@@ -679,11 +679,11 @@ class Batch:
         """Device address of a CUDA tensor (float32, or ``dtype``) of the
         pool's device with this shape; ``rows``: dense rows at any distance
         instead of contiguous."""
-        torch = _torch()
+        torch = _torch_module or _torch()
         if not isinstance(t, torch.Tensor):
             raise TypeError("expected a torch tensor")
-        if t.shape == shape and t.dtype is (dtype or torch.float32) and t.is_cuda \
-                and t.get_device() == self.pool.device:
+        # (a tensor on the host is on device -1, and the pool is not)
+        if t.shape == shape and t.dtype is (dtype or torch.float32) and t.get_device() == self.pool.device:
             if t.is_contiguous():
                 return t.data_ptr()
             if rows:

@@ -457,3 +457,22 @@ def test_long_caches_of_one_sequence(hq, hkv, lengths, counts, dtype):
 def test_shared_and_long_runs_with_one_query_head(dtype):
     paths = [path((1, 1600), (9000 * i, 1300 + 7 * i)) for i in range(1, 4)]
     Forest(4, 4, paths, [40, 33, 1], dtype, seed=5).check()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_an_outlying_channel_on_the_tensor_cores(dtype):
+    """One channel of the keys 2^17 times the others, of the queries 2^-17 times:
+    the others keep 2^-40 of the large ones at least, 2^-22 of their own size."""
+    n, prefix, hq, hkv = 48, 1024, 8, 2
+    f = Forest(hq, hkv, [path((1, prefix), (70 * i, 3)) for i in range(2, 2 + n)], [1] * n, dtype, seed=24)
+    key, _ = f.pool.storage()
+    key[0, ..., 7] *= 2.0**17  # exact in both types
+    for x in f.kv:
+        f.kv[x][0][:, 7] *= 2.0**17
+    q, nk, nv = f.new_rows()
+    q[:, :, 7] *= 2.0**-17
+    nk[:, :, 7] *= 2.0**17
+    with f.pool.begin(f.caches, f.counts) as b:
+        out = f.attend(b, 0, (q, nk, nv))
+    ref, tol = f.reference(0, q, nk, nv)
+    assert (out.double() - ref).abs().max().item() <= tol
