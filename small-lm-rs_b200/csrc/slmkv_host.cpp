@@ -220,11 +220,11 @@ struct slm_ctx {
   // (the batch's up_slot), and the parts of rows joined from several runs.
   // Both are allocated at the first call and grown on demand.
   struct SharedIo {
-    uint8_t* h[kUploadSlots] = {};
-    uint8_t* d[kUploadSlots] = {};
+    uint8_t* h = nullptr;  // all slots', pinned and on the device
+    uint8_t* d = nullptr;
     cudaEvent_t copied[kUploadSlots] = {};
     size_t cap = 0;  // bytes a slot
-    float* part_acc = nullptr;
+    float* part_acc = nullptr;  // and behind them part_ml
     float2* part_ml = nullptr;
     size_t part_cap = 0;  // row slots
     // The batch that used the parts last: its descriptor slot and stream.
@@ -825,13 +825,11 @@ void destroy_device(slm_ctx* c) {
       if (ev) cudaEventDestroy(ev);
   }
   if (c->io.h2d) cudaStreamDestroy(c->io.h2d);
-  for (int k = 0; k < kUploadSlots; ++k) {
-    if (c->shared.h[k]) cudaFreeHost(c->shared.h[k]);
-    if (c->shared.d[k]) cudaFree(c->shared.d[k]);
-    if (c->shared.copied[k]) cudaEventDestroy(c->shared.copied[k]);
-  }
+  for (cudaEvent_t ev : c->shared.copied)
+    if (ev) cudaEventDestroy(ev);
+  if (c->shared.h) cudaFreeHost(c->shared.h);
+  if (c->shared.d) cudaFree(c->shared.d);
   if (c->shared.part_acc) cudaFree(c->shared.part_acc);
-  if (c->shared.part_ml) cudaFree(c->shared.part_ml);
   if (c->copy_stream) cudaStreamDestroy(c->copy_stream);
   if (c->readback_stream) cudaStreamDestroy(c->readback_stream);
 }
@@ -2097,40 +2095,36 @@ slm_status shared_prepare(slm_batch* b) {
     return e;
   };
   if (bytes > io.cap) {
-    CU(c, cudaDeviceSynchronize());  // a slot may be in use
-    for (int i = 0; i < kUploadSlots; ++i) {
-      if (io.h[i]) cudaFreeHost(io.h[i]);
-      if (io.d[i]) cudaFree(io.d[i]);
-      io.h[i] = io.d[i] = nullptr;
-    }
+    if (io.cap) CU(c, cudaDeviceSynchronize());  // a slot may be in use
+    if (io.h) cudaFreeHost(io.h);
+    if (io.d) cudaFree(io.d);
+    io.h = io.d = nullptr;
     c->device_bytes -= static_cast<int64_t>(io.cap) * kUploadSlots;
     io.cap = 0;
     const size_t cap = align16(bytes + bytes / 2 + 4096);
-    for (int i = 0; i < kUploadSlots; ++i) {
-      CU(c, allocated(cudaMallocHost(reinterpret_cast<void**>(&io.h[i]), cap)));
-      CU(c, allocated(cudaMalloc(reinterpret_cast<void**>(&io.d[i]), cap)));
-      if (!io.copied[i]) CU(c, cudaEventCreateWithFlags(&io.copied[i], cudaEventDisableTiming));
-    }
+    CU(c, allocated(cudaMallocHost(reinterpret_cast<void**>(&io.h), cap * kUploadSlots)));
+    CU(c, allocated(cudaMalloc(reinterpret_cast<void**>(&io.d), cap * kUploadSlots)));
+    for (cudaEvent_t& ev : io.copied)
+      if (!ev) CU(c, cudaEventCreateWithFlags(&ev, cudaEventDisableTiming));
     io.cap = cap;
     c->device_bytes += static_cast<int64_t>(cap) * kUploadSlots;
   }
   if (static_cast<size_t>(plan.parts) > io.part_cap) {
-    CU(c, cudaDeviceSynchronize());
+    if (io.part_cap) CU(c, cudaDeviceSynchronize());
     if (io.part_acc) cudaFree(io.part_acc);
-    if (io.part_ml) cudaFree(io.part_ml);
     io.part_acc = nullptr;
     io.part_ml = nullptr;
     constexpr size_t kPart = kHeadDim * sizeof(float) + sizeof(float2);
     c->device_bytes -= static_cast<int64_t>(io.part_cap * kPart);
     io.part_cap = 0;
     const size_t cap = static_cast<size_t>(plan.parts) + static_cast<size_t>(plan.parts) / 4;
-    CU(c, allocated(cudaMalloc(reinterpret_cast<void**>(&io.part_acc), cap * kHeadDim * sizeof(float))));
-    CU(c, allocated(cudaMalloc(reinterpret_cast<void**>(&io.part_ml), cap * sizeof(float2))));
+    CU(c, allocated(cudaMalloc(reinterpret_cast<void**>(&io.part_acc), cap * kPart)));
+    io.part_ml = reinterpret_cast<float2*>(io.part_acc + cap * kHeadDim);
     io.part_cap = cap;
     c->device_bytes += static_cast<int64_t>(cap * kPart);
   }
   CU(c, cudaEventSynchronize(io.copied[k]));  // the slot's last upload has left the pinned buffer
-  uint8_t* h = io.h[k];
+  uint8_t* h = io.h + k * io.cap;
   auto put = [&](size_t at, const auto& v) { memcpy(h + at, v.data(), v.size() * sizeof(v[0])); };
   put(o_items, plan.items);
   put(o_tc, plan.tc_items);
@@ -2146,10 +2140,10 @@ slm_status shared_prepare(slm_batch* b) {
     CU(c, cudaStreamWaitEvent(b->stream, c->up_batch.consumed[io.last_slot], 0));
   io.last_slot = k;
   io.last_stream = b->stream;
-  CU(c, cudaMemcpyAsync(io.d[k], h, bytes, cudaMemcpyHostToDevice, b->stream));
+  CU(c, cudaMemcpyAsync(io.d + k * io.cap, h, bytes, cudaMemcpyHostToDevice, b->stream));
   CU(c, cudaEventRecord(io.copied[k], b->stream));
   SharedAttentionLaunch& p = b->shared;
-  const uint8_t* d = io.d[k];
+  const uint8_t* d = io.d + k * io.cap;
   p.items = reinterpret_cast<const SharedItem*>(d + o_items);
   p.tc_items = reinterpret_cast<const SharedItem*>(d + o_tc);
   p.list_start = reinterpret_cast<const int32_t*>(d + o_lists);
