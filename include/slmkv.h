@@ -262,7 +262,7 @@ slm_status slm_batch_append_layer_normed(slm_batch* batch, int32_t layer, const 
  * Same arguments; 16-byte aligned buffers that do not overlap. Meant for few new tokens a sequence: long prompts run faster
  * through slm_batch_prefill_attention. A batch's first call plans it for all
  * layers; plan buffers and the joined parts' scratch are allocated by the
- * context's first call and grow when a call needs more (which waits for the
+ * context's first such calls and grow when one needs more (which waits for the
  * device). A batch's first call is refused while its stream is being captured
  * into a graph; a captured later one may be replayed until the batch ends. */
 slm_status slm_batch_shared_attention(slm_batch* batch, int32_t layer, const float* d_query,

@@ -218,12 +218,12 @@ struct slm_ctx {
   } io;
   // slm_batch_shared_attention: plan staging, one buffer per descriptor slot
   // (the batch's up_slot), and the parts of rows joined from several runs.
-  // Both are allocated at the first call and grown on demand.
+  // Both are allocated by the first calls and grown on demand.
   struct SharedIo {
-    uint8_t* h = nullptr;  // all slots', pinned and on the device
-    uint8_t* d = nullptr;
+    uint8_t* h[kUploadSlots] = {};
+    uint8_t* d[kUploadSlots] = {};
     cudaEvent_t copied[kUploadSlots] = {};
-    size_t cap = 0;  // bytes a slot
+    size_t cap[kUploadSlots] = {};  // bytes
     float* part_acc = nullptr;  // and behind them part_ml
     float2* part_ml = nullptr;
     size_t part_cap = 0;  // row slots
@@ -825,10 +825,11 @@ void destroy_device(slm_ctx* c) {
       if (ev) cudaEventDestroy(ev);
   }
   if (c->io.h2d) cudaStreamDestroy(c->io.h2d);
-  for (cudaEvent_t ev : c->shared.copied)
-    if (ev) cudaEventDestroy(ev);
-  if (c->shared.h) cudaFreeHost(c->shared.h);
-  if (c->shared.d) cudaFree(c->shared.d);
+  for (int k = 0; k < kUploadSlots; ++k) {
+    if (c->shared.h[k]) cudaFreeHost(c->shared.h[k]);
+    if (c->shared.d[k]) cudaFree(c->shared.d[k]);
+    if (c->shared.copied[k]) cudaEventDestroy(c->shared.copied[k]);
+  }
   if (c->shared.part_acc) cudaFree(c->shared.part_acc);
   if (c->copy_stream) cudaStreamDestroy(c->copy_stream);
   if (c->readback_stream) cudaStreamDestroy(c->readback_stream);
@@ -2094,20 +2095,19 @@ slm_status shared_prepare(slm_batch* b) {
     if (e != cudaSuccess) cudaGetLastError();
     return e;
   };
-  if (bytes > io.cap) {
-    if (io.cap) CU(c, cudaDeviceSynchronize());  // a slot may be in use
-    if (io.h) cudaFreeHost(io.h);
-    if (io.d) cudaFree(io.d);
-    io.h = io.d = nullptr;
-    c->device_bytes -= static_cast<int64_t>(io.cap) * kUploadSlots;
-    io.cap = 0;
+  if (bytes > io.cap[k]) {  // (a slot at a time: large pinned allocations take milliseconds)
+    if (io.cap[k]) CU(c, cudaDeviceSynchronize());  // it may be in use
+    if (io.h[k]) cudaFreeHost(io.h[k]);
+    if (io.d[k]) cudaFree(io.d[k]);
+    io.h[k] = io.d[k] = nullptr;
+    c->device_bytes -= static_cast<int64_t>(io.cap[k]);
+    io.cap[k] = 0;
     const size_t cap = align16(bytes + bytes / 2 + 4096);
-    CU(c, allocated(cudaMallocHost(reinterpret_cast<void**>(&io.h), cap * kUploadSlots)));
-    CU(c, allocated(cudaMalloc(reinterpret_cast<void**>(&io.d), cap * kUploadSlots)));
-    for (cudaEvent_t& ev : io.copied)
-      if (!ev) CU(c, cudaEventCreateWithFlags(&ev, cudaEventDisableTiming));
-    io.cap = cap;
-    c->device_bytes += static_cast<int64_t>(cap) * kUploadSlots;
+    CU(c, allocated(cudaMallocHost(reinterpret_cast<void**>(&io.h[k]), cap)));
+    CU(c, allocated(cudaMalloc(reinterpret_cast<void**>(&io.d[k]), cap)));
+    if (!io.copied[k]) CU(c, cudaEventCreateWithFlags(&io.copied[k], cudaEventDisableTiming));
+    io.cap[k] = cap;
+    c->device_bytes += static_cast<int64_t>(cap);
   }
   if (static_cast<size_t>(plan.parts) > io.part_cap) {
     if (io.part_cap) CU(c, cudaDeviceSynchronize());
@@ -2124,7 +2124,7 @@ slm_status shared_prepare(slm_batch* b) {
     c->device_bytes += static_cast<int64_t>(cap * kPart);
   }
   CU(c, cudaEventSynchronize(io.copied[k]));  // the slot's last upload has left the pinned buffer
-  uint8_t* h = io.h + k * io.cap;
+  uint8_t* h = io.h[k];
   auto put = [&](size_t at, const auto& v) { memcpy(h + at, v.data(), v.size() * sizeof(v[0])); };
   put(o_items, plan.items);
   put(o_tc, plan.tc_items);
@@ -2140,10 +2140,10 @@ slm_status shared_prepare(slm_batch* b) {
     CU(c, cudaStreamWaitEvent(b->stream, c->up_batch.consumed[io.last_slot], 0));
   io.last_slot = k;
   io.last_stream = b->stream;
-  CU(c, cudaMemcpyAsync(io.d + k * io.cap, h, bytes, cudaMemcpyHostToDevice, b->stream));
+  CU(c, cudaMemcpyAsync(io.d[k], h, bytes, cudaMemcpyHostToDevice, b->stream));
   CU(c, cudaEventRecord(io.copied[k], b->stream));
   SharedAttentionLaunch& p = b->shared;
-  const uint8_t* d = io.d + k * io.cap;
+  const uint8_t* d = io.d[k];
   p.items = reinterpret_cast<const SharedItem*>(d + o_items);
   p.tc_items = reinterpret_cast<const SharedItem*>(d + o_tc);
   p.list_start = reinterpret_cast<const int32_t*>(d + o_lists);
