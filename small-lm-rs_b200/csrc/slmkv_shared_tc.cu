@@ -15,8 +15,11 @@
 //                 power-of-two scales that bring the largest value of a query row
 //                 or a key block (16 tokens of a head) to 2^14..2^15
 //   bf16 values   one f16 part, exact under the block's scale
-//   f32 values, P two f16 parts, under the block's scale and 2^15
-// (an f32 value more than 2^17 below the largest one keeps 2^-40 of that instead). So
+//   f32 values, P two f16 parts, under the block's scale and a scale of P's that
+//                 makes the largest product of the row's weights and a block's
+//                 values one unit
+// (an f32 value more than 2^17 below the largest one, or such a weight's product, keeps
+// 2^-40 of that instead). So
 // O takes two products a tile with bf16 values and S three; f32 pools take three
 // each (lo times lo, below 2^-22 of a term, is left out). With three bf16 parts for
 // everything it were three and three, six and six, and 96 columns of P. All of Q
@@ -61,7 +64,7 @@ constexpr int kMmaWarp = 8, kLoadWarp = 9;
 constexpr int kTmemCols = 256, kQCol = 0, kBufCol = 64, kBufCols = 64, kOCol = 192;
 struct Scales {  // of a tile's blocks
   float key[4];   // 2^-b: of the scores
-  int value[4];   // c + 127: values are times 2^c
+  float value[4];  // c: values are times 2^c
 };
 template <int BF16>
 struct TcCfg {
@@ -249,6 +252,14 @@ __device__ __forceinline__ Halves split_halves(uint64_t xy) {
 // 2^14..2^15, as c + 127; a block or row of zeros, or nearly, gets 2^126.
 __device__ __forceinline__ int scale_field(int exponent) { return min(268 - exponent, 253); }
 __device__ __forceinline__ float power_of_field(int field) { return __int_as_float(field << 23); }
+// The nearest whole number, of numbers to 2^22; and 2^e of a whole e from -127
+// (0) to 127. Both by the lowest bits of a sum with 1.5 2^23, since conversions
+// have a slow unit.
+constexpr float kWhole = 12582912.f;
+__device__ __forceinline__ float whole(float x) { return __fadd_rn(__fadd_rn(x, kWhole), -kWhole); }
+__device__ __forceinline__ float power(float e) {
+  return __int_as_float((__float_as_int(__fadd_rn(e, kWhole)) << 23) + (127 << 23));
+}
 // One lane of the warp, in a form that keeps the issued operands uniform: under
 // `lane == 0` each product took 100 to 200 cycles to issue.
 __device__ __forceinline__ bool elect_one() {
@@ -436,7 +447,8 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
         for (int i = 0; i < kTokens; ++i) s[i] = __uint_as_float(v[i >> 5][i & 31]);
       }
       const Scales& sc = ring[j % Cfg::kRing];
-      const int4 vf = *reinterpret_cast<const int4*>(sc.value);
+      const float4 vc4 = *reinterpret_cast<const float4*>(sc.value);
+      const float vc[4] = {vc4.x, vc4.y, vc4.z, vc4.w};
       float f[4] = {1.f, 1.f, 1.f, 1.f};
       if constexpr (!BF16) {
         const float4 ks4 = *reinterpret_cast<const float4*>(sc.key);
@@ -464,9 +476,8 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
       }
       // the running maximum, rounded up to a whole number: its differences and the
       // exponents below are exact
-      float mx;
+      float mx, m4[4];  // (m4: of a block)
       {  // four chains
-        float m4[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           float x = fmax3(s[16 * k], s[16 * k + 1], s[16 * k + 2]);
@@ -485,15 +496,23 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
         f[0] = f[1] = f[2] = f[3] = 1.f;
         ref = 0.f;
       }
-      // Weights are times 2^15, and a block's by what its values' scale is above
-      // the tile's least (at most 2^60: beyond, the values are nothing beside the
-      // largest ones), so that the products are all in one unit.
-      const int least = min(min(vf.x, vf.y), min(vf.z, vf.w));
-      const int above[4] = {min(vf.x - least, 60), min(vf.y - least, 60), min(vf.z - least, 60), min(vf.w - least, 60)};
+      // A block's values are times 2^c and its weights, at most 2^e (a whole number at
+      // or less than two above the largest exponent), times 2^(15 - a) with a = c - u, so that the products of
+      // all blocks are in the row's one unit 2^-(u + 15). u is the least of c - e:
+      // then no weight passes 2^15, and what parts cut off of weights is 2^-40 of the
+      // largest product of a weight and a value that the row has, not of the largest
+      // value, which it may not attend to. (Beyond u = 126 products fade below f32,
+      // beyond a = 60 a block's are nothing beside the largest ones.)
+      float u = 126.f, above[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        u = fminf(u, vc[k] - whole(fmaxf(m4[k] - mx, -1024.f) + 0.5f));
+#pragma unroll
+      for (int k = 0; k < 4; ++k) above[k] = fmaxf(fminf(vc[k] - u, 60.f), -127.f);
       l *= next_corr;
 #pragma unroll
       for (int ks = 0; ks < kTokens / 16; ++ks) {
-        const float add = 15.f - ref - static_cast<float>(above[ks]);
+        const float add = 15.f - ref - above[ks];
         const uint64_t f2 = pack2(f[ks], f[ks]), up = pack2(add, add);
         uint64_t sum = 0ull;
         uint32_t hi[8], lo[8];
@@ -511,7 +530,7 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
         tmem_store16(buf + part_col(ks, 0), hi, lo);
         float a, b;
         unpack2(sum, a, b);
-        l = fmaf(a + b, power_of_field(127 + above[ks]), l);
+        l = fmaf(a + b, power(above[ks]), l);
       }
       if (j > 0) {  // the last tile's O, before the next product takes its place
         if (!(ok = wait(Cfg::kBarODone, (j - 1) & 1))) break;
@@ -519,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
         add_o();
       }
       corr = next_corr;
-      unit = power_of_field(254 - least);
+      unit = power(-u);
       tmem_wait_store();
       fence_before();
       __syncwarp();
@@ -632,7 +651,7 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) {
-        ring[j % Cfg::kRing].value[block] = value;
+        ring[j % Cfg::kRing].value[block] = static_cast<float>(value - 127);
         bar_arrive(bar(Cfg::kBarVFull + st));
       }
     }
