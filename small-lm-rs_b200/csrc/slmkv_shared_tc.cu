@@ -501,9 +501,9 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
       // all blocks are in the row's one unit 2^-(u + 15). u is the least of c - e:
       // then no weight passes 2^15, and what parts cut off of weights is 2^-40 of the
       // largest product of a weight and a value that the row has, not of the largest
-      // value, which it may not attend to. (Beyond u = 126 products fade below f32,
-      // beyond a = 60 a block's are nothing beside the largest ones.)
-      float u = 126.f, above[4];
+      // value, which it may not attend to. (u stays at 111: products below f32's
+      // normal numbers fade. Beyond a = 60 a block's are nothing beside the largest ones.)
+      float u = 111.f, above[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k)
         u = fminf(u, vc[k] - whole(fmaxf(m4[k] - mx, -1024.f) + 0.5f));
@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
         add_o();
       }
       corr = next_corr;
-      unit = power(-u);
+      unit = power(-15.f - u);  // (undone a tile: O times 2^15 would leave f32 where the sum does not)
       tmem_wait_store();
       fence_before();
       __syncwarp();
@@ -563,11 +563,9 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
       // product has read it), two whole rows a store. A row a thread, each store
       // met 32 lines, 3500 cycles an item.
       uint8_t* rows = sm + warp * (32 * D * 4);
-      const uint64_t down = pack2(0x1p-15f, 0x1p-15f);
 #pragma unroll
       for (int i = 0; i < D / 4; ++i)
-        *reinterpret_cast<ulonglong2*>(rows + lane * (D * 4) + ((i ^ (lane & 15)) << 4)) =
-            make_ulonglong2(mul2(o[2 * i], down), mul2(o[2 * i + 1], down));
+        *reinterpret_cast<ulonglong2*>(rows + lane * (D * 4) + ((i ^ (lane & 15)) << 4)) = make_ulonglong2(o[2 * i], o[2 * i + 1]);
       __syncwarp();
       const int live = it.n_tokens * G - warp * 32, u = lane & 15;
       float4* dst = reinterpret_cast<float4*>(p.part_acc + (static_cast<size_t>(it.part) + warp * 32) * D);

@@ -141,6 +141,17 @@ def test_sizes_and_weights_that_balance(spread, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("size", [1e30, 1e34, 1e35, 1e-30, 1e-36])
+def test_values_near_the_ends_of_f32(size, dtype):
+    """Sums of weights times values stay in f32's range: 1024 of 1e35 do."""
+    f = Shared(dtype, 7)
+    k, v = f.shared_like()
+    f.write(0.5 * k, (1 + 0.1 * v) * size)
+    q, nk, nv = f.randn(N, HQ, D), f.randn(N, HKV, D), (1 + 0.1 * f.randn(N, HKV, D)) * size
+    f.check(0.25 * q, nk, nv)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("scale_k,size_v", [(1e-20, 1e12), (1e20, 1e-12), (1.0, 1.0), (1e-30, 1e-20)])
 def test_magnitudes(scale_k, size_v, dtype):
     """Keys and queries of any size whose product stays of order one; a block of
