@@ -298,11 +298,13 @@ slm_status slm_batch_token_probabilities(slm_batch* batch, const float* d_logits
  * rejected draft's row (from its p where nothing of that is left), or after the
  * last draft from its row's p: the first token whose running sum of weights in
  * token order exceeds u times their total. Outside [0, 1) u counts as the nearer
- * end, NaN as 0. The outputs overlap nothing else. Kept cache lengths: slm_seqs_truncate_all to base + 1 + accepted after
- * the batch's end. A drafted token outside the vocabulary fails its sequence with
- * SLM_ERR_INVALID_INPUT when the batch ends, a row it reads that is negative, not
- * finite or all zero with SLM_ERR_NON_FINITE; both give 0 accepted and next token
- * -1. vocab_size up to 655360. */
+ * end, NaN as 0. The outputs overlap nothing else. Kept cache lengths:
+ * slm_seqs_truncate_all to base + 1 + accepted after the batch's end. A drafted
+ * token outside the vocabulary fails its sequence with SLM_ERR_INVALID_INPUT when
+ * the batch ends; values it reads that are negative or not finite (p and q at the
+ * drafts up to the first rejected one, the row or rows that the next token is drawn
+ * from), or a row to draw from that is all zero, with SLM_ERR_NON_FINITE. Both
+ * give 0 accepted and next token -1. vocab_size up to 655360. */
 slm_status slm_batch_verify_drafts(slm_batch* batch, int32_t vocab_size, const int32_t* d_token_ids,
                                    const float* d_target, const float* d_draft,
                                    const float* d_uniforms, int32_t* d_accepted,

@@ -274,6 +274,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyL
     s_flags = 0;
   }
   __syncthreads();
+  auto usable = [](float w) { return w >= 0.f && w <= FLT_MAX; };
   auto uniform = [&](int r) { return fmin(fmax(static_cast<double>(p.uniforms[r]), 0.0), 1.0); };  // (NaN: 0)
   for (int j = tid; j < k; j += kVerifyThreads) {
     const int x = p.token_ids[r0 + j + 1];
@@ -283,7 +284,9 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyL
     }
     const float pt = p.target[static_cast<int64_t>(r0 + j) * V + x];
     const float qt = p.draft ? p.draft[(q0 + j) * V + x] : 1.f;
-    if (!(uniform(r0 + j) * qt < static_cast<double>(pt))) atomicMin(&s_first, j);
+    // values that are no probabilities count as a rejection: the row they are in is
+    // then read whole, and fails the sequence
+    if (!(usable(pt) && usable(qt) && uniform(r0 + j) * qt < static_cast<double>(pt))) atomicMin(&s_first, j);
   }
   const double u = uniform(r0 + k);
   __syncthreads();
@@ -294,7 +297,6 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyL
   const int tiles = (V + kTile - 1) / kTile, per = (tiles + ctas - 1) / ctas;
   const int first_tile = rank * per, n_tiles = max(0, min(tiles, first_tile + per) - first_tile);
   bool rest = a < k;  // the residual; the row itself when nothing of it is left
-  auto usable = [](float w) { return w >= 0.f && w <= FLT_MAX; };
   // of token x; q is zero where there is none
   auto weight = [&](float pv, float qv, int x) {
     return fmax(static_cast<double>(rest && x == skip ? 0.f : pv) - static_cast<double>(qv), 0.0);

@@ -1,0 +1,85 @@
+"""The speculative step's operators at the ends of what their calls allow:
+vocabularies beyond a cluster's shared memory, temperatures at the ends of f32,
+probabilities that are none at accepted drafts, captured calls that are refused
+or dropped, and the model's scores on each of its projection paths."""
+
+import gc
+import math
+
+import numpy as np
+import pytest
+
+import oracle as O
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+slmkv = pytest.importorskip("slmkv")
+
+from test_gpu_model import parity_metrics, random_model  # noqa: E402
+from test_gpu_speculative_step import (D, check_probabilities, gen, randn, rows_batch, run_verify,  # noqa: E402
+                                       verify_reference)
+
+
+# ---- verification ------------------------------------------------------------------
+
+
+def test_verify_values_that_are_no_probabilities_fail_at_accepted_drafts():
+    """What the acceptance of a draft reads has to be a probability, as the rows
+    have to: else the sequence fails. Behind the first rejected draft nothing is
+    read."""
+    vocab, bad = 300, slmkv.ERR_NON_FINITE
+    cases = [  # (p at the draft, q at the draft, status); u is 0.5
+        (0.5, 0.25, 0), (math.inf, 0.25, bad), (0.5, -0.25, bad), (0.5, -math.inf, bad), (math.inf, math.inf, bad),
+        (math.nan, 0.25, bad), (0.5, math.nan, bad), (-0.5, -2.0, bad), (0.5, math.inf, bad), (-0.0, -0.0, 0)]
+    n = len(cases)
+    p = torch.full((3 * n, vocab), 1 / 512, device="cuda")
+    q = torch.full((2 * n, vocab), 1 / 512, device="cuda")
+    ids = torch.tensor([0, 7, 9] * n, dtype=torch.int32, device="cuda")
+    for i, (x, y, _) in enumerate(cases):
+        p[3 * i, 7], q[2 * i, 7] = x, y
+    u = torch.full((3 * n,), 0.5, device="cuda")
+    acc, nxt, status = run_verify([3] * n, ids, p, q, u, end=True)
+    assert status == [c[2] for c in cases]
+    assert [a for a, s in zip(acc, status) if s == 0] == [2, 0]
+    assert all((a, t) == (0, -1) for a, t, s in zip(acc, nxt, status) if s)
+    # the second draft's values, the first one accepted or not
+    for first, want in ((0.5, bad), (0.0, 0)):
+        p[:], q[:] = 1 / 512, 1 / 512
+        p[0::3, 7], p[1::3, 9] = first, math.inf
+        _, _, status = run_verify([3] * n, ids, p, q, u, end=True)
+        assert status == [want] * n
+    # drafts chosen outright
+    p[:] = 1 / 512
+    p[0::3, 7], p[3, 7], p[6, 7] = 0.75, math.inf, math.nan
+    _, _, status = run_verify([3] * n, ids, p, None, u, end=True)
+    assert status == [0, bad, bad] + [0] * (n - 3)
+
+
+@pytest.mark.parametrize("vocab,n", [(81_921, 300), (655_360, 80), (655_360, 1), (655_231, 3), (400_001, 150)])
+def test_verify_wide_rows_of_many_sequences(vocab, n):
+    """More tiles than a CTA's sums have room for, where the number of sequences
+    alone asks for fewer CTAs a row; weights that are exact in any order."""
+    g = gen(vocab + n)
+    p = torch.zeros((n, vocab), device="cuda")
+    at = torch.randint(0, vocab, (n, 40), generator=g, device="cuda")
+    at[:, 0], at[:, 1] = 0, vocab - 1
+    p.scatter_(1, at, torch.randint(1, 1000, at.shape, generator=g, device="cuda") / 1024.0)
+    u = torch.rand((n,), generator=g, device="cuda")
+    ids = torch.zeros(n, dtype=torch.int32, device="cuda")
+    acc, nxt, _ = run_verify([1] * n, ids, p, None, u)
+    assert acc == [0] * n
+    for i in range(n):
+        x = torch.unique(at[i]).cpu().numpy()  # ascending
+        run = np.cumsum(p[i].cpu().numpy()[x].astype(np.float64))
+        assert nxt[i] == x[np.nonzero(run > float(u[i]) * run[-1])[0][0]]
+
+
+def test_verify_dense_rows_at_the_widest():
+    g = gen(77)
+    counts, vocab = [2, 1, 3], 655_360
+    p, q = torch.softmax(2 * randn(g, 6, vocab), -1), torch.softmax(2 * randn(g, 3, vocab), -1)
+    ids = torch.randint(0, vocab, (6,), generator=g, device="cuda", dtype=torch.int32)
+    u = torch.rand((6,), generator=g, device="cuda")
+    acc, nxt, _ = run_verify(counts, ids, p, q, u)
+    assert (acc, nxt) == verify_reference(counts, ids.tolist(), p, q, u)
