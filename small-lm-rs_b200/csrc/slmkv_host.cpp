@@ -2060,14 +2060,19 @@ void build_shared_plan(const slm_ctx* c, const slm_batch* b, SharedPlan& plan) {
   }
 }
 
-// Builds and uploads the open batch's plan (once a batch: its layers share it).
+// Builds and uploads the open batch's plan (once a batch: its layers share it),
+// and sends the table entries that the kernels read: an open batch's do not change,
+// and others' that come up later are no part of its calls, which may be captured.
 slm_status shared_prepare(slm_batch* b) {
   slm_ctx* c = b->ctx;
-  // Planning waits for the slot's last upload, and the plan is one batch's.
+  // Planning waits for the slot's last upload, and the plan is one batch's; a
+  // refused call must leave nothing in the graph.
   cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
   CU(c, cudaStreamIsCapturing(b->stream, &capture));
   if (capture != cudaStreamCaptureStatusNone)
     return input_error(c, SLM_ERR_INVALID_INPUT, "shared prefix attention", "a batch's first call cannot be captured");
+  const slm_status sent = flush_excess(c, b->stream, 0, 0);
+  if (sent) return sent;
   if (!c->have_maps) {
     const slm_status rc = make_pool_maps(c);
     if (rc) return rc;
@@ -2180,8 +2185,6 @@ slm_status slm_batch_shared_attention(slm_batch* b, int32_t layer, const float* 
   const size_t bytes = static_cast<size_t>(b->total_tokens) * ctx->cfg.num_query_heads * kHeadDim * sizeof(float);
   if (ranges_overlap(d_query, bytes, d_out, bytes))
     return input_error(ctx, SLM_ERR_INVALID_INPUT, what, "the output may not overlap the query");
-  rc = flush_excess(ctx, b->stream, 0, 0);  // the kernels read the device block table
-  if (rc) return rc;
   if (!b->shared_ready && (rc = shared_prepare(b))) return rc;
   SharedAttentionLaunch& p = b->shared;
   p.layer = layer;

@@ -83,3 +83,79 @@ def test_verify_dense_rows_at_the_widest():
     u = torch.rand((6,), generator=g, device="cuda")
     acc, nxt, _ = run_verify(counts, ids, p, q, u)
     assert (acc, nxt) == verify_reference(counts, ids.tolist(), p, q, u)
+
+
+# ---- calls under capture -------------------------------------------------------------
+
+
+def one_layer_pool(hq=4, hkv=2, seqs=3, context=128):
+    pool = slmkv.KvPool(num_layers=1, num_query_heads=hq, num_key_value_heads=hkv, context_length=context,
+                        num_blocks=40, max_sequences=seqs)
+    pool.shuffle(3)
+    return pool
+
+
+def test_a_first_call_refused_under_capture_leaves_nothing_in_the_graph():
+    """A decode step leaves its new block's table entry to the next call that
+    reads the table: a refused call must not put it into a graph that is dropped."""
+    g = gen(31)
+    pool = one_layer_pool()
+    cache = pool.allocate_kv_cache(128)
+    k, v = randn(g, 16, 2, D), randn(g, 16, 2, D)
+    cache.append_layer(0, k, v, 16)
+    assert cache.blocks() != [0]
+    q, nk, nv = randn(g, 1, 4, D), randn(g, 1, 2, D), randn(g, 1, 2, D)
+    want, out = torch.empty_like(q), torch.empty_like(q)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        b = pool.begin([cache], 1)
+        assert 0 not in cache.blocks()  # (an entry that was never written is 0)
+        b.decode_layer(0, q, nk, nv, want)
+        graph = torch.cuda.CUDAGraph()
+        before = pool.launch_count()
+        with torch.cuda.graph(graph, stream=stream):
+            torch.ones(1, device="cuda")  # (a graph of something)
+            with pytest.raises(slmkv.InvalidInput, match="captured"):
+                b.shared_prefix_attention(0, q, out)
+        assert pool.launch_count() == before
+        del graph
+        gc.collect()
+        b.shared_prefix_attention(0, q, out)
+        b.end()
+    # both are f32 means of 17 values of N(0, 1)
+    assert (out - want).abs().max().item() <= 2e-5
+
+
+def test_a_captured_call_takes_no_other_sequences_table_entries():
+    """Blocks that another sequence got meanwhile are no part of the graph: it
+    may be dropped, or replayed when they are another's."""
+    g = gen(32)
+    pool = one_layer_pool()
+    a, c, d = (pool.allocate_kv_cache(128) for _ in range(3))
+    tokens = list(range(32))
+    k, v = randn(g, 32, 2, D), randn(g, 32, 2, D)
+    a.append_layer(0, k, v, 32)
+    a.publish_prefix(tokens)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    q, nk, nv = randn(g, 2, 4, D), randn(g, 2, 2, D), randn(g, 2, 2, D)
+    out = torch.empty_like(q)
+    with torch.cuda.stream(stream):
+        b = pool.begin([a], 2)
+        b.append_layer(0, nk, nv)
+        b.shared_prefix_attention(0, q, out)
+        assert c.attach_prefix(tokens) == 32  # its table entries wait for a call that reads them
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            b.shared_prefix_attention(0, q, out)
+        del graph
+        gc.collect()
+        b.end()
+        assert 0 not in c.blocks()
+        again = torch.empty_like(q)
+        with pool.begin([c], 2) as b:
+            b.append_layer(0, nk, nv)
+            b.shared_prefix_attention(0, q, again)
+    stream.synchronize()
+    assert torch.equal(out, again)  # the same tokens, read alike
