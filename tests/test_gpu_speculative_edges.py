@@ -21,6 +21,48 @@ from test_gpu_speculative_step import (D, check_probabilities, gen, randn, rows_
                                        verify_reference)
 
 
+# ---- token probabilities ---------------------------------------------------------
+
+
+@pytest.mark.parametrize("vocab", [458_745, 458_752, 458_753, 458_761, 500_003, 1_000_001])
+@pytest.mark.parametrize("rows,start", [(1, 0), (3, 1)])
+def test_probabilities_of_rows_beyond_shared_memory(vocab, rows, start):
+    g = gen(vocab)
+    pool, b = rows_batch([1] * rows)
+    wide = 3 * randn(g, rows, vocab + 3)
+    wide[torch.rand(wide.shape, generator=g, device="cuda") < 0.2] = -math.inf
+    wide[:, vocab // 2] = 0.5
+    t = torch.tensor([1.0, 0.0, 0.25], device="cuda")[:rows]
+    x = wide[:, start:start + vocab]
+    out = torch.full((rows, vocab), math.nan, device="cuda")
+    b.token_probabilities(x, out, t)
+    check_probabilities(out, x, t)
+    here = x.clone()
+    b.token_probabilities(here, here, t)  # in place
+    check_probabilities(here, x, t)
+    x[0, vocab - 1] = math.nan
+    b.token_probabilities(x, out, t)
+    assert not out[0].any() and (rows == 1 or out[1:].sum(1).sub(1).abs().max() < 1e-4)
+    b.rollback()
+
+
+@pytest.mark.parametrize("vocab", [300_001, 2**24 + 3])
+def test_probabilities_of_many_equal_weights(vocab):
+    """A sum of equal weights that are no power of two: each addition is rounded
+    the same way, so a long chain of them in 32 bits would drift."""
+    pool, b = rows_batch([1])
+    x = torch.full((1, vocab), -0.3, device="cuda")
+    x[0, 5] = 0.0
+    b.token_probabilities(x, x)
+    w = math.exp(float(np.float32(-0.3)))
+    want = w / (1 + (vocab - 1) * w)
+    # as check_probabilities: two roundings of an exponent of 0.43, a few of 2^-22
+    tol = want * (2 * 2.0**-24 + 8 * 2.0**-22)
+    assert abs(x[0, 0].item() - want) <= tol and abs(x[0, -1].item() - want) <= tol
+    assert abs(x[0, 5].item() - want / w) <= tol / w
+    b.rollback()
+
+
 # ---- verification ------------------------------------------------------------------
 
 
