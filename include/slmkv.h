@@ -262,9 +262,9 @@ slm_status slm_batch_append_layer_normed(slm_batch* batch, int32_t layer, const 
  * softmax weight to 2^-22, or so that its part of the output is off by 2^-38 of
  * the largest that the row has: a weight times the largest value of its block;
  * numbers below 2^-117 to 2^-134; the sum of a row's values, weighted relative
- * to its largest score, has to stay in f32's range). Same arguments; 16-byte aligned buffers that
- * do not overlap. Meant for few new tokens a sequence: long prompts run faster
- * through slm_batch_prefill_attention. A batch's first call plans it for all
+ * to its largest score, has to stay in f32's range). Same arguments; 16-byte
+ * aligned buffers that do not overlap. Meant for few new tokens a sequence: long
+ * prompts run faster through slm_batch_prefill_attention. A batch's first call plans it for all
  * layers; plan buffers and the joined parts' scratch are allocated by the
  * context's first such calls and grow when one needs more (which waits for the
  * device). A batch's first call is refused while its stream is being captured
@@ -276,12 +276,12 @@ slm_status slm_batch_shared_attention(slm_batch* batch, int32_t layer, const flo
  * T = 0 one at the first maximal logit (greedy.rs), zero elsewhere. d_logits:
  * `rows` rows of vocab_size f32, logits_stride values apart; rows is the batch's
  * number of tokens (slm_model_score) or of sequences (slm_model_prefill,
- * slm_model_decode). d_temperatures: [rows], or NULL for 1. d_probabilities:
- * [rows, vocab_size], dense; it may be d_logits when those are dense. vocab_size
- * up to 2^30. A logit of
- * -inf is a masked token. A row with a NaN or +inf logit, with nothing but -inf,
- * or with a temperature that is negative or not finite becomes zeros and its
- * sequence fails with SLM_ERR_NON_FINITE when the batch ends. */
+ * slm_model_decode). d_temperatures: [rows], or NULL for 1; one above 0 and below
+ * 2^-126 counts as that. d_probabilities: [rows, vocab_size], dense; it may be
+ * d_logits when those are dense. vocab_size up to 2^30. A logit of -inf is a masked
+ * token. A row with a NaN or +inf logit, with nothing but -inf, or with a
+ * temperature that is negative or not finite becomes zeros and its sequence fails
+ * with SLM_ERR_NON_FINITE when the batch ends. */
 slm_status slm_batch_token_probabilities(slm_batch* batch, const float* d_logits, int32_t rows,
                                          int32_t vocab_size, int64_t logits_stride,
                                          const float* d_temperatures, float* d_probabilities);

@@ -115,6 +115,11 @@ __global__ void __launch_bounds__(kProbThreads, 4) probabilities_kernel(const Pr
   };
   const float4* x4 = reinterpret_cast<const float4*>(x - shift);
   float4* y4 = reinterpret_cast<float4*>(y - shift);  // (whole lines of y where `lines` holds)
+  // Two logits may differ by more than f32 holds, which a temperature near f32's end
+  // makes a small number again (below 2^100 the power is 0): there all that follows
+  // is of halves.
+  const float t = p.temperatures ? p.temperatures[row] : 1.f;
+  const float h = t > 0x1p100f ? 0.5f : 1.f;
   if constexpr (KEEP) {
     for_lines([&](int i, auto whole) {
       if constexpr (decltype(whole)::value)
@@ -127,11 +132,15 @@ __global__ void __launch_bounds__(kProbThreads, 4) probabilities_kernel(const Pr
     });
     asm volatile("cp.async.wait_all;" ::: "memory");
   }
+  auto times = [](const float4& a, float s) { return make_float4(a.x * s, a.y * s, a.z * s, a.w * s); };
   auto load = [&](int i, auto whole) -> float4 {
     if constexpr (KEEP) return kept[i - begin];
-    else if constexpr (decltype(whole)::value) return x4[i];
-    else return edge(i);
+    else if constexpr (decltype(whole)::value) return times(x4[i], h);
+    else return times(edge(i), h);
   };
+  if constexpr (KEEP) {
+    if (h != 1.f) for_lines([&](int i, auto) { kept[i - begin] = times(kept[i - begin], h); });
+  }
   auto store = [&](int i, auto whole, float4 v) {
     if (decltype(whole)::value && lines) {
       y4[i] = v;
@@ -143,7 +152,6 @@ __global__ void __launch_bounds__(kProbThreads, 4) probabilities_kernel(const Pr
     if (e + 2 >= 0 && e + 2 < V) y[e + 2] = v.z;
     if (e + 3 >= 0 && e + 3 < V) y[e + 3] = v.w;
   };
-  const float t = p.temperatures ? p.temperatures[row] : 1.f;
   float m = -INFINITY;  // NaN once a value is not a number
   for_lines([&](int i, auto whole) {
     const float4 a = load(i, whole);
@@ -152,8 +160,9 @@ __global__ void __launch_bounds__(kProbThreads, 4) probabilities_kernel(const Pr
   int bad = !(t >= 0.f && t <= FLT_MAX) | !(m <= FLT_MAX);  // or a value is +inf
   m = block_reduce<float, kProbThreads>(m, red_max, [](float a, float b) { return fmaxf(a, b); });
   const float base = m == -INFINITY ? 0.f : m;
-  // the least T whose reciprocal is in range keeps 0 * c = 0 at the maximum
-  const float c = t > 0.f ? fminf(kLog2e / t, FLT_MAX) : 0.f;
+  // (a temperature below the normal numbers counts as the least of them, whose
+  // reciprocal is in range)
+  const float c = t > 0.f ? kLog2e / fmaxf(t * h, FLT_MIN) : 0.f;
   const uint64_t base2 = pack2(-base, -base), c2 = pack2(c, c);
   struct Line {
     uint64_t xy, zw;

@@ -25,14 +25,14 @@ from test_gpu_speculative_step import (D, check_probabilities, gen, randn, rows_
 
 
 @pytest.mark.parametrize("vocab", [458_745, 458_752, 458_753, 458_761, 500_003, 1_000_001])
-@pytest.mark.parametrize("rows,start", [(1, 0), (3, 1)])
+@pytest.mark.parametrize("rows,start", [(1, 0), (4, 1)])
 def test_probabilities_of_rows_beyond_shared_memory(vocab, rows, start):
     g = gen(vocab)
     pool, b = rows_batch([1] * rows)
     wide = 3 * randn(g, rows, vocab + 3)
     wide[torch.rand(wide.shape, generator=g, device="cuda") < 0.2] = -math.inf
     wide[:, vocab // 2] = 0.5
-    t = torch.tensor([1.0, 0.0, 0.25], device="cuda")[:rows]
+    t = torch.tensor([1.0, 0.0, 0.25, 3e38], device="cuda")[:rows]
     x = wide[:, start:start + vocab]
     out = torch.full((rows, vocab), math.nan, device="cuda")
     b.token_probabilities(x, out, t)
@@ -60,6 +60,38 @@ def test_probabilities_of_many_equal_weights(vocab):
     tol = want * (2 * 2.0**-24 + 8 * 2.0**-22)
     assert abs(x[0, 0].item() - want) <= tol and abs(x[0, -1].item() - want) <= tol
     assert abs(x[0, 5].item() - want / w) <= tol / w
+    b.rollback()
+
+
+def test_probabilities_at_temperatures_near_the_ends_of_f32():
+    """Logits at f32's ends differ by more than f32 holds, and a temperature as
+    large makes that difference a small number again."""
+    top = torch.finfo(torch.float32).max
+    t = torch.tensor([1e38, 3e38, top, 1e37, 2.0**100, 1.0, 2.0**-126, 1e-37, 4.0], device="cuda")
+    pool, b = rows_batch([1] * len(t))
+    x = torch.full((len(t), 41), -3e38, device="cuda")
+    x[:, 3], x[:, 4], x[:, 5], x[:, 6] = 3e38, 2.9e38, -top, top
+    x[6] = torch.linspace(0, 40, 41, device="cuda") * 2.0**-126
+    x[7] = torch.linspace(-20, 20, 41, device="cuda") * 1e-37
+    x[8] = torch.linspace(-60, 60, 41, device="cuda")
+    out = torch.empty_like(x)
+    b.token_probabilities(x, out, t)
+    check_probabilities(out, x, t)
+    big = x.repeat(1, 400)  # a cluster a row, some slices without the maximum
+    big[:, 41:] = torch.minimum(big[:, 41:], big[:, :1])
+    out = torch.empty_like(big)
+    b.token_probabilities(big, out, t)
+    check_probabilities(out, big, t)
+    b.rollback()
+
+
+def test_temperatures_below_the_normal_numbers_count_as_the_least_normal_one():
+    pool, b = rows_batch([1] * 3)
+    x = (torch.arange(12, device="cuda") * 2.0**-127).repeat(3, 1)
+    out = torch.empty_like(x)
+    b.token_probabilities(x, out, torch.tensor([1e-45, 1e-40, 2.0**-126], device="cuda"))
+    assert torch.equal(out[0], out[2]) and torch.equal(out[1], out[2])
+    check_probabilities(out, x, torch.full((3,), 2.0**-126, device="cuda"))
     b.rollback()
 
 
