@@ -759,8 +759,9 @@ __global__ void __launch_bounds__(kThreads, 2) shared_tc_kernel(const __grid_con
         if (j + 2 < n_tiles && !(ok = wait(Cfg::kBarODone, j & 1) && scores(j + 2))) break;
       }
       if (!ok) raise();
-      // every product completes before TMEM is released
-      if (lane == 0) mma_commit(bar(Cfg::kBarDrain));
+      // every product completes before TMEM is released (a commit covers the
+      // products of the thread that makes it)
+      if (one) mma_commit(bar(Cfg::kBarDrain));
       bar_wait(bar(Cfg::kBarDrain), 0, 0);
       __syncwarp();
     }
