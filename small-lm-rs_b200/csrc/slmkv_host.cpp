@@ -227,9 +227,7 @@ struct slm_ctx {
     float* part_acc = nullptr;  // and behind them part_ml
     float2* part_ml = nullptr;
     size_t part_cap = 0;  // row slots
-    // The batch that used the parts last: its descriptor slot and stream.
-    int32_t last_slot = -1;
-    cudaStream_t last_stream = nullptr;
+    int32_t last_slot = -1;  // the descriptor slot of the batch that used the parts last
   } shared;
   size_t upd_cap = 0, copy_cap = 0;
 
@@ -2140,11 +2138,10 @@ slm_status shared_prepare(slm_batch* b) {
   put(o_merge, plan.merge);
   // the kernels that last read the slot's device buffer are done
   CU(c, cudaStreamWaitEvent(b->stream, c->up_batch.consumed[k], 0));
-  // and so are those that last used the parts, of a batch on another stream too
-  if (io.last_slot >= 0 && io.last_stream != b->stream)
-    CU(c, cudaStreamWaitEvent(b->stream, c->up_batch.consumed[io.last_slot], 0));
+  // and so are those that last used the parts, on whatever stream (a stream's handle
+  // may be another's that was destroyed with its kernels still running)
+  if (io.last_slot >= 0) CU(c, cudaStreamWaitEvent(b->stream, c->up_batch.consumed[io.last_slot], 0));
   io.last_slot = k;
-  io.last_stream = b->stream;
   CU(c, cudaMemcpyAsync(io.d[k], h, bytes, cudaMemcpyHostToDevice, b->stream));
   CU(c, cudaEventRecord(io.copied[k], b->stream));
   SharedAttentionLaunch& p = b->shared;

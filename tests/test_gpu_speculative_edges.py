@@ -233,3 +233,39 @@ def test_a_captured_call_takes_no_other_sequences_table_entries():
             b.shared_prefix_attention(0, q, again)
     stream.synchronize()
     assert torch.equal(out, again)  # the same tokens, read alike
+
+
+# ---- streams -------------------------------------------------------------------------
+
+
+def test_batches_on_streams_that_come_and_go():
+    """Each step on a stream of its own, destroyed while its kernels may run;
+    the joined parts' scratch passes from one to the next."""
+    import ctypes
+
+    cudart = ctypes.CDLL("libcudart.so.12")
+    g = gen(33)
+    pool = slmkv.KvPool(num_layers=1, num_query_heads=8, num_key_value_heads=2, context_length=1100, num_blocks=400,
+                        max_sequences=64)
+    caches = [pool.allocate_kv_cache(1100) for _ in range(64)]
+    k, v = randn(g, 1024, 2, D), randn(g, 1024, 2, D)
+    caches[0].append_layer(0, k, v, 1024)
+    caches[0].publish_prefix([1] * 1024)
+    for c in caches[1:]:
+        c.attach_prefix([1] * 1024)
+    q, nk, nv = randn(g, 64, 8, D), randn(g, 64, 2, D), randn(g, 64, 2, D)
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(12):
+        h = ctypes.c_void_p()
+        assert cudart.cudaStreamCreateWithFlags(ctypes.byref(h), 1) == 0
+        out = torch.empty_like(q)
+        torch.cuda.synchronize()
+        b = pool.begin(caches, 1, stream=torch.cuda.ExternalStream(h.value))
+        b.append_layer(0, nk, nv)
+        b.shared_prefix_attention(0, q, out)
+        b.rollback()
+        assert cudart.cudaStreamDestroy(h) == 0
+        outs.append(out)
+    torch.cuda.synchronize()
+    assert all(torch.equal(outs[0], o) for o in outs[1:])
