@@ -1440,6 +1440,8 @@ slm_status slm_batch_begin(slm_ctx* ctx, int32_t n, const int32_t* h_seq_ids,
     return rc;
   }
   b->layer_done.assign(ctx->cfg.num_layers, 0);
+  b->poison_base.assign(n, -1);  // (a submitted batch may fail while this one is open)
+  b->poison_code.assign(n, 0);
   ctx->open_batch = b.get();
   *out = b.release();
   return SLM_OK;
@@ -2402,11 +2404,11 @@ namespace {
 void roll_back_seq(slm_ctx* ctx, const slm_batch* from, int32_t id, int32_t target, int32_t code) {
   Seq& q = ctx->seqs[id];
   for (auto& v : q.layer_len) v = std::min(v, target);
-  release_tail(ctx, id, blocks_for(seq_max_len(q)));
-  bool later = false;
+  bool later = false, held = false;
   auto poison = [&](slm_batch* m) {
     for (size_t j = 0; j < m->seq_ids.size(); ++j)
       if (m->seq_ids[j] == id) {
+        held = true;
         if (m->poison_base[j] < 0 || target < m->poison_base[j]) m->poison_base[j] = target;
         if (!m->poison_code[j]) m->poison_code[j] = code;
       }
@@ -2419,16 +2421,20 @@ void roll_back_seq(slm_ctx* ctx, const slm_batch* from, int32_t id, int32_t targ
     if (later && !m->resolved) poison(m);
   }
   if (ctx->open_batch && ctx->open_batch != from) poison(ctx->open_batch);
+  // A later batch still writes to the blocks it was planned on: they are kept
+  // until its own end, which rolls back as far.
+  if (!held) release_tail(ctx, id, blocks_for(seq_max_len(q)));
 }
 
 // Drops an open batch (slm_batch_rollback, or a failed submit): every
-// sequence back to its begin length.
+// sequence back to its begin length, or an earlier batch's where that failed.
 void batch_discard(slm_batch* b) {
   slm_ctx* ctx = b->ctx;
   if (has_device(ctx)) cudaEventRecord(ctx->up_batch.consumed[b->up_slot], b->stream);
   for (size_t i = 0; i < b->seq_ids.size(); ++i) {
     ctx->seqs[b->seq_ids[i]].in_batch = false;
-    roll_back_seq(ctx, b, b->seq_ids[i], b->base[i], SLM_ERR_INVALID_INPUT);
+    const int32_t target = b->poison_base[i] < 0 ? b->base[i] : std::min(b->base[i], b->poison_base[i]);
+    roll_back_seq(ctx, b, b->seq_ids[i], target, SLM_ERR_INVALID_INPUT);
   }
   ctx->open_batch = nullptr;
   delete b;
@@ -2551,8 +2557,6 @@ slm_status submit(slm_batch* b, bool extra_slot) {
                     : cuda_fail(ctx, e, "slm_batch_submit");
   }
   b->complete.assign(n, 1);
-  b->poison_base.assign(n, -1);
-  b->poison_code.assign(n, 0);
   for (size_t i = 0; i < n; ++i) {
     Seq& q = ctx->seqs[b->seq_ids[i]];
     const int32_t want = b->base[i] + b->counts[i];
