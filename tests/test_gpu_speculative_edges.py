@@ -269,3 +269,54 @@ def test_batches_on_streams_that_come_and_go():
         outs.append(out)
     torch.cuda.synchronize()
     assert all(torch.equal(outs[0], o) for o in outs[1:])
+
+
+# ---- the model's scores ----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("kv_dtype", [slmkv.KV_F32, slmkv.KV_BF16])
+@pytest.mark.parametrize("exact_rows,lengths", [
+    (1024, [5, 1, 33]),            # the exact-order kernels
+    (0, [5, 1, 33]),               # this library's row GEMMs, the split head
+    (0, [17, 64, 100, 250]),       # the same, more rows than one tile
+    (0, [200, 120, 1, 255]),       # cuBLAS, as many vocabulary rows
+    (16, [1, 3, 7])])
+def test_model_scores_of_every_row_on_each_projection_path(exact_rows, lengths, kv_dtype):
+    """Every position's logits against the oracle's, by the thresholds that the
+    model's other steps are held to on that path."""
+    vocab, hq, hkv, inter, layers, ctx = 1024, 4, 2, 704, 2, 256
+    hidden = hq * D
+    tensors = random_model(7, vocab, hidden, hkv, inter, layers, scale=0.8 / np.sqrt(hidden))
+    omodel = O.Model(dict(vocab_size=vocab, hidden_size=hidden, intermediate_size=inter, num_layers=layers,
+                          num_query_heads=hq, num_key_value_heads=hkv, head_dimension=D, rms_norm_epsilon=1e-5,
+                          rope_theta=10000.0, situ_beta_gate=4.0, situ_beta_up=25.0), tensors)
+    pool = slmkv.KvPool(num_layers=layers, num_query_heads=hq, num_key_value_heads=hkv, context_length=ctx,
+                        num_blocks=len(lengths) * (ctx // 16 + 1), max_sequences=len(lengths), kv_dtype=kv_dtype)
+    pool.shuffle(5)
+    model = slmkv.Model(pool, vocab_size=vocab, intermediate_size=inter, tensors=tensors)
+    model.set_exact_rows(exact_rows)
+    rng = np.random.default_rng(sum(lengths))
+    prompts = [rng.integers(0, vocab, n).astype(np.uint32) for n in lengths]
+    ref = np.concatenate([omodel.prefill(omodel.new_cache(ctx, quantize_bf16=kv_dtype == slmkv.KV_BF16), p,
+                                         O.max_threads()) for p in prompts])
+    t = sum(lengths)
+    logits = torch.full((t, vocab), math.nan, device="cuda")
+    nxt = torch.empty(t, dtype=torch.int32, device="cuda")
+    caches = [pool.allocate_kv_cache(ctx) for _ in lengths]
+    with pool.begin(caches, lengths) as b:
+        model.score(b, torch.from_numpy(np.concatenate(prompts).astype(np.int32)).cuda(), logits, nxt)
+    assert torch.equal(nxt.long(), logits.argmax(1))
+    m = parity_metrics(logits.cpu().numpy(), ref)
+    # (top1 of hundreds of rows may meet near ties: held by the errors instead)
+    assert m["max_abs"] <= 0.1 and m["mean_abs"] <= 0.01 and m["rms"] <= 0.02 and m["cosine"] >= 0.9999, m
+    if t <= exact_rows and kv_dtype == slmkv.KV_F32:
+        assert m["max_abs"] <= 1e-4, m  # (a bf16 pool holds keys and values to 2^-9 that the oracle's prompts do not round)
+    last = np.cumsum(lengths) - 1
+    one = torch.empty((len(lengths), vocab), device="cuda")
+    pool.truncate_many(caches, [0] * len(lengths))
+    with pool.begin(caches, lengths) as b:
+        model.prefill(b, torch.from_numpy(np.concatenate(prompts).astype(np.int32)).cuda(), one)
+    # the same layers; the vocabulary projection of other row counts sums in
+    # another order, or over split operands: 2^-14 of |x| |w| = 16 * 0.8 at most
+    assert (one - logits[torch.from_numpy(last).cuda()]).abs().max().item() <= 16 * 0.8 * 1.3 * 2.0**-14
+    model.close()
