@@ -727,8 +727,8 @@ class Batch:
         strides = ((query.stride(0), keys.stride(0), values.stride(0)) if t > 1 else
                    (q_shape[1] * width, k_shape[1] * width, k_shape[1] * width))
         rc = _fast.append_normed(
-            self._h, layer, *ins, *strides, self._tensor("query_norm", query_norm, (width,)),
-            self._tensor("key_norm", key_norm, (width,)), epsilon, 1 if rotate else 0,
+            self._h, int(layer), *ins, *strides, self._tensor("query_norm", query_norm, (width,)),
+            self._tensor("key_norm", key_norm, (width,)), float(epsilon), 1 if rotate else 0,
             self._tensor("query_out", query_out, q_shape))
         if rc:
             self.pool.check(rc)
@@ -738,7 +738,7 @@ class Batch:
         share cached prefixes, whose blocks are read once for all of them;
         query / out [tokens, q_heads, d]."""
         _, shape, _ = self._shapes()
-        rc = _fast.shared_attention(self._h, layer, self._tensor("query", query, shape),
+        rc = _fast.shared_attention(self._h, int(layer), self._tensor("query", query, shape),
                                     1 if rotate_query else 0, self._tensor("out", out, shape))
         if rc:
             self.pool.check(rc)

@@ -320,3 +320,21 @@ def test_model_scores_of_every_row_on_each_projection_path(exact_rows, lengths, 
     # another order, or over split operands: 2^-14 of |x| |w| = 16 * 0.8 at most
     assert (one - logits[torch.from_numpy(last).cuda()]).abs().max().item() <= 16 * 0.8 * 1.3 * 2.0**-14
     model.close()
+
+
+# ---- Python arguments ------------------------------------------------------------------
+
+
+def test_layers_and_epsilon_of_numpy_types_are_taken():
+    """As the batch's other calls take them."""
+    g = gen(34)
+    pool = slmkv.KvPool(num_layers=2, num_query_heads=4, num_key_value_heads=2, context_length=64, num_blocks=8,
+                        max_sequences=1)
+    cache = pool.allocate_kv_cache(64)
+    q, k, v, w = randn(g, 2, 4, D), randn(g, 2, 2, D), randn(g, 2, 2, D), torch.ones(D, device="cuda")
+    outs = [[torch.empty_like(q) for _ in range(2)] for _ in range(2)]
+    with pool.begin([cache], 2) as b:
+        for layer, i in ((0, 0), (np.int64(1), 1)):
+            b.append_layer_normed(layer, q, k, v, w, w, outs[i][0], epsilon=np.float32(1e-5) if i else 1e-5)
+            b.shared_prefix_attention(layer, outs[i][0], outs[i][1], rotate_query=False)
+    assert all(torch.equal(a, c) for a, c in zip(*outs))
