@@ -57,8 +57,9 @@ __device__ __forceinline__ T block_reduce(T v, T* scratch, Op op) {
 // 2^24 were 3e-6 off).
 //
 // Every thread copies, and reads back, its own 16-byte lines, so the copies need
-// no barrier; slices of up to 56 KiB leave four CTAs an SM, one's copies under
-// another's arithmetic. 320 rows of 100003: 55 us, 4.6 TB/s. What is missing to a
+// no barrier; slices of up to 56 KiB leave four CTAs an SM (three in the last 256
+// bytes, still ahead of twice the CTAs: 1184 rows of 14300 in 28.7 us, 32.8), one's
+// copies under another's arithmetic. 320 rows of 100003: 55.6 us, 4.6 TB/s. What is missing to a
 // copy's 6.5 is the last, partly filled wave and the CTAs' own chain of copy,
 // maximum, sum, exchange and write. (Slices in registers, 8 lines a thread: 91 us at
 // two CTAs an SM; loads through registers into shared memory, fewer in flight: 69;
@@ -493,8 +494,8 @@ cudaError_t launch_clusters(Kernel kernel, const Launch& p, int rows, int thread
 
 cudaError_t launch_probabilities(const ProbabilitiesLaunch& p0, cudaStream_t s) {
   ProbabilitiesLaunch p = p0;
-  // The fewest CTAs a row whose slices are small enough for four CTAs an SM (up
-  // to 3 values of a first line lie outside the row); more while the SMs are not
+  // The fewest CTAs a row whose slices are small enough for four (or three) CTAs an
+  // SM (up to 3 values of a first line lie outside the row); more while the SMs are not
   // filled and a thread keeps two lines.
   const int64_t lines = (static_cast<int64_t>(p.vocab) + 6) / 4;
   auto per = [&](int c) { return (lines + c - 1) / c; };
