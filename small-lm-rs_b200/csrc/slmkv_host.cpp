@@ -506,6 +506,19 @@ DescLayout desc_layout(size_t n, size_t n_pairs, size_t n_chunks, size_t n_warps
   return L;
 }
 
+// The first nu pending table updates, as they go to the device: an entry may be
+// pending more than once (a block attached and then copied on write, or given back
+// and replaced, or of a slot that changed hands), and all writes of it run at once,
+// so each carries the entry's block of now.
+void put_updates(const slm_ctx* c, uint8_t* at, size_t nu) {
+  TableUpdate* to = reinterpret_cast<TableUpdate*>(at);
+  for (size_t i = 0; i < nu; ++i) {
+    to[i] = c->pending_updates[i];
+    const std::vector<int32_t>& blocks = c->seqs[to[i].slot].blocks;
+    if (static_cast<size_t>(to[i].index) < blocks.size()) to[i].block = blocks[to[i].index];
+  }
+}
+
 // Sends pending table updates / copies that would not fit into a descriptor
 // upload, through the aux region, and applies them.
 slm_status flush_excess(slm_ctx* c, cudaStream_t s, size_t keep_updates, size_t keep_copies) {
@@ -514,7 +527,7 @@ slm_status flush_excess(slm_ctx* c, cudaStream_t s, size_t keep_updates, size_t 
     const size_t nc = std::min(c->pending_copies.size(), c->copy_cap);
     DescLayout L = desc_layout(0, 0, 0, 0, nu, nc);
     uint8_t* h = upload_begin(c->up_aux);
-    memcpy(h + L.updates, c->pending_updates.data(), nu * sizeof(TableUpdate));
+    put_updates(c, h + L.updates, nu);
     memcpy(h + L.copies, c->pending_copies.data(), nc * sizeof(CopyJob));
     CU(c, upload_end(c->up_aux, L.total, s, c->copy_stream));
     c->prev_decode_layer = -1;
@@ -669,7 +682,7 @@ slm_status upload_step(slm_ctx* c, Upload& u, cudaStream_t s, const std::vector<
   if (np) memcpy(h + L.pairs, plan->pairs.data(), sizeof(PairEntry) * np);
   if (nch) memcpy(h + L.chunks, plan->chunks.data(), sizeof(int32_t) * nch);
   if (nw) memcpy(h + L.wfp, plan->warp_start.data(), sizeof(int4) * 2 * nw);
-  if (nu) memcpy(h + L.updates, c->pending_updates.data(), nu * sizeof(TableUpdate));
+  put_updates(c, h + L.updates, nu);
   if (nc) memcpy(h + L.copies, c->pending_copies.data(), nc * sizeof(CopyJob));
   CU(c, upload_end(u, L.total, s, c->copy_stream));
   uint8_t* d = u.device();

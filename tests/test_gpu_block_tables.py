@@ -1,0 +1,74 @@
+"""Block tables and copied blocks when several changes of one entry, or copies
+that follow one another, are sent to the device together."""
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+slmkv = pytest.importorskip("slmkv")
+
+D = 64
+
+
+def rows(g, t, *heads):
+    return tuple(torch.randn((t, h, D), generator=g, device="cuda") for h in heads)
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_attached_then_truncated_sequences_write_to_their_copies(seed):
+    """An attached block's entry and that of the copy which a truncated sequence
+    writes to, sent at once: the copy's holds."""
+    g, n = gen(seed), 60
+    pool = slmkv.KvPool(num_layers=1, num_query_heads=4, num_key_value_heads=2, context_length=300,
+                        num_blocks=300, max_sequences=n + 1)
+    pool.shuffle(seed)
+    first = pool.allocate_kv_cache(300)
+    k, v = rows(g, 256, 2, 2)
+    first.append_layer(0, k, v, 256)
+    first.publish_prefix(list(range(256)))
+    caches = [pool.allocate_kv_cache(300) for _ in range(n)]
+    for i, c in enumerate(caches):
+        assert c.attach_prefix(list(range(256))) == 256
+        c.truncate_all(20 + 3 * i)
+    q, nk, nv = rows(g, 2 * n, 4, 2, 2)
+    out, want = torch.empty_like(q), torch.empty_like(q)
+    with pool.begin(caches, 2) as b:
+        b.append_layer(0, nk, nv, rotate_keys=False)
+        b.shared_prefix_attention(0, q, out, rotate_query=False)
+    for i, c in enumerate(caches):
+        m = 20 + 3 * i
+        assert torch.equal(c.layer_keys(0), torch.cat((k[:m], nk[2 * i:2 * i + 2])))
+        assert torch.equal(c.layer_values(0), torch.cat((v[:m], nv[2 * i:2 * i + 2])))
+    assert torch.equal(first.layer_keys(0), k)
+
+
+def test_blocks_given_back_and_replaced_between_decode_steps():
+    """Decode steps leave table entries for later: a block that was given back by
+    a truncation, its successor, and a slot's next owner are pending together."""
+    g, n = gen(9), 40
+    pool = slmkv.KvPool(num_layers=1, num_query_heads=4, num_key_value_heads=2, context_length=64, num_blocks=4 * n,
+                        max_sequences=n)
+    pool.shuffle(2)
+    caches = [pool.allocate_kv_cache(64) for _ in range(n)]
+    q, k, v = rows(g, 16 * n, 4, 2, 2)
+    with pool.begin(caches, 16) as b:
+        b.append_layer(0, k, v, rotate_keys=False)
+    out = torch.empty((n, 4, D), device="cuda")
+    for turn in range(3):  # a new block each time, in another order
+        order = caches[turn:] + caches[:turn]
+        q, nk, nv = rows(g, n, 4, 2, 2)
+        with pool.begin(order, 1) as b:
+            b.decode_layer(0, q, nk, nv, out)
+        if turn < 2:
+            pool.truncate_many(caches, [16] * n)
+    for i, c in enumerate(caches):
+        at = (i - 2) % n
+        got = c.layer_values(0)
+        assert torch.equal(got[:16], v[16 * i:16 * i + 16]) and torch.equal(got[16], nv[at]), i
