@@ -242,6 +242,8 @@ struct slm_ctx {
   uint64_t clock = 0;
   std::vector<TableUpdate> pending_updates;
   std::vector<CopyJob> pending_copies;
+  std::vector<int64_t> copy_read, copy_written;  // per block: the last launch of copies that did (scratch)
+  int64_t copy_turn = 0;
   slm_batch* open_batch = nullptr;
   StreamPlan plan;  // decode plan of the open batch (reused storage)
   SharedPlan shared_plan;  // reused storage
@@ -519,6 +521,32 @@ void put_updates(const slm_ctx* c, uint8_t* at, size_t nu) {
   }
 }
 
+// Applies nu table updates and the first nc pending copies, uploaded at `updates`
+// and `copies`. A launch copies its blocks all at once: where the pool is full, a
+// block may be copied, given up by its last sequence, evicted from the index and
+// taken as another copy's target, which then goes into a launch of its own.
+slm_status apply_pending(slm_ctx* c, const uint8_t* updates, size_t nu, const uint8_t* copies, size_t nc,
+                         cudaStream_t s) {
+  c->prev_decode_layer = -1;
+  c->copy_read.resize(c->cfg.num_blocks, 0);
+  c->copy_written.resize(c->cfg.num_blocks, 0);
+  size_t from = 0, at = 0;
+  do {
+    const int64_t turn = ++c->copy_turn;
+    for (; at < nc; ++at) {
+      const CopyJob& j = c->pending_copies[at];
+      if (c->copy_written[j.src] == turn || c->copy_written[j.dst] == turn || c->copy_read[j.dst] == turn) break;
+      c->copy_read[j.src] = c->copy_written[j.dst] = turn;
+    }
+    CU(c, launch_apply_updates(c->geom(), reinterpret_cast<const TableUpdate*>(updates),
+                               static_cast<int32_t>(from ? 0 : nu), reinterpret_cast<const CopyJob*>(copies) + from,
+                               static_cast<int32_t>(at - from), s));
+    ++c->launches;
+    from = at;
+  } while (at < nc);
+  return SLM_OK;
+}
+
 // Sends pending table updates / copies that would not fit into a descriptor
 // upload, through the aux region, and applies them.
 slm_status flush_excess(slm_ctx* c, cudaStream_t s, size_t keep_updates, size_t keep_copies) {
@@ -530,12 +558,8 @@ slm_status flush_excess(slm_ctx* c, cudaStream_t s, size_t keep_updates, size_t 
     put_updates(c, h + L.updates, nu);
     memcpy(h + L.copies, c->pending_copies.data(), nc * sizeof(CopyJob));
     CU(c, upload_end(c->up_aux, L.total, s, c->copy_stream));
-    c->prev_decode_layer = -1;
-    CU(c, launch_apply_updates(c->geom(), reinterpret_cast<TableUpdate*>(c->up_aux.d + L.updates),
-                               static_cast<int32_t>(nu),
-                               reinterpret_cast<CopyJob*>(c->up_aux.d + L.copies),
-                               static_cast<int32_t>(nc), s));
-    ++c->launches;
+    const slm_status rc = apply_pending(c, c->up_aux.d + L.updates, nu, c->up_aux.d + L.copies, nc, s);
+    if (rc) return rc;
     c->pending_updates.erase(c->pending_updates.begin(), c->pending_updates.begin() + nu);
     c->pending_copies.erase(c->pending_copies.begin(), c->pending_copies.begin() + nc);
   }
@@ -687,11 +711,7 @@ slm_status upload_step(slm_ctx* c, Upload& u, cudaStream_t s, const std::vector<
   CU(c, upload_end(u, L.total, s, c->copy_stream));
   uint8_t* d = u.device();
   if (nu || nc) {
-    c->prev_decode_layer = -1;
-    CU(c, launch_apply_updates(c->geom(), reinterpret_cast<TableUpdate*>(d + L.updates),
-                               static_cast<int32_t>(nu), reinterpret_cast<CopyJob*>(d + L.copies),
-                               static_cast<int32_t>(nc), s));
-    ++c->launches;
+    if ((rc = apply_pending(c, d + L.updates, nu, d + L.copies, nc, s))) return rc;
     if (with_table_updates) c->pending_updates.clear();
     c->pending_copies.clear();
   }

@@ -72,3 +72,34 @@ def test_blocks_given_back_and_replaced_between_decode_steps():
         at = (i - 2) % n
         got = c.layer_values(0)
         assert torch.equal(got[:16], v[16 * i:16 * i + 16]) and torch.equal(got[16], nv[at]), i
+
+
+def test_a_copys_source_that_becomes_another_copys_target():
+    """A full pool: the block that one sequence copies, and gives up, is evicted
+    from the index and taken for the other sequence's copy in the same step."""
+    g = gen(5)
+    pool = slmkv.KvPool(num_layers=2, num_query_heads=4, num_key_value_heads=2, context_length=64, num_blocks=5,
+                        max_sequences=2)
+    tokens = [list(range(32)), list(range(100, 132))]
+    kv = [[rows(g, 32, 2, 2) for _ in range(2)] for _ in tokens]
+    for t, layers in zip(tokens, kv):
+        c = pool.allocate_kv_cache(64)
+        for layer, (k, v) in enumerate(layers):
+            c.append_layer(layer, k, v, 32)
+        c.publish_prefix(t)
+        c.free()
+    caches = [pool.allocate_kv_cache(64) for _ in tokens]
+    for c, t in zip(caches, tokens):
+        assert c.attach_prefix(t) == 32
+        c.truncate_all(24)  # writes go into the second block, which is copied first
+    source = caches[0].blocks()[1]
+    assert pool.stats()[0] == 1
+    nk, nv = rows(g, 2, 2, 2)
+    with pool.begin(caches, 1) as b:
+        for layer in range(2):
+            b.append_layer(layer, nk, nv, rotate_keys=False)
+    assert caches[1].blocks()[1] == source  # the case that is meant
+    for i, c in enumerate(caches):
+        for layer in range(2):
+            assert torch.equal(c.layer_keys(layer), torch.cat((kv[i][layer][0][:24], nk[i:i + 1])))
+            assert torch.equal(c.layer_values(layer), torch.cat((kv[i][layer][1][:24], nv[i:i + 1])))
