@@ -420,16 +420,21 @@ bool reserve_positions(slm_ctx* c, int32_t slot, int32_t from, int32_t to, Undo&
 }
 
 void rollback_reserve(slm_ctx* c, Undo& undo) {
-  // Restore block lists (this re-acquires shared blocks released by COW).
-  for (auto it = undo.old_blocks.rbegin(); it != undo.old_blocks.rend(); ++it) {
-    Seq& s = c->seqs[it->first];
-    for (int32_t b : it->second)
-      if (std::find(s.blocks.begin(), s.blocks.end(), b) == s.blocks.end()) ++c->refcount[b];
-    s.blocks = it->second;
-  }
   for (int32_t b : undo.taken) {
     c->refcount[b] = 0;
     c->free_list.push_back(b);
+  }
+  // Restore block lists: this re-acquires shared blocks released by
+  // copy-on-write, also one that was evicted and taken since, maybe by the same
+  // sequence.
+  for (auto it = undo.old_blocks.rbegin(); it != undo.old_blocks.rend(); ++it) {
+    Seq& s = c->seqs[it->first];
+    for (size_t j = 0; j < it->second.size(); ++j) {
+      const int32_t b = it->second[j];
+      if (s.blocks[j] != b && c->refcount[b]++ == 0)  // (a list only grows, or has blocks replaced)
+        c->free_list.erase(std::find(c->free_list.begin(), c->free_list.end(), b));
+    }
+    s.blocks = it->second;
   }
   c->pending_updates.resize(undo.updates_mark);
   c->pending_copies.resize(undo.copies_mark);

@@ -103,3 +103,27 @@ def test_a_copys_source_that_becomes_another_copys_target():
         for layer in range(2):
             assert torch.equal(c.layer_keys(layer), torch.cat((kv[i][layer][0][:24], nk[i:i + 1])))
             assert torch.equal(c.layer_values(layer), torch.cat((kv[i][layer][1][:24], nv[i:i + 1])))
+
+
+def test_a_refused_step_gives_back_blocks_that_changed_hands_in_it():
+    """The pool runs out in the middle of a step's reservations: a sequence's
+    shared block, which it was to copy, was evicted and taken by another one. It
+    stays the first one's."""
+    g = gen(6)
+    pool = slmkv.KvPool(num_layers=1, num_query_heads=4, num_key_value_heads=2, context_length=64, num_blocks=2,
+                        max_sequences=3)
+    a, b, c = (pool.allocate_kv_cache(64) for _ in range(3))
+    k, v = rows(g, 16, 2, 2)
+    a.append_layer(0, k, v, 16)
+    a.publish_prefix(list(range(16)))
+    a.truncate_all(5)
+    held = a.blocks()
+    for step, counts in (([a, b, c], 1), ([a, b], [20, 1]), ([a], 30), ([a, b, c], 1)):
+        with pytest.raises(slmkv.InvalidInput, match="no free block"):
+            pool.begin(step, counts)
+        assert a.blocks() == held and b.blocks() == c.blocks() == [] and pool.stats()[0] == 1
+    nk, nv = rows(g, 2, 2, 2)
+    with pool.begin([b, a], 1) as step:
+        step.append_layer(0, nk, nv, rotate_keys=False)
+    assert not set(a.blocks()) & set(b.blocks()) and pool.stats()[0] == 0
+    assert torch.equal(a.layer_keys(0), torch.cat((k[:5], nk[1:]))) and torch.equal(b.layer_keys(0), nk[:1])
