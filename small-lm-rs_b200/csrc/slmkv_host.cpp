@@ -533,8 +533,6 @@ void put_updates(const slm_ctx* c, uint8_t* at, size_t nu) {
 slm_status apply_pending(slm_ctx* c, const uint8_t* updates, size_t nu, const uint8_t* copies, size_t nc,
                          cudaStream_t s) {
   c->prev_decode_layer = -1;
-  c->copy_read.resize(c->cfg.num_blocks, 0);
-  c->copy_written.resize(c->cfg.num_blocks, 0);
   size_t from = 0, at = 0;
   do {
     const int64_t turn = ++c->copy_turn;
@@ -972,6 +970,8 @@ slm_status slm_create(const slm_config* config, int32_t device, slm_ctx** out) {
   c->seqs.resize(k.max_sequences);
   for (int32_t i = k.max_sequences - 1; i >= 0; --i) c->free_slots.push_back(i);
   c->refcount.assign(k.num_blocks, 0);
+  c->copy_read.assign(k.num_blocks, 0);
+  c->copy_written.assign(k.num_blocks, 0);
   c->meta.resize(k.num_blocks);
   for (int32_t b = k.num_blocks - 1; b >= 0; --b) c->free_list.push_back(b);
   c->upd_cap = std::max<size_t>(4096, 2 * static_cast<size_t>(k.max_sequences));
