@@ -268,7 +268,8 @@ slm_status slm_batch_append_layer_normed(slm_batch* batch, int32_t layer, const 
  * layers; plan buffers and the joined parts' scratch are allocated by the
  * context's first such calls and grow when one needs more (which waits for the
  * device). A batch's first call is refused while its stream is being captured
- * into a graph; a captured later one may be replayed until the batch ends. */
+ * into a graph; a captured later one may be replayed until the batch ends or is
+ * submitted, in the order of its stream (a context's calls share that scratch). */
 slm_status slm_batch_shared_attention(slm_batch* batch, int32_t layer, const float* d_query,
                                       int32_t rotate_query, float* d_out);
 /* Probabilities of logit rows (no reference counterpart: greedy.rs takes the

@@ -59,9 +59,9 @@ __device__ __forceinline__ T block_reduce(T v, T* scratch, Op op) {
 // Every thread copies, and reads back, its own 16-byte lines, so the copies need
 // no barrier; slices of up to 56 KiB leave four CTAs an SM (three in the last 256
 // bytes, still ahead of twice the CTAs: 1184 rows of 14300 in 28.7 us, 32.8), one's
-// copies under another's arithmetic. 320 rows of 100003: 55.6 us, 4.6 TB/s. What is missing to a
-// copy's 6.5 is the last, partly filled wave and the CTAs' own chain of copy,
-// maximum, sum, exchange and write. (Slices in registers, 8 lines a thread: 91 us at
+// copies under another's arithmetic. 320 rows of 100003: 55.6 us, 4.6 TB/s. What is
+// missing to a copy's 6.5 is the last, partly filled wave and the CTAs' own chain of
+// copy, maximum, sum, exchange and write. (Slices in registers, 8 lines a thread: 91 us at
 // two CTAs an SM; loads through registers into shared memory, fewer in flight: 69;
 // one bulk copy a slice: 58; slices of 112 KiB, two CTAs: 62; clusters of 16 with 27
 // KiB: 59; persistent CTAs: 99.) 64 rows of 8192: 4 us, latency. Rows may start anywhere
@@ -268,8 +268,9 @@ __global__ void __launch_bounds__(kProbThreads, 4) probabilities_kernel(const Pr
 // tile among the sums and reads that tile again. One sequence at 32003 tokens: 5.5
 // us, of which reading and summing 1.6 (each step of a 64-bit sum across a warp is
 // about 150 cycles), the two dependent reads before 1.0, the exchange 0.5, the
-// border 1.2; 64 sequences of 4 drafts at 8192: 5.7 us. (One CTA a row: 42 us at
-// 32003 tokens. Every tile summed by its own five steps: 6.1, and 9.8 with eight CTAs a row.)
+// border 1.2; 64 sequences of 4 drafts at 8192: 5.7 us. 64 registers for four CTAs an
+// SM, 88 bytes spilled. (One CTA a row: 42 us at 32003 tokens. Every tile summed by
+// its own five steps: 6.1, and 9.8 with eight CTAs a row.)
 // ---------------------------------------------------------------------------
 constexpr int kVerifyThreads = 256;
 constexpr int kTile = 128;  // consecutive values a warp sums

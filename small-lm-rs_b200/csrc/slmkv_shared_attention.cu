@@ -126,7 +126,8 @@ __device__ __forceinline__ SharedItem load_item(const SharedItem* p) {
 // latency of a step's chain of products, maximum and powers after that: 128 rows'
 // own 256 tokens of 8 heads (68 MB) take 15 us, 4.5 TB/s, and their start 2 more.
 // 168 registers a thread, three CTAs an SM (128 and four: 23 -> 30 us for these and
-// their joining).
+// their joining); bf16 spills 24 to 40 bytes of them, f32 8 with eight query heads a
+// key head.
 template <int BF16, int G>
 __global__ void __launch_bounds__(kThreads, 3) shared_rows_kernel(const __grid_constant__ SharedAttentionLaunch p) {
   using Cfg = RowsCfg<BF16>;
@@ -493,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, 3) shared_rows_kernel(const __grid_c
 // from its own up to the root; a warp takes 32 of them at a time, lane l the
 // maximum and sum of the l-th, and values 2l and 2l + 1 of all. The plan is read
 // while the kernels before finish; what is left then is one round of reads for up
-// to 8 W parts.
+// to 8 W parts. 48 registers for five CTAs an SM, with about 55 bytes spilled.
 constexpr int kMergeThreads = 256;
 constexpr int kMergeDepth = 4;  // edges whose units are read ahead
 template <int W>

@@ -19,8 +19,7 @@
 //                 makes the largest product of the row's weights and a block's
 //                 values one unit
 // (an f32 value more than 2^17 below the largest one, or such a weight's product, keeps
-// 2^-40 of that instead). So
-// O takes two products a tile with bf16 values and S three; f32 pools take three
+// 2^-40 of that instead). So O takes two products a tile with bf16 values and S three; f32 pools take three
 // each (lo times lo, below 2^-22 of a term, is left out). With three bf16 parts for
 // everything it were three and three, six and six, and 96 columns of P. All of Q
 // but its lo part lies in TMEM: a product takes 34 cycles from there, 51 with both
@@ -32,8 +31,8 @@
 // What bounds it is each CTA's chain: a tile takes 2560 cycles (bf16), of which
 // powers and parts 1300, the maximum 450, waits 450, adding O 320; with two CTAs the
 // tensor cores are busy 59 % of the time, the schedulers 55 %, the exponential unit
-// 40 %. 170 rows x 8 heads over 8192 tokens: 38 us, 340 TFLOP/s of the 4 n d flops
-// that the formula has. (Keys as f16 too, two products for S but twice the parts to
+// 40 %. 173 tokens x 32 query heads over 8192 tokens: 38 us, 305 TFLOP/s of the 4 n d
+// flops that the formula has. (Keys as f16 too, two products for S but twice the parts to
 // make: 46 us. Three bf16 parts for all: 43. One CTA an SM: 2070 cycles a tile
 // against 1300 at two. Half the registers for the softmax, so that a CTA of the other
 // kernel fits beside two: that kernel then spills, 23 -> 30 us.)

@@ -235,6 +235,62 @@ def test_a_captured_call_takes_no_other_sequences_table_entries():
     assert torch.equal(out, again)  # the same tokens, read alike
 
 
+def test_a_captured_step_of_all_operators():
+    """Appends, attention, probabilities and verification in one graph, replayed
+    on new contents: the same as the calls themselves."""
+    g = gen(35)
+    n, hq, hkv, layers, vocab = 5, 8, 2, 3, 1001
+    pool = slmkv.KvPool(num_layers=layers, num_query_heads=hq, num_key_value_heads=hkv, context_length=256,
+                        num_blocks=100, max_sequences=n)
+    caches = [pool.allocate_kv_cache(256) for _ in range(n)]
+    lengths, counts = [30, 16, 1, 100, 64], [3, 1, 4, 2, 2]
+    t = sum(counts)
+    with pool.begin(caches, lengths) as b:
+        for layer in range(layers):
+            b.append_layer(layer, randn(g, sum(lengths), hkv, D), randn(g, sum(lengths), hkv, D))
+    q, k, v, w = randn(g, t, hq, D), randn(g, t, hkv, D), randn(g, t, hkv, D), randn(g, D).abs() + 0.5
+    turned, outs = torch.empty_like(q), [torch.empty_like(q) for _ in range(layers)]
+    logits, temperatures = randn(g, t, vocab), torch.full((t,), 0.8, device="cuda")
+    draft, u = torch.softmax(randn(g, t - n, vocab), -1), torch.rand((t,), generator=g, device="cuda")
+    ids = torch.randint(0, vocab, (t,), generator=g, device="cuda", dtype=torch.int32)
+    p, acc = torch.empty_like(logits), torch.empty(n, dtype=torch.int32, device="cuda")
+    nxt = torch.empty_like(acc)
+
+    def step(b, first):
+        for layer in range(first, layers):
+            b.append_layer_normed(layer, q, k, v, w, w, turned)
+            b.shared_prefix_attention(layer, turned, outs[layer], rotate_query=False)
+        b.token_probabilities(logits, p, temperatures)
+        b.verify_drafts(ids, p, draft, u, acc, nxt)
+
+    def results():
+        return [x.clone() for x in (*outs[1:], p, acc, nxt)]
+
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        b = pool.begin(caches, counts)
+        b.append_layer_normed(0, q, k, v, w, w, turned)
+        b.shared_prefix_attention(0, turned, outs[0], rotate_query=False)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            step(b, 1)
+        for x in (q, k, v, logits):
+            x.copy_(randn(g, *x.shape))
+        graph.replay()
+        graph.replay()
+        got = results()
+        stream.synchronize()
+        del graph
+        assert b.end() == [0] * n
+        pool.truncate_many(caches, lengths)
+        with pool.begin(caches, counts) as b:
+            step(b, 0)
+        want = results()
+    stream.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
 # ---- streams -------------------------------------------------------------------------
 
 
