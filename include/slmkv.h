@@ -261,8 +261,9 @@ slm_status slm_batch_append_layer_normed(slm_batch* batch, int32_t layer, const 
  * 2^-40 of the largest one of its query row or block where that is more, and a
  * softmax weight to 2^-22, or so that its part of the output is off by 2^-38 of
  * the largest that the row has: a weight times the largest value of its block;
- * numbers below 2^-117 to 2^-134; the sum of a row's values, weighted relative
- * to its largest score, has to stay in f32's range). Same arguments; 16-byte
+ * numbers below 2^-117 to 2^-134; a weight below 2^-126 of the largest counts as
+ * 0; the sum of a row's values, weighted relative to its largest score, has to
+ * stay in f32's range). Same arguments; 16-byte
  * aligned buffers that do not overlap. Meant for few new tokens a sequence: long
  * prompts run faster through slm_batch_prefill_attention. A batch's first call plans it for all
  * layers; plan buffers and the joined parts' scratch are allocated by the
